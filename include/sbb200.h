@@ -449,6 +449,63 @@ int sbb_read_raw_u8_images(const char *path, int dtype, void *out, long samples,
  * (first_label = 1). */
 int sbb_read_raw_u8_labels(const char *path, int dtype, void *out, long samples, long classes, long first_label);
 
+/* ------------------------------------------------------------------------
+ * Operators on unit codes.  A code is the position of one active unit in a layer's output (or input): a sample
+ * of `codes_per_row` codes stands for a row with ones there and zeros elsewhere.  All pointers are DEVICE
+ * pointers of the current device; work is queued on `stream`, nothing is allocated, and the calls neither
+ * synchronise nor keep anything between calls: they may be captured into a graph, and run at once on several
+ * streams (with a workspace each).  Element types: SBB_F32, SBB_F64 and, for these calls only, SBB_F16 and
+ * SBB_BF16; sums are held in 32 bits (64 for SBB_F64) and rounded once.  `code_bytes`: 4 (int32) or 8 (int64).
+ * Codes outside [0, N) -- -1 by convention -- name nothing.  Every call gives the same bits for the same
+ * inputs.  No counterpart in the reference, whose layers take dense rows only.
+ * ---------------------------------------------------------------------- */
+#define SBB_F16 2
+#define SBB_BF16 3
+
+/* out[rows, M] = scale * sum over l of weights[codes[row, l], :], weights[N, M]: what weights times the coded
+ * input give. */
+int sbb_lookup(int dtype, const void *weights_dev, const void *codes_dev, int code_bytes, long rows,
+               long codes_per_row, long N, long M, double scale, void *out_dev, void *stream);
+/* Its gradient: out[i, :] = scale * sum of grad[row, :] over the (row, l) with codes[row, l] == i, summed in the
+ * order of the codes; rows that no code names are set to zero.  With `accumulate` the sums are added to what
+ * `out` holds and rows that no code names are left alone.  `workspace`: 16-byte aligned device memory of
+ * sbb_lookup_gradient_workspace() bytes (0: may be null) that nothing else uses until the call's work has ended. */
+size_t sbb_lookup_gradient_workspace(int dtype, long rows, long codes_per_row, long N, long M);
+int sbb_lookup_gradient(int dtype, const void *grad_dev, const void *codes_dev, int code_bytes, long rows,
+                        long codes_per_row, long N, long M, double scale, int accumulate, void *out_dev,
+                        void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* How a unit is drawn.  With w_i = exp((x_i - max) / temperature) and a group's units in order of falling w, equal
+ * ones by their index: the first top_k are kept (all where top_k <= 0), of these the shortest beginning whose sum
+ * reaches top_p times their sum (all where top_p >= 1, at least one), of these the ones with w_i >= min_p (at least
+ * the largest).  temperature <= 0: the largest, the first of equal ones.  A NaN support counts as -infinity; where
+ * the largest is +infinity the units that have it are equally likely and the others out.
+ * `*_rows` (may be null): device arrays with a value per row, used instead of the number beside them. */
+typedef struct sbb_sampling {
+  double temperature, top_p, min_p;
+  long top_k;
+  const float *temperature_rows, *top_p_rows, *min_p_rows;
+  const int *top_k_rows;
+} sbb_sampling;
+/* codes[rows, H] (int64) = h * Mc + the unit drawn from hypercolumn h of support[rows, H * Mc]: the first unit in
+ * index order at which the running sum of the kept w passes random[row, h] times their sum; random[rows, H] in
+ * [0, 1).  -1 where every unit of the hypercolumn is at -infinity.  Weights are formed in 64 bits. */
+int sbb_sample_minicolumns(int dtype, const void *support_dev, const float *random_dev, long rows, long H, long Mc,
+                           const sbb_sampling *how, long long *codes_dev, void *stream);
+
+/* Distillation from the kept units of a teacher.  With p = softmax(teacher / temperature) over a hypercolumn's K
+ * kept units and q = softmax(support / temperature) over all its Mc units:
+ *   loss[row, h] = weight[row] temperature^2 sum_k p_k (log p_k - log q_{unit_k})
+ *   gradient[row, h * Mc + i] = weight[row] temperature (q_i - sum over the k with unit_k == i of p_k),
+ * the derivative of the loss with respect to support[rows, H * Mc].  teacher_units[rows, H, K] counts from 0 within
+ * the hypercolumn (unit_bytes: 4 or 8); entries outside [0, Mc) are absent, a unit named twice has both parts.
+ * teacher[rows, H, K] is of the support's type; loss and weight (null: 1) are float, double for SBB_F64.
+ * gradient may be null: the loss alone; it must not overlap an input.  Where the weight is 0, where no unit is kept,
+ * or where a hypercolumn's support (or the teacher's) is -infinity throughout, both are exactly 0. */
+int sbb_distill(int dtype, const void *support_dev, const void *teacher_units_dev, int unit_bytes,
+                const void *teacher_dev, const void *weight_dev, long rows, long H, long Mc, long K,
+                double temperature, void *loss_dev, void *gradient_dev, void *stream);
+
 /* Measured float64 rates of the current device in TFLOP/s: a register-resident DFMA loop and a loop of the
  * float64 tensor-core instruction (mma.sync.m8n8k4): the denominators of the float64 kernels' roofline, and the
  * evidence for running them on the FP64 pipe (on B200 the two rates are equal).  Synchronises the device.  No

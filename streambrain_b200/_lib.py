@@ -21,6 +21,7 @@ ERR_NAMES = {1: "SBB_ERR_INVALID", 2: "SBB_ERR_CUDA", 3: "SBB_ERR_NO_DEVICE", 4:
              5: "SBB_ERR_TIMEOUT"}
 ERR_INVALID, ERR_CUDA, ERR_NO_DEVICE, ERR_UNSUPPORTED, ERR_TIMEOUT = 1, 2, 3, 4, 5
 F32, F64 = 0, 1
+F16, BF16 = 2, 3   # operators on unit codes only
 SHARD_BUFFERS, SHARD_HANDLE_BYTES = 7, 64
 DENSE, PLASTIC = 0, 1
 STATE = {"weights": 0, "bias": 1, "Ci": 2, "Cj": 3, "Cij": 4, "kbi": 5, "wmask": 6}
@@ -36,6 +37,13 @@ class LayerDesc(ctypes.Structure):
     _fields_ = [("dtype", c_int), ("kind", c_int), ("in_features", c_long), ("hypercolumns", c_long),
                 ("minicolumns", c_long), ("taupdt", c_double), ("khalf", c_double), ("pmin", c_double),
                 ("taubdt", c_double), ("mask_iterations", c_long)]
+
+
+class Sampling(ctypes.Structure):
+    """``sbb_sampling``: how a unit is drawn from a hypercolumn."""
+    _fields_ = [("temperature", c_double), ("top_p", c_double), ("min_p", c_double), ("top_k", c_long),
+                ("temperature_rows", c_void_p), ("top_p_rows", c_void_p), ("min_p_rows", c_void_p),
+                ("top_k_rows", c_void_p)]
 
 
 REDUCE_BEGIN_FN = ctypes.CFUNCTYPE(c_long, c_void_p, c_void_p, c_size_t, c_int, c_void_p)
@@ -129,6 +137,14 @@ SIGNATURES = {
     "sbb_raw_u8_count": (c_int, [c_char_p, POINTER(c_long)]),
     "sbb_read_raw_u8_images": (c_int, [c_char_p, c_int, c_void_p, c_long, c_long]),
     "sbb_read_raw_u8_labels": (c_int, [c_char_p, c_int, c_void_p, c_long, c_long, c_long]),
+    "sbb_lookup": (c_int, [c_int, c_void_p, c_void_p, c_int, c_long, c_long, c_long, c_long, c_double, c_void_p, c_void_p]),
+    "sbb_lookup_gradient_workspace": (c_size_t, [c_int, c_long, c_long, c_long, c_long]),
+    "sbb_lookup_gradient": (c_int, [c_int, c_void_p, c_void_p, c_int, c_long, c_long, c_long, c_long, c_double, c_int,
+                                    c_void_p, c_void_p, c_size_t, c_void_p]),
+    "sbb_sample_minicolumns": (c_int, [c_int, c_void_p, c_void_p, c_long, c_long, c_long, POINTER(Sampling), c_void_p,
+                                       c_void_p]),
+    "sbb_distill": (c_int, [c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_long, c_long, c_long, c_double,
+                            c_void_p, c_void_p, c_void_p]),
     "sbb_measure_fp64_rates": (c_int, [POINTER(c_double), POINTER(c_double)]),
     "sbb_kernel_launches": (c_ulonglong, []),
     "sbb_cta_pair_launches": (c_ulonglong, []),

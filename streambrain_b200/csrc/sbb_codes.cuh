@@ -1,0 +1,87 @@
+// Launch interface of the operators on unit codes (device pointers, asynchronous on the given stream) and the types they
+// share.  Every launcher returns cudaSuccess or the launch error and bumps the process-wide launch counter.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sbb {
+
+void count_launches(int n);   // sbb_kernels.cu
+int sm_count();
+
+// What sums are held in: 32 bits for everything narrower, 64 for double.
+template <typename T>
+struct WideOf {
+  using type = float;
+};
+template <>
+struct WideOf<double> {
+  using type = double;
+};
+template <typename T>
+using Wide = typename WideOf<T>::type;
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ double widen(double v) { return v; }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// The one rounding of a result, to nearest.
+template <typename T>
+__device__ __forceinline__ T narrow_to(Wide<T> v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half narrow_to<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow_to<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// V neighbours, loaded and stored in one access.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+// How many elements one access may hold: 16 bytes where all rows start on such a boundary, two 16-bit elements where they start
+// on one of four bytes (a warp's request is then a whole line), else one.
+template <typename T>
+inline int vector_width(long row_elems, const void *a, const void *b) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (uintptr_t)(row_elems * (long)sizeof(T));
+  if ((bits & 15u) == 0) return 16 / (int)sizeof(T);
+  if (sizeof(T) == 2 && (bits & 3u) == 0) return 2;
+  return 1;
+}
+
+// out[r, :] = scale * sum_l weights[codes[r, l], :]   (weights is [N, M]; codes outside [0, N) name nothing)
+template <typename T, typename I>
+cudaError_t launch_lookup(const T *weights, const I *codes, long rows, long L, long N, long M, double scale, T *out, cudaStream_t st);
+
+// out[i, :] = scale * sum over (r, l) with codes[r, l] == i of grad[r, :], added to what is there with `accumulate`.
+// `workspace`: lookup_gradient_workspace() bytes, 16-byte aligned, free again when the call's work has ended.
+size_t lookup_gradient_workspace(long rows, long L, long N, long M, size_t wide);
+template <typename T, typename I>
+cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, long L, long N, long M, double scale, bool accumulate, T *out,
+                                   void *workspace, cudaStream_t st);
+
+// One unit per (row, group of Mc) drawn from the softmax of support[rows, H * Mc]; codes[rows, H] = h * Mc + unit, or -1.
+struct Sampling {
+  double temperature, top_p, min_p;
+  long top_k;
+  const float *temperature_rows, *top_p_rows, *min_p_rows;   // not null: a value per row in place of the scalar
+  const int *top_k_rows;
+};
+template <typename T>
+cudaError_t launch_sample(const T *support, const float *random, long rows, long H, long Mc, Sampling s, long long *codes, cudaStream_t st);
+
+// loss[rows, H] and (gradient != null) gradient[rows, H * Mc] of the divergence from a teacher's K kept units per group.
+template <typename T, typename I>
+cudaError_t launch_distill(const T *support, const I *units, const T *teacher, const Wide<T> *weight, long rows, long H, long Mc, long K,
+                           double temperature, Wide<T> *loss, T *gradient, cudaStream_t st);
+
+}  // namespace sbb
