@@ -40,29 +40,323 @@ __global__ void __launch_bounds__(kThreads)
   *reinterpret_cast<Vec<T, V> *>(out + r * M + col) = o;
 }
 
-// A warp per weight row: it reads all codes in order and adds the gradient's row for each that names its own.
-template <typename T, typename I>
+// ---- gradient --------------------------------------------------------------
+//
+// The codes are sorted (stably, so that the sums of a weight row run in the order of the samples whatever the schedule), and
+// then every weight row is the sum of a run of the gradient's rows.  Runs may be of any length, so the sorted entries are cut
+// into equal chunks: a chunk writes the runs that lie in it and leaves the part of a run that crosses its border in the
+// workspace, from where join_kernel adds the parts in order.
+
+constexpr unsigned kRankMost = 8192;   // entries that are ranked by comparing all with all
+
+__device__ __forceinline__ unsigned key_of(long code, long N) { return code >= 0 && code < N ? (unsigned)code : (unsigned)N; }
+
+// Sorted position of an entry = the entries with a smaller key + those with the same key in front.  A warp takes four entries;
+// one launch where a radix sort is four.
+template <typename I>
 __global__ void __launch_bounds__(kThreads)
-    gradient_kernel(const T *__restrict__ grad, const I *__restrict__ codes, long entries, long L, long N, long M, Wide<T> scale, bool accumulate,
-                    T *__restrict__ out) {
+    rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, unsigned *__restrict__ key, unsigned *__restrict__ row) {
   after_previous();
-  using W = Wide<T>;
-  const int lane = threadIdx.x & 31;
-  const long i = (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), col = (long)blockIdx.y * 32 + lane;
-  if (i >= N) return;
-  W acc = (W)0;
-  bool any = false;
-  for (long e = 0; e < entries; e += 32) {
-    const bool hit = e + lane < entries && (long)codes[e + lane] == i;
-    for (unsigned m = __ballot_sync(0xffffffffu, hit); m != 0; m &= m - 1) {
-      any = true;
-      if (col < M) acc += widen(grad[(e + __ffs(m) - 1) / L * M + col]);
+  __shared__ uint4 s_key[kRankMost / 4];
+  unsigned *const s = reinterpret_cast<unsigned *>(s_key);
+  const unsigned padded = (entries + 3) & ~3u;
+  for (unsigned i = threadIdx.x; i < padded; i += kThreads) s[i] = i < entries ? key_of((long)codes[i], N) : ~0u;
+  __syncthreads();
+  const unsigned lane = threadIdx.x & 31, e0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 4;
+  if (e0 >= entries) return;
+  const uint4 own = s_key[e0 / 4];
+  const unsigned k[4] = {own.x, own.y, own.z, own.w};
+  unsigned n[4] = {0, 0, 0, 0};
+  for (unsigned j = lane; j < e0 / 4; j += 32) {
+    const uint4 o = s_key[j];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) n[q] += (o.x <= k[q]) + (o.y <= k[q]) + (o.z <= k[q]) + (o.w <= k[q]);
+  }
+  for (unsigned j = e0 / 4 + 1 + lane; j < padded / 4; j += 32) {
+    const uint4 o = s_key[j];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) n[q] += (o.x < k[q]) + (o.y < k[q]) + (o.z < k[q]) + (o.w < k[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    unsigned r = __reduce_add_sync(0xffffffffu, n[q]);
+#pragma unroll
+    for (int o = 0; o < 4; ++o) r += o < q ? k[o] <= k[q] : k[o] < k[q];
+    if (lane == 0 && e0 + q < entries) {
+      key[r] = k[q];
+      row[r] = (e0 + q) / L;
     }
   }
-  if (col >= M || (accumulate && !any)) return;
-  acc *= scale;
-  if (accumulate) acc += widen(out[i * M + col]);
-  out[i * M + col] = narrow_to<T>(acc);
+}
+
+// A pass of a radix sort, least significant digit first: counts of the digits of every tile of entries ...
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
+
+template <typename I, bool FIRST>
+__device__ __forceinline__ unsigned sort_key(const I *codes, const unsigned *key, unsigned i, long N) {
+  return FIRST ? key_of((long)codes[i], N) : key[i];
+}
+
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads)
+    digits_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, unsigned entries, long N, int shift, unsigned tile,
+                  unsigned *__restrict__ counts) {
+  after_previous();
+  __shared__ unsigned s_count[kDigits];
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) s_count[d] = 0;
+  __syncthreads();
+  const unsigned lo = blockIdx.x * tile, hi = min(entries, lo + tile);
+  for (unsigned i = lo + threadIdx.x; i < hi; i += kSortThreads)
+    atomicAdd(&s_count[(sort_key<I, FIRST>(codes, key, i, N) >> shift) & (kDigits - 1)], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[blockIdx.x * kDigits + d] = s_count[d];
+}
+
+// ... and the move: an entry goes behind all smaller digits, the same digit in tiles in front, in the tile's warps in front, and
+// in its own warp in front.
+template <typename I, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads)
+    move_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, const unsigned *__restrict__ row, unsigned entries, unsigned L, long N,
+                int shift, unsigned tile, const unsigned *__restrict__ counts, unsigned *__restrict__ key_to, unsigned *__restrict__ row_to) {
+  after_previous();
+  static_assert(kDigits == kSortThreads, "a thread per digit");
+  __shared__ unsigned s_at[kSortWarps][kDigits];
+  __shared__ unsigned s_warp[kSortWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&s_at[0][0])[i] = 0;
+  __syncthreads();
+  const unsigned each = tile / kSortWarps, lo = blockIdx.x * tile + warp * each, hi = min(entries, lo + each);   // (tile: a multiple of 512)
+  for (unsigned i = lo + lane; i < hi; i += 32) atomicAdd(&s_at[warp][(sort_key<I, FIRST>(codes, key, i, N) >> shift) & (kDigits - 1)], 1u);
+  unsigned all = 0, before = 0;
+#pragma unroll 16
+  for (unsigned b = 0; b < gridDim.x; ++b) {
+    const unsigned c = counts[b * kDigits + threadIdx.x];
+    all += c;
+    before += b < blockIdx.x ? c : 0;
+  }
+  unsigned in = all;
+  for (int off = 1; off < 32; off *= 2) {
+    const unsigned o = __shfl_up_sync(0xffffffffu, in, off);
+    if (lane >= off) in += o;
+  }
+  if (lane == 31) s_warp[warp] = in;
+  __syncthreads();
+  unsigned at = before + in - all;
+  for (int w = 0; w < warp; ++w) at += s_warp[w];
+  for (int w = 0; w < kSortWarps; ++w) {
+    const unsigned c = s_at[w][threadIdx.x];
+    s_at[w][threadIdx.x] = at;
+    at += c;
+  }
+  __syncthreads();
+  for (unsigned i0 = lo; i0 < hi; i0 += 32) {
+    const bool there = i0 + lane < hi;
+    const unsigned kk = there ? sort_key<I, FIRST>(codes, key, i0 + lane, N) : 0;
+    const unsigned digit = there ? (kk >> shift) & (kDigits - 1) : kDigits;
+    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    if (there) {
+      const unsigned to = s_at[warp][digit] + __popc(same & ((1u << lane) - 1));
+      key_to[to] = kk;
+      row_to[to] = FIRST ? (i0 + lane) / L : row[i0 + lane];
+    }
+    __syncwarp();
+    if (there && (same >> lane) == 1u) s_at[warp][digit] += __popc(same);   // the last of its kind
+    __syncwarp();
+  }
+}
+
+template <typename T, int V>
+struct Sums {
+  const T *grad;
+  const unsigned *key, *row;   // sorted; readable up to a multiple of eight
+  unsigned entries, chunk;
+  long N, M;
+  Wide<T> scale;
+  bool accumulate;
+  T *out;
+  Wide<T> *partial;   // [chunk][run from the chunk before, run into the next][M]
+  int lanes;
+  unsigned tiles;     // of `lanes` vectors
+
+  using W = Wide<T>;
+  __device__ __forceinline__ void write(unsigned i, long col, const W (&acc)[V]) const {
+    T *const to = out + (long)i * M + col;
+    Vec<T, V> o;
+    if (accumulate) o = *reinterpret_cast<const Vec<T, V> *>(to);
+#pragma unroll
+    for (int v = 0; v < V; ++v) o.v[v] = narrow_to<T>(accumulate ? acc[v] * scale + widen(o.v[v]) : acc[v] * scale);
+    *reinterpret_cast<Vec<T, V> *>(to) = o;
+  }
+  __device__ __forceinline__ W *part(unsigned c, int which, long col) const { return partial + (2l * c + which) * M + col; }
+};
+
+constexpr int kZeroRows = 64;
+
+// Position of the first key that is not below `k`.
+__device__ __forceinline__ unsigned lower_bound(const unsigned *key, unsigned entries, unsigned k) {
+  unsigned lo = 0, n = entries;
+  while (n > 0) {
+    const unsigned half = n / 2;
+    if (key[lo + half] < k) {
+      lo += half + 1;
+      n -= half + 1;
+    } else {
+      n = half;
+    }
+  }
+  return lo;
+}
+
+// `lanes` threads take a chunk and a tile of columns; the blocks from `sum_blocks` on set rows without a code to zero.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) sums_kernel(const Sums<T, V> p, unsigned sum_blocks) {
+  after_previous();
+  using W = Wide<T>;
+  if (blockIdx.x >= sum_blocks) {
+    __shared__ bool s_absent[kZeroRows];
+    const long n0 = (long)(blockIdx.x - sum_blocks) * kZeroRows;
+    const int rows = (int)min((long)kZeroRows, p.N - n0);
+    if ((int)threadIdx.x < rows) {
+      const unsigned n = (unsigned)n0 + threadIdx.x, at = lower_bound(p.key, p.entries, n);
+      s_absent[threadIdx.x] = at >= p.entries || p.key[at] != n;
+    }
+    __syncthreads();
+    Vec<T, V> zero;
+#pragma unroll
+    for (int v = 0; v < V; ++v) zero.v[v] = narrow_to<T>((W)0);
+    const long across = p.M / V;
+    long r = threadIdx.x / across, c = threadIdx.x % across;
+    const long dr = kThreads / across, dc = kThreads % across;
+    while (r < rows) {
+      if (s_absent[r]) *reinterpret_cast<Vec<T, V> *>(p.out + (n0 + r) * p.M + c * V) = zero;
+      r += dr;
+      c += dc;
+      if (c >= across) c -= across, ++r;
+    }
+    return;
+  }
+  const unsigned g = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes, c = g / p.tiles;
+  const long col = ((long)(g % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
+  const unsigned b = c * p.chunk, e = min(p.entries, b + p.chunk);
+  if (c >= (p.entries + p.chunk - 1) / p.chunk || col >= p.M) return;
+  W acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = (W)0;
+  unsigned cur = p.key[b];
+  bool head = b > 0 && p.key[b - 1] == cur;
+  auto flush = [&](int which) {   // 2: the run lies in the chunk
+    if (cur >= (unsigned)p.N) return;
+    if (which == 2) {
+      p.write(cur, col, acc);
+    } else {
+      W *const to = p.part(c, which, col);
+#pragma unroll
+      for (int v = 0; v < V; ++v) to[v] = acc[v];
+    }
+  };
+  constexpr int U = 8;
+  for (unsigned i = b; i < e; i += U) {
+    unsigned k[U], r[U];
+    Vec<T, V> x[U];
+    *reinterpret_cast<uint4 *>(k) = *reinterpret_cast<const uint4 *>(p.key + i);
+    *reinterpret_cast<uint4 *>(k + 4) = *reinterpret_cast<const uint4 *>(p.key + i + 4);
+    *reinterpret_cast<uint4 *>(r) = *reinterpret_cast<const uint4 *>(p.row + i);
+    *reinterpret_cast<uint4 *>(r + 4) = *reinterpret_cast<const uint4 *>(p.row + i + 4);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i + u < e && k[u] < (unsigned)p.N) x[u] = *reinterpret_cast<const Vec<T, V> *>(p.grad + (long)r[u] * p.M + col);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= e) break;
+      if (k[u] != cur) {
+        flush(head ? 0 : 2);
+        cur = k[u];
+        head = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = (W)0;
+      }
+      if (cur < (unsigned)p.N)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] += widen(x[u].v[v]);
+    }
+  }
+  flush(head ? 0 : e < p.entries && p.key[e] == cur ? 1 : 2);
+}
+
+// Adds the parts of the runs that cross the end of a chunk and begin in it.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
+  after_previous();
+  using W = Wide<T>;
+  const unsigned g = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes, c = g / p.tiles;
+  const long col = ((long)(g % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
+  const unsigned b = c * p.chunk, e = b + p.chunk;
+  if (c >= (p.entries + p.chunk - 1) / p.chunk || e >= p.entries || col >= p.M) return;
+  const unsigned cur = p.key[e - 1];
+  if (p.key[e] != cur || cur >= (unsigned)p.N || (b > 0 && p.key[b] == cur && p.key[b - 1] == cur)) return;
+  const unsigned last = (lower_bound(p.key, p.entries, cur + 1) - 1) / p.chunk;
+  W acc[V];
+  const W *const from = p.part(c, 1, col);
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = from[v];
+#pragma unroll 8
+  for (unsigned q = c + 1; q <= last; ++q) {
+    const W *const more = p.part(q, 0, col);
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] += more[v];
+  }
+  p.write(cur, col, acc);
+}
+
+// Sizes of a gradient call.
+struct GradientPlan {
+  unsigned entries, chunk, chunks;
+  bool rank;
+  unsigned tile, blocks;   // of the sort's passes
+  int passes;
+  size_t padded, counts, partial;   // elements: a key or row array, the digits' counts, the parts of runs
+};
+GradientPlan gradient_plan(long rows, long L, long N, long M) {
+  GradientPlan p = {};
+  p.entries = (unsigned)(rows * L);
+  p.rank = p.entries <= kRankMost;
+  // as many chunks as keep all threads busy with a vector of 16 bytes each, of 8 to 64 entries
+  const long want = 2048l * sm_count() * 4;
+  long chunk = (long)p.entries * M / want / 8 * 8;
+  chunk = chunk < 8 ? 8 : chunk > 64 ? 64 : chunk;
+  p.chunk = (unsigned)chunk;
+  p.chunks = (p.entries + p.chunk - 1) / p.chunk;
+  p.padded = ((size_t)p.entries + 7) / 8 * 8;
+  p.partial = p.chunks > 1 ? 2 * (size_t)p.chunks * (size_t)M : 0;
+  if (!p.rank) {
+    int bits = 1;
+    while (bits < 32 && (N >> bits) != 0) ++bits;   // N stands for codes that name nothing
+    p.passes = (bits + kDigitBits - 1) / kDigitBits;
+    // up to 128 tiles: every block of a pass reads the counts of all
+    p.tile = ((p.entries + 127) / 128 + kSortThreads - 1) / kSortThreads * kSortThreads;
+    if (p.tile < 1024) p.tile = 1024;
+    p.blocks = (p.entries + p.tile - 1) / p.tile;
+    p.counts = (size_t)p.blocks * kDigits;
+  }
+  return p;
+}
+
+template <typename T, int V>
+cudaError_t launch_sums(Sums<T, V> p, unsigned chunks, cudaStream_t st) {
+  const long across = p.M / V;
+  p.lanes = 4;
+  while (p.lanes < 32 && p.lanes < across) p.lanes *= 2;
+  p.tiles = (unsigned)((across + p.lanes - 1) / p.lanes);
+  const unsigned per = kThreads / p.lanes;
+  const size_t blocks = ((size_t)chunks * p.tiles + per - 1) / per, zero = p.accumulate ? 0 : ((size_t)p.N + kZeroRows - 1) / kZeroRows;
+  if (blocks + zero > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  cudaError_t e = launch_next(sums_kernel<T, V>, dim3((unsigned)(blocks + zero)), kThreads, 0, st, p, (unsigned)blocks);
+  if (e != cudaSuccess) return e;
+  count_launches(1);
+  if (chunks == 1) return e;
+  e = launch_next(join_kernel<T, V>, dim3((unsigned)blocks), kThreads, 0, st, p);
+  if (e == cudaSuccess) count_launches(1);
+  return e;
 }
 
 }  // namespace
@@ -86,15 +380,48 @@ cudaError_t launch_lookup(const T *weights, const I *codes, long rows, long L, l
   return e;
 }
 
-size_t lookup_gradient_workspace(long, long, long, long, size_t) { return 0; }
+size_t lookup_gradient_workspace(long rows, long L, long N, long M, size_t wide) {
+  const GradientPlan p = gradient_plan(rows, L, N, M);
+  return ((p.rank ? 2 : 4) * p.padded + p.counts) * sizeof(unsigned) + 16 + p.partial * wide;
+}
 
 template <typename T, typename I>
 cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, long L, long N, long M, double scale, bool accumulate, T *out,
-                                   void *, cudaStream_t st) {
-  const dim3 grid((unsigned)((N + kThreads / 32 - 1) / (kThreads / 32)), (unsigned)((M + 31) / 32));
-  const cudaError_t e = launch_next(gradient_kernel<T, I>, grid, kThreads, 0, st, grad, codes, rows * L, L, N, M, (Wide<T>)scale, accumulate, out);
-  if (e == cudaSuccess) count_launches(1);
-  return e;
+                                   void *workspace, cudaStream_t st) {
+  const GradientPlan p = gradient_plan(rows, L, N, M);
+  unsigned *key = static_cast<unsigned *>(workspace), *row = key + p.padded, *end = row + p.padded;
+  cudaError_t e;
+  if (p.rank) {
+    e = launch_next(rank_kernel<I>, dim3((p.entries + kThreads / 8 - 1) / (kThreads / 8)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, key, row);
+    if (e != cudaSuccess) return e;
+    count_launches(1);
+  } else {
+    unsigned *key2 = end, *row2 = key2 + p.padded, *counts = row2 + p.padded;
+    end = counts + p.counts;
+    for (int pass = 0; pass < p.passes; ++pass) {
+      const int shift = pass * kDigitBits;
+      const bool first = pass == 0;
+      e = first ? launch_next(digits_kernel<I, true>, dim3(p.blocks), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts)
+                : launch_next(digits_kernel<I, false>, dim3(p.blocks), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts);
+      if (e != cudaSuccess) return e;
+      e = first ? launch_next(move_kernel<I, true>, dim3(p.blocks), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile,
+                              counts, key2, row2)
+                : launch_next(move_kernel<I, false>, dim3(p.blocks), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile,
+                              counts, key2, row2);
+      if (e != cudaSuccess) return e;
+      count_launches(2);
+      unsigned *const k = key, *const r = row;
+      key = key2, row = row2, key2 = k, row2 = r;
+    }
+  }
+  Wide<T> *const partial = reinterpret_cast<Wide<T> *>((reinterpret_cast<uintptr_t>(end) + 15) / 16 * 16);
+  const int vec = vector_width<T>(M, grad, out);
+  const Wide<T> s = (Wide<T>)scale;
+  constexpr int V = 16 / (int)sizeof(T);
+  if (vec == V) return launch_sums(Sums<T, V>{grad, key, row, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 2) return launch_sums(Sums<T, 2>{grad, key, row, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+  return launch_sums(Sums<T, 1>{grad, key, row, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
 }
 
 #define SBB_INSTANCE(T, I)                                                                                              \
