@@ -51,16 +51,27 @@ constexpr unsigned kRankMost = 8192;   // entries that are ranked by comparing a
 
 __device__ __forceinline__ unsigned key_of(long code, long N) { return code >= 0 && code < N ? (unsigned)code : (unsigned)N; }
 
+// a < b for numbers of up to 2^31 (the difference's sign: an instruction less than a comparison and a choice)
+__device__ __forceinline__ unsigned below(unsigned a, unsigned b) { return (a - b) >> 31; }
+
 // Sorted position of an entry = the entries with a smaller key + those with the same key in front.  A warp takes four entries;
 // one launch where a radix sort is four.
 template <typename I>
 __global__ void __launch_bounds__(kThreads)
-    rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, unsigned *__restrict__ key, unsigned *__restrict__ row) {
+    rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, unsigned *__restrict__ key, unsigned *__restrict__ row,
+                unsigned *__restrict__ some) {
   after_previous();
   __shared__ uint4 s_key[kRankMost / 4];
   unsigned *const s = reinterpret_cast<unsigned *>(s_key);
   const unsigned padded = (entries + 3) & ~3u;
-  for (unsigned i = threadIdx.x; i < padded; i += kThreads) s[i] = i < entries ? key_of((long)codes[i], N) : ~0u;
+  for (unsigned i0 = threadIdx.x; i0 < padded; i0 += 8 * kThreads) {   // (eight loads in flight: one by one the 30 KB took 8 us)
+    long c[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) c[u] = i0 + u * kThreads < entries ? (long)codes[i0 + u * kThreads] : -1;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (i0 + u * kThreads < padded) s[i0 + u * kThreads] = i0 + u * kThreads < entries ? key_of(c[u], N) : 0x7fffffffu;
+  }
   __syncthreads();
   const unsigned lane = threadIdx.x & 31, e0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 4;
   if (e0 >= entries) return;
@@ -70,12 +81,12 @@ __global__ void __launch_bounds__(kThreads)
   for (unsigned j = lane; j < e0 / 4; j += 32) {
     const uint4 o = s_key[j];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) n[q] += (o.x <= k[q]) + (o.y <= k[q]) + (o.z <= k[q]) + (o.w <= k[q]);
+    for (int q = 0; q < 4; ++q) n[q] += below(o.x, k[q] + 1) + below(o.y, k[q] + 1) + below(o.z, k[q] + 1) + below(o.w, k[q] + 1);
   }
   for (unsigned j = e0 / 4 + 1 + lane; j < padded / 4; j += 32) {
     const uint4 o = s_key[j];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) n[q] += (o.x < k[q]) + (o.y < k[q]) + (o.z < k[q]) + (o.w < k[q]);
+    for (int q = 0; q < 4; ++q) n[q] += below(o.x, k[q]) + below(o.y, k[q]) + below(o.z, k[q]) + below(o.w, k[q]);
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -85,6 +96,7 @@ __global__ void __launch_bounds__(kThreads)
     if (lane == 0 && e0 + q < entries) {
       key[r] = k[q];
       row[r] = (e0 + q) / L;
+      if (some != nullptr && k[q] < (unsigned)N) some[k[q]] = r;
     }
   }
 }
@@ -117,7 +129,8 @@ __global__ void __launch_bounds__(kSortThreads)
 template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
     move_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, const unsigned *__restrict__ row, unsigned entries, unsigned L, long N,
-                int shift, unsigned tile, const unsigned *__restrict__ counts, unsigned *__restrict__ key_to, unsigned *__restrict__ row_to) {
+                int shift, unsigned tile, const unsigned *__restrict__ counts, unsigned *__restrict__ key_to, unsigned *__restrict__ row_to,
+                unsigned *__restrict__ some) {
   after_previous();
   static_assert(kDigits == kSortThreads, "a thread per digit");
   __shared__ unsigned s_at[kSortWarps][kDigits];
@@ -158,6 +171,7 @@ __global__ void __launch_bounds__(kSortThreads)
       const unsigned to = s_at[warp][digit] + __popc(same & ((1u << lane) - 1));
       key_to[to] = kk;
       row_to[to] = FIRST ? (i0 + lane) / L : row[i0 + lane];
+      if (some != nullptr && kk < (unsigned)N) some[kk] = to;
     }
     __syncwarp();
     if (there && (same >> lane) == 1u) s_at[warp][digit] += __popc(same);   // the last of its kind
@@ -168,7 +182,8 @@ __global__ void __launch_bounds__(kSortThreads)
 template <typename T, int V>
 struct Sums {
   const T *grad;
-  const unsigned *key, *row;   // sorted; readable up to a multiple of eight
+  const unsigned *key, *row;   // sorted
+  const unsigned *some;        // per weight row: the position of a code that names it, or anything where none does
   unsigned entries, chunk;
   long N, M;
   Wide<T> scale;
@@ -177,6 +192,7 @@ struct Sums {
   Wide<T> *partial;   // [chunk][run from the chunk before, run into the next][M]
   int lanes;
   unsigned tiles;     // of `lanes` vectors
+  int zero_rows;      // of a block
 
   using W = Wide<T>;
   __device__ __forceinline__ void write(unsigned i, long col, const W (&acc)[V]) const {
@@ -190,62 +206,62 @@ struct Sums {
   __device__ __forceinline__ W *part(unsigned c, int which, long col) const { return partial + (2l * c + which) * M + col; }
 };
 
-constexpr int kZeroRows = 64;
+constexpr int kZeroRows = 128;   // most rows of a block that sets rows to zero
 
-// Position of the first key that is not below `k`.
-__device__ __forceinline__ unsigned lower_bound(const unsigned *key, unsigned entries, unsigned k) {
-  unsigned lo = 0, n = entries;
-  while (n > 0) {
-    const unsigned half = n / 2;
-    if (key[lo + half] < k) {
-      lo += half + 1;
-      n -= half + 1;
-    } else {
-      n = half;
-    }
-  }
-  return lo;
-}
-
-// `lanes` threads take a chunk and a tile of columns; the blocks from `sum_blocks` on set rows without a code to zero.
+// `lanes` threads take a chunk and a tile of columns.  Among the `sum_blocks` blocks that do so lie `zero_blocks` that set rows
+// without a code to zero, evenly, so that memory is read and written at the same time.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) sums_kernel(const Sums<T, V> p, unsigned sum_blocks) {
+__global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p, unsigned sum_blocks, unsigned zero_blocks) {
   after_previous();
   using W = Wide<T>;
-  if (blockIdx.x >= sum_blocks) {
+  const unsigned zero_before = (unsigned)((unsigned long long)blockIdx.x * zero_blocks / gridDim.x);
+  if ((unsigned)((unsigned long long)(blockIdx.x + 1) * zero_blocks / gridDim.x) != zero_before) {
     __shared__ bool s_absent[kZeroRows];
-    const long n0 = (long)(blockIdx.x - sum_blocks) * kZeroRows;
-    const int rows = (int)min((long)kZeroRows, p.N - n0);
+    const long n0 = (long)zero_before * p.zero_rows;
+    const int rows = (int)min((long)p.zero_rows, p.N - n0);
     if ((int)threadIdx.x < rows) {
-      const unsigned n = (unsigned)n0 + threadIdx.x, at = lower_bound(p.key, p.entries, n);
+      const unsigned n = (unsigned)n0 + threadIdx.x, at = p.some[n];   // (nothing has written it where no code names the row)
       s_absent[threadIdx.x] = at >= p.entries || p.key[at] != n;
     }
     __syncthreads();
     Vec<T, V> zero;
 #pragma unroll
     for (int v = 0; v < V; ++v) zero.v[v] = narrow_to<T>((W)0);
-    const long across = p.M / V;
-    long r = threadIdx.x / across, c = threadIdx.x % across;
-    const long dr = kThreads / across, dc = kThreads % across;
-    while (r < rows) {
-      if (s_absent[r]) *reinterpret_cast<Vec<T, V> *>(p.out + (n0 + r) * p.M + c * V) = zero;
+    const unsigned across = (unsigned)(p.M / V);
+    unsigned r = threadIdx.x / across, c = threadIdx.x % across;
+    const unsigned dr = kThreads / across, dc = kThreads % across;
+    while ((int)r < rows) {
+      if (s_absent[r]) *reinterpret_cast<Vec<T, V> *>(p.out + (n0 + r) * p.M + (long)c * V) = zero;
       r += dr;
       c += dc;
       if (c >= across) c -= across, ++r;
     }
     return;
   }
-  const unsigned g = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes, c = g / p.tiles;
+  // the block's sorted entries, with one more at either end
+  extern __shared__ unsigned s_entry[];
+  const unsigned groups = kThreads / p.lanes, g0 = (blockIdx.x - zero_before) * groups, g = g0 + threadIdx.x / p.lanes, c = g / p.tiles;
+  const unsigned first = g0 / p.tiles * p.chunk, end = min(p.entries, ((g0 + groups - 1) / p.tiles + 1) * p.chunk), size = end > first ? end - first : 0;
+  unsigned *const s_key = s_entry + 1, *const s_row = s_entry + size + 2;
+  for (unsigned i = threadIdx.x; i < size + 2; i += kThreads) {
+    const unsigned at = first + i - 1;   // (wraps below zero)
+    s_entry[i] = at < p.entries ? p.key[at] : ~0u;
+  }
+  for (unsigned i = threadIdx.x; i < size; i += kThreads) s_row[i] = p.row[first + i];
+  __syncthreads();
   const long col = ((long)(g % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
   const unsigned b = c * p.chunk, e = min(p.entries, b + p.chunk);
-  if (c >= (p.entries + p.chunk - 1) / p.chunk || col >= p.M) return;
+  if (b >= p.entries || col >= p.M) return;
   W acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = (W)0;
-  unsigned cur = p.key[b];
-  bool head = b > 0 && p.key[b - 1] == cur;
+  const unsigned *key = s_key + (b - first), *row = s_row + (b - first);
+  unsigned n = e - b;
+  while (n > 0 && key[n - 1] >= (unsigned)p.N) --n;   // codes that name nothing are the last ones
+  if (n == 0) return;
+  unsigned cur = key[0];
+  bool head = s_entry[b - first] == cur;
   auto flush = [&](int which) {   // 2: the run lies in the chunk
-    if (cur >= (unsigned)p.N) return;
     if (which == 2) {
       p.write(cur, col, acc);
     } else {
@@ -254,58 +270,106 @@ __global__ void __launch_bounds__(kThreads) sums_kernel(const Sums<T, V> p, unsi
       for (int v = 0; v < V; ++v) to[v] = acc[v];
     }
   };
-  constexpr int U = 8;
-  for (unsigned i = b; i < e; i += U) {
-    unsigned k[U], r[U];
+  // Four loads without conditions in flight, four blocks on an SM.  65536 rows of 1024 bf16 elements, us a call: with conditions
+  // between the loads 117, eight loads and three blocks 78, two pairs of four in turn 79 to 90 (registers), this 79.
+  constexpr int U = 4;
+  const T *const from = p.grad + col;
+  for (unsigned i = 0; i < n; i += U) {
     Vec<T, V> x[U];
-    *reinterpret_cast<uint4 *>(k) = *reinterpret_cast<const uint4 *>(p.key + i);
-    *reinterpret_cast<uint4 *>(k + 4) = *reinterpret_cast<const uint4 *>(p.key + i + 4);
-    *reinterpret_cast<uint4 *>(r) = *reinterpret_cast<const uint4 *>(p.row + i);
-    *reinterpret_cast<uint4 *>(r + 4) = *reinterpret_cast<const uint4 *>(p.row + i + 4);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (i + u < e && k[u] < (unsigned)p.N) x[u] = *reinterpret_cast<const Vec<T, V> *>(p.grad + (long)r[u] * p.M + col);
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Vec<T, V> *>(from + (long)row[min(i + u, n - 1)] * p.M);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (i + u >= e) break;
-      if (k[u] != cur) {
+      if (i + u >= n) break;
+      const unsigned k = key[i + u];
+      if (k != cur) {
         flush(head ? 0 : 2);
-        cur = k[u];
+        cur = k;
         head = false;
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = (W)0;
       }
-      if (cur < (unsigned)p.N)
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += widen(x[u].v[v]);
+      for (int v = 0; v < V; ++v) acc[v] += widen(x[u].v[v]);
     }
   }
-  flush(head ? 0 : e < p.entries && p.key[e] == cur ? 1 : 2);
+  flush(head ? 0 : key[n] == cur ? 1 : 2);
 }
 
-// Adds the parts of the runs that cross the end of a chunk and begin in it.
+// Adds the parts of the runs that cross the end of a chunk and begin in it: a group of `lanes` threads for each chunk and tile
+// of columns, all groups of the block together for runs of many parts (of which a block, with chunks that follow one another,
+// has few).
+constexpr unsigned kLongRun = 32;
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
   after_previous();
   using W = Wide<T>;
-  const unsigned g = blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes, c = g / p.tiles;
-  const long col = ((long)(g % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
-  const unsigned b = c * p.chunk, e = b + p.chunk;
-  if (c >= (p.entries + p.chunk - 1) / p.chunk || e >= p.entries || col >= p.M) return;
-  const unsigned cur = p.key[e - 1];
-  if (p.key[e] != cur || cur >= (unsigned)p.N || (b > 0 && p.key[b] == cur && p.key[b - 1] == cur)) return;
-  const unsigned last = (lower_bound(p.key, p.entries, cur + 1) - 1) / p.chunk;
-  W acc[V];
-  const W *const from = p.part(c, 1, col);
+  __shared__ unsigned s_last[kThreads / 4];   // of each group's run, 0: none or short
+  __shared__ W s_sum[kThreads * V];
+  const unsigned groups = kThreads / p.lanes, own = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
+  const unsigned chunks = (p.entries + p.chunk - 1) / p.chunk;
+  auto sum = [&](W(&acc)[V], unsigned from, unsigned to, unsigned step, long col) {   // parts [from, to], four in flight
+    for (; from <= to; from += 4 * step) {
+      Vec<W, V> x[4];
 #pragma unroll
-  for (int v = 0; v < V; ++v) acc[v] = from[v];
-#pragma unroll 8
-  for (unsigned q = c + 1; q <= last; ++q) {
-    const W *const more = p.part(q, 0, col);
+      for (int u = 0; u < 4; ++u)
+        if (from + u * step <= to) x[u] = *reinterpret_cast<const Vec<W, V> *>(p.part(from + u * step, 0, col));
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] += more[v];
+      for (int u = 0; u < 4; ++u)
+        if (from + u * step <= to)
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[v] += x[u].v[v];
+    }
+  };
+  const unsigned blocks = (chunks + groups - 1) / groups, c0 = blockIdx.x % blocks * groups, c = c0 + own;
+  const long col = ((long)(blockIdx.x / blocks) * p.lanes + lane) * V;
+  unsigned cur = 0, last = 0;
+  if (c + 1 < chunks) {
+    const unsigned b = c * p.chunk, e = b + p.chunk;
+    cur = p.key[e - 1];
+    if (p.key[e] == cur && cur < (unsigned)p.N && !(b > 0 && p.key[b] == cur && p.key[b - 1] == cur)) {
+      // the last chunk that begins inside the run: the group's threads try that many places at a time
+      last = c + 1;
+      unsigned end = chunks;
+      const unsigned mask = (p.lanes == 32 ? ~0u : (1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
+      for (unsigned step = 1; last + 1 < end; step = (end - last - 1 + p.lanes - 1) / p.lanes) {   // first the chunks that follow
+        const unsigned at = last + (lane + 1) * step;
+        const int in = __popc(__ballot_sync(mask, at < end && p.key[at * p.chunk] == cur));
+        last += in * step;
+        if (in < p.lanes) end = min(end, last + step);
+      }
+    }
   }
-  p.write(cur, col, acc);
+  if (lane == 0) s_last[own] = last > c + kLongRun ? last : 0;
+  W acc[V];
+  if (last > 0 && col < p.M) {
+    const W *const from = p.part(c, 1, col);
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = from[v];
+    if (last <= c + kLongRun) {
+      sum(acc, c + 1, last, 1, col);
+      p.write(cur, col, acc);
+    }
+  }
+  __syncthreads();
+  for (unsigned q = 0; q < groups; ++q) {
+    const unsigned to = s_last[q];
+    if (to == 0) continue;
+    W part[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) part[v] = (W)0;
+    if (col < p.M) sum(part, c0 + q + 1 + own, to, groups, col);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_sum[threadIdx.x * V + v] = part[v];
+    __syncthreads();
+    if (own == q && col < p.M) {
+      for (unsigned o = 0; o < groups; ++o)
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] += s_sum[(o * p.lanes + lane) * V + v];
+      p.write(cur, col, acc);
+    }
+    __syncthreads();
+  }
 }
 
 // Sizes of a gradient call.
@@ -314,7 +378,7 @@ struct GradientPlan {
   bool rank;
   unsigned tile, blocks;   // of the sort's passes
   int passes;
-  size_t padded, counts, partial;   // elements: a key or row array, the digits' counts, the parts of runs
+  size_t padded, counts, some, partial;   // elements: a key or row array, the digits' counts, a position per row, the parts of runs
 };
 GradientPlan gradient_plan(long rows, long L, long N, long M) {
   GradientPlan p = {};
@@ -327,6 +391,7 @@ GradientPlan gradient_plan(long rows, long L, long N, long M) {
   p.chunk = (unsigned)chunk;
   p.chunks = (p.entries + p.chunk - 1) / p.chunk;
   p.padded = ((size_t)p.entries + 7) / 8 * 8;
+  p.some = ((size_t)N + 7) / 8 * 8;
   p.partial = p.chunks > 1 ? 2 * (size_t)p.chunks * (size_t)M : 0;
   if (!p.rank) {
     int bits = 1;
@@ -348,13 +413,17 @@ cudaError_t launch_sums(Sums<T, V> p, unsigned chunks, cudaStream_t st) {
   while (p.lanes < 32 && p.lanes < across) p.lanes *= 2;
   p.tiles = (unsigned)((across + p.lanes - 1) / p.lanes);
   const unsigned per = kThreads / p.lanes;
-  const size_t blocks = ((size_t)chunks * p.tiles + per - 1) / per, zero = p.accumulate ? 0 : ((size_t)p.N + kZeroRows - 1) / kZeroRows;
+  const long zero_rows = 32768 / (p.M * (long)sizeof(T));   // 32 KB a block
+  p.zero_rows = (int)(zero_rows < 1 ? 1 : zero_rows > kZeroRows ? kZeroRows : zero_rows);
+  const size_t blocks = ((size_t)chunks * p.tiles + per - 1) / per, zero = p.accumulate ? 0 : ((size_t)p.N + p.zero_rows - 1) / p.zero_rows;
   if (blocks + zero > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  cudaError_t e = launch_next(sums_kernel<T, V>, dim3((unsigned)(blocks + zero)), kThreads, 0, st, p, (unsigned)blocks);
+  const size_t smem = (2 * ((per + p.tiles - 1) / p.tiles + 1) * (size_t)p.chunk + 2) * sizeof(unsigned);
+  cudaError_t e = launch_next(sums_kernel<T, V>, dim3((unsigned)(blocks + zero)), kThreads, smem, st, p, (unsigned)blocks, (unsigned)zero);
   if (e != cudaSuccess) return e;
   count_launches(1);
   if (chunks == 1) return e;
-  e = launch_next(join_kernel<T, V>, dim3((unsigned)blocks), kThreads, 0, st, p);
+  const size_t join = (((size_t)chunks + per - 1) / per) * p.tiles;
+  e = launch_next(join_kernel<T, V>, dim3((unsigned)join), kThreads, 0, st, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
@@ -382,17 +451,17 @@ cudaError_t launch_lookup(const T *weights, const I *codes, long rows, long L, l
 
 size_t lookup_gradient_workspace(long rows, long L, long N, long M, size_t wide) {
   const GradientPlan p = gradient_plan(rows, L, N, M);
-  return ((p.rank ? 2 : 4) * p.padded + p.counts) * sizeof(unsigned) + 16 + p.partial * wide;
+  return ((p.rank ? 2 : 4) * p.padded + p.counts + p.some) * sizeof(unsigned) + 64 + p.partial * wide;
 }
 
 template <typename T, typename I>
 cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, long L, long N, long M, double scale, bool accumulate, T *out,
                                    void *workspace, cudaStream_t st) {
   const GradientPlan p = gradient_plan(rows, L, N, M);
-  unsigned *key = static_cast<unsigned *>(workspace), *row = key + p.padded, *end = row + p.padded;
+  unsigned *key = static_cast<unsigned *>(workspace), *row = key + p.padded, *const some = accumulate ? nullptr : row + p.padded, *end = row + p.padded + p.some;
   cudaError_t e;
   if (p.rank) {
-    e = launch_next(rank_kernel<I>, dim3((p.entries + kThreads / 8 - 1) / (kThreads / 8)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, key, row);
+    e = launch_next(rank_kernel<I>, dim3((p.entries + kThreads / 8 - 1) / (kThreads / 8)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, key, row, some);
     if (e != cudaSuccess) return e;
     count_launches(1);
   } else {
@@ -401,27 +470,28 @@ cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, lon
     for (int pass = 0; pass < p.passes; ++pass) {
       const int shift = pass * kDigitBits;
       const bool first = pass == 0;
+      unsigned *const last = pass + 1 == p.passes ? some : nullptr;
       e = first ? launch_next(digits_kernel<I, true>, dim3(p.blocks), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts)
                 : launch_next(digits_kernel<I, false>, dim3(p.blocks), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts);
       if (e != cudaSuccess) return e;
       e = first ? launch_next(move_kernel<I, true>, dim3(p.blocks), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile,
-                              counts, key2, row2)
+                              counts, key2, row2, last)
                 : launch_next(move_kernel<I, false>, dim3(p.blocks), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile,
-                              counts, key2, row2);
+                              counts, key2, row2, last);
       if (e != cudaSuccess) return e;
       count_launches(2);
       unsigned *const k = key, *const r = row;
       key = key2, row = row2, key2 = k, row2 = r;
     }
   }
-  Wide<T> *const partial = reinterpret_cast<Wide<T> *>((reinterpret_cast<uintptr_t>(end) + 15) / 16 * 16);
+  Wide<T> *const partial = reinterpret_cast<Wide<T> *>((reinterpret_cast<uintptr_t>(end) + 63) / 64 * 64);   // (read 32 bytes at a time)
   const int vec = vector_width<T>(M, grad, out);
   const Wide<T> s = (Wide<T>)scale;
   constexpr int V = 16 / (int)sizeof(T);
-  if (vec == V) return launch_sums(Sums<T, V>{grad, key, row, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+  if (vec == V) return launch_sums(Sums<T, V>{grad, key, row, some, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
   if constexpr (sizeof(T) == 2)
-    if (vec == 2) return launch_sums(Sums<T, 2>{grad, key, row, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
-  return launch_sums(Sums<T, 1>{grad, key, row, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+    if (vec == 2) return launch_sums(Sums<T, 2>{grad, key, row, some, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+  return launch_sums(Sums<T, 1>{grad, key, row, some, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
 }
 
 #define SBB_INSTANCE(T, I)                                                                                              \
