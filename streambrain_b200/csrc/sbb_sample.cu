@@ -1,14 +1,20 @@
 // Drawing a unit of every group from the softmax of its support, with temperature, top-k, top-p and min-p, from given numbers.
 //
 // With w_i = exp((x_i - max) / t) and the units in order of falling w (equal ones: lowest index first), top-k, top-p and min-p
-// each keep a beginning of that order, so what is kept is all units not behind one (value, index).  Finding that unit takes no
-// sort: a histogram of counts and masses over the values' bits says which bin it lies in, and the bin is cut again until few
-// units are left, which are compared with one another.
+// each keep a beginning of that order, so what is kept is all units not behind one (value, index): a cut.  Finding it takes no
+// sort of the group: counts and masses over parts of the values' range say in which part it lies, and the few units of that part
+// are compared with one another.
 // A random number may lie next to the border of two units, and of a million draws some do within 32 bits' accuracy.  So weights
 // are formed in 64 bits and summed as integers, multiples of 2^-q: the sums are the same in any order and their errors below
 // n 2^-q of the largest weight.
+// Groups of up to 512 units are a warp's, in its registers; wider ones a cluster's of blocks, each with a part of the group in
+// shared memory, so that the support is read from memory once.
 #include "sbb_codes.cuh"
 #include "sbb_launch.cuh"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
 
 namespace sbb {
 namespace {
@@ -25,6 +31,7 @@ struct Keys<float> {
     const unsigned b = __float_as_uint(v + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
   }
+  static __device__ __forceinline__ float value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 };
 template <>
 struct Keys<double> {
@@ -33,6 +40,7 @@ struct Keys<double> {
     const u64 b = (u64)__double_as_longlong(v + 0.0);
     return b >> 63 ? ~b : b | (1ull << 63);
   }
+  static __device__ __forceinline__ double value(u64 k) { return __longlong_as_double((long long)(k >> 63 ? k ^ (1ull << 63) : ~k)); }
 };
 template <typename W>
 __device__ __forceinline__ W no_nan(W v) {
@@ -41,300 +49,798 @@ __device__ __forceinline__ W no_nan(W v) {
 
 struct Settings {
   double inv_t, top_p, min_p;
-  long top_k;   // n: all
+  unsigned top_k;   // n: all
 };
-__device__ __forceinline__ Settings settings_of(const Sampling &s, long row, long n) {
+__device__ __forceinline__ Settings settings_of(const Sampling &s, long row, unsigned n) {
   const double t = s.temperature_rows ? (double)s.temperature_rows[row] : s.temperature;
+  const long k = s.top_k_rows ? (long)s.top_k_rows[row] : s.top_k;
   Settings r;
-  r.top_k = s.top_k_rows ? (long)s.top_k_rows[row] : s.top_k;
+  r.top_k = k <= 0 || k > (long)n ? n : (unsigned)k;
   r.top_p = s.top_p_rows ? (double)s.top_p_rows[row] : s.top_p;
   r.min_p = s.min_p_rows ? (double)s.min_p_rows[row] : s.min_p;
-  if (r.top_k <= 0 || r.top_k > n) r.top_k = n;
   if (!(t > 0)) r.top_k = 1;
-  r.inv_t = t > 0 ? 1 / t : 1;
+  r.inv_t = t > 1e-300 ? 1 / t : t > 0 ? 1e300 : 1;
   return r;
 }
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kBinsEach = kBins / kThreads, kFew = 256;
+// round(exp(d / t) 2^q) for d <= 0, by Tang's method (ACM TOMS 15, 1989): 2^(n/64) from a table, exp of the rest (below
+// ln 2 / 128) by its series to the fifth power (3e-17).  A dozen operations on the FP64 pipe.
+constexpr int kTable = 64;
+struct Weights {
+  const double *table;   // 2^(j/64), in shared memory
+  double c;              // 64 / (t ln 2)
+  int q;
 
-struct Shared {
-  u64 mass[kBins];
-  unsigned count[kBins];
-  u64 few_key[kFew], few_mass[kFew];
-  long few_index[kFew];
-  u64 sum[kWarps];
-  u64 result[4];
-  long index[2];
-  int bin;
-  unsigned few;
+  static __device__ __forceinline__ void fill(double *table) {
+    if (threadIdx.x < kTable) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / kTable));
+  }
+  __device__ __forceinline__ Weights(const double *tab, double inv_t, int q_) : table(tab), c(inv_t * 92.332482616893656877), q(q_) {}
+  __device__ __forceinline__ u64 one() const { return 1ull << q; }
+  __device__ __forceinline__ u64 mass(double d) const {
+    constexpr double kRound = 6755399441055744.0;            // 1.5 * 2^52: what is added to it is rounded to an integer
+    constexpr double a = 0.010830424696249145252;            // ln 2 / 64
+    constexpr double a2 = a * a / 2, a3 = a2 * a / 3, a4 = a3 * a / 4, a5 = a4 * a / 5;
+    const double t = d * c;
+    if (!(t > -(double)kTable * (q + 2))) return 0;
+    const double big = t + kRound, r = t - (big - kRound);
+    const int n = __double2loint(big);
+    const double p = fma(fma(fma(fma(fma(a5, r, a4), r, a3), r, a2), r, a), r, 1.0);
+    const double v = table[n & (kTable - 1)] * p;
+    const double scaled = __hiloint2double(__double2hiint(v) + (((n >> 6) + q) << 20), __double2loint(v));
+    return (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+  }
+  template <typename W>
+  __device__ __forceinline__ u64 of(W v, W best) const {   // v is no NaN
+    return v == best ? one() : mass((double)v - (double)best);
+  }
 };
+
+// A cut, and the mass of what is not behind it.
+template <typename Key>
+struct Cut {
+  Key key;
+  unsigned index;
+  u64 mass;
+};
+template <typename Key>
+__device__ __forceinline__ bool kept(Key key, unsigned i, const Cut<Key> &c) {
+  return key > c.key || (key == c.key && i <= c.index);
+}
+// Whether a unit with this much in front of it is kept: by count where a count is asked for, else by mass; the first always.
+struct Want {
+  bool by_count;
+  unsigned count;
+  double limit;
+  __device__ __forceinline__ bool inside(unsigned c, u64 m) const { return by_count ? c < count : c == 0 || (double)m < limit; }
+};
+// How many of `in` equal units of mass m are kept, the first of which is.
+__device__ __forceinline__ unsigned equal_ones(const Want &w, unsigned in, u64 m, unsigned above_count, u64 above_mass) {
+  if (w.by_count) return min(in, w.count - above_count);
+  if (m == 0) return in;
+  const double r = (w.limit - (double)above_mass) / (double)m;
+  unsigned t = r > 1 ? (r < (double)in ? (unsigned)r : in) : 1;
+  while (t > 1 && !((double)(above_mass + (t - 1) * m) < w.limit)) --t;
+  while (t < in && (double)(above_mass + t * m) < w.limit) ++t;
+  return t;
+}
+__device__ __forceinline__ u64 target_of(float random, u64 total) {
+  const double at = (double)random * (double)total;
+  const u64 t = at > 0 ? at < 9e18 ? (u64)at : total : 0;
+  return t < total ? t : total - 1;   // (a random number of 1, or the product's rounding)
+}
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
 }
+template <typename V>
+__device__ __forceinline__ V warp_up_to(V v) {   // the sum over the lanes in front and one's own
+  const int lane = threadIdx.x & 31;
+  for (int off = 1; off < 32; off *= 2) {
+    const V o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
+  return v;
+}
+__device__ __forceinline__ unsigned warp_max(unsigned v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ u64 warp_max(u64 v) {
+  for (int off = 16; off > 0; off >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+__device__ __forceinline__ unsigned warp_min(unsigned v) { return __reduce_min_sync(0xffffffffu, v); }
+__device__ __forceinline__ u64 warp_min(u64 v) { return ~warp_max(~v); }
+
+// ---- a warp per group ------------------------------------------------------
+
+constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
+
+template <typename Key>
+struct Few {   // the units a cut lies among
+  u64 mass[32];
+  Key key[32];
+  unsigned index[32];
+};
+
+// A group in a warp: lane l holds units l * EACH to l * EACH + EACH - 1, those behind the group's end at -infinity.
+template <typename W, int EACH>
+struct WarpGroup {
+  using Key = typename Keys<W>::type;
+  Key key[EACH];
+  u64 mass[EACH];
+
+  __device__ __forceinline__ unsigned first() const { return (threadIdx.x & 31) * EACH; }
+
+  __device__ Cut<Key> cut(const Want &want, Key best, Few<Key> &few) const {
+    const unsigned lane = threadIdx.x & 31;
+    // units in [lo, hi], units above; those at -infinity, which are never drawn, are out of it
+    const Key none = Keys<W>::of((W)-INFINITY);
+    Key lo = ~(Key)0, hi = best;
+    unsigned in = 0, above_count = 0;
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+      if (key[r] > none) {
+        lo = min(lo, key[r]);
+        in += 1;
+      }
+    lo = warp_min(lo);
+    in = __reduce_add_sync(0xffffffffu, in);
+    u64 above_mass = 0;
+    for (int round = 0; in > 32 && lo < hi; ++round) {
+      const W mid = Keys<W>::value(lo) * (W)0.5 + Keys<W>::value(hi) * (W)0.5;
+      Key pivot = round < 8 && mid == mid ? Keys<W>::of(mid) : lo + (hi - lo) / 2 + 1;   // half the values, later half the bits
+      pivot = pivot <= lo ? lo + 1 : pivot > hi ? hi : pivot;
+      unsigned c = 0;
+      u64 m = 0;
+#pragma unroll
+      for (int r = 0; r < EACH; ++r)
+        if (key[r] >= pivot && key[r] <= hi) c += 1, m += mass[r];
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (!want.by_count) m = warp_sum(m);
+      if (c < in && want.inside(above_count + c, above_mass + m)) {
+        above_count += c;
+        above_mass += m;
+        in -= c;
+        hi = pivot - 1;
+      } else {
+        in = c;
+        lo = pivot;
+      }
+    }
+    Cut<Key> r;
+    if (in > 32) {   // equal ones
+      unsigned c = 0;
+      u64 m = 0;
+#pragma unroll
+      for (int q = 0; q < EACH; ++q)
+        if (key[q] == lo) c += 1, m = mass[q];
+      const unsigned up_to = warp_up_to(c);
+      m = warp_max(m);
+      const unsigned take = equal_ones(want, in, m, above_count, above_mass);
+      unsigned at = up_to - c, index = 0;
+#pragma unroll
+      for (int q = 0; q < EACH; ++q)
+        if (key[q] == lo && ++at == take) index = first() + q + 1;
+      r.key = lo;
+      r.index = __reduce_max_sync(0xffffffffu, index) - 1;
+      r.mass = above_mass + take * m;
+    } else {
+      unsigned c = 0;
+#pragma unroll
+      for (int q = 0; q < EACH; ++q) c += key[q] >= lo && key[q] <= hi;
+      unsigned at = warp_up_to(c) - c;
+#pragma unroll
+      for (int q = 0; q < EACH; ++q)
+        if (key[q] >= lo && key[q] <= hi) {
+          few.key[at] = key[q];
+          few.mass[at] = mass[q];
+          few.index[at] = first() + q;
+          ++at;
+        }
+      __syncwarp();
+      const Key k = lane < in ? few.key[lane] : 0;
+      unsigned cb = above_count;
+      u64 mb = above_mass;
+      for (unsigned j = 0; j < in; ++j) {   // (they lie in index order)
+        const Key o = few.key[j];
+        if (o > k || (o == k && j < lane)) cb += 1, mb += few.mass[j];
+      }
+      const unsigned keep = __ballot_sync(0xffffffffu, lane < in && want.inside(cb, mb));
+      const unsigned last = __popc(keep) - 1;
+      const unsigned who = __ffs(__ballot_sync(0xffffffffu, lane < in && cb == above_count + last)) - 1;
+      r.key = __shfl_sync(0xffffffffu, k, who);
+      r.index = few.index[who];
+      r.mass = __shfl_sync(0xffffffffu, mb, who) + few.mass[who];
+      __syncwarp();
+    }
+    // by count, the masses in front have not been summed in the rounds
+    if (want.by_count) {
+      u64 m = 0;
+#pragma unroll
+      for (int q = 0; q < EACH; ++q)
+        if (kept(key[q], first() + q, r)) m += mass[q];
+      r.mass = warp_sum(m);
+    }
+    return r;
+  }
+};
+
+template <typename T, int EACH>
+__global__ void __launch_bounds__(kWarpThreads)
+    sample_warp_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned groups, unsigned H, unsigned n, bool whole,
+                       const Sampling how, int q, long long *__restrict__ codes) {
+  after_previous();
+  using W = Wide<T>;
+  using Key = typename Keys<W>::type;
+  __shared__ double s_table[kTable];
+  __shared__ Few<Key> s_few[kWarps];
+  Weights::fill(s_table);
+  __syncthreads();
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (unsigned g = blockIdx.x * kWarps + warp; g < groups; g += gridDim.x * kWarps) {
+    const T *const x = support + (long)g * n;
+    WarpGroup<W, EACH> group;
+    W v[EACH];
+    if (whole) {   // rows and lanes' parts start on boundaries, and a lane's part is the group's or not
+      constexpr int V = EACH * (int)sizeof(T) <= 16 ? EACH : 16 / (int)sizeof(T);
+#pragma unroll
+      for (int r = 0; r < EACH; r += V) {
+        if (lane * EACH < n) {
+          const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(x + lane * EACH + r);
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[r + i] = no_nan(widen(a.v[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[r + i] = (W)-INFINITY;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < EACH; ++r) v[r] = lane * EACH + r < n ? no_nan(widen(x[lane * EACH + r])) : (W)-INFINITY;
+    }
+    const Settings set = settings_of(how, g / H, n);
+    Key top = 0;
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      group.key[r] = Keys<W>::of(v[r]);
+      top = max(top, group.key[r]);
+    }
+    top = warp_max(top);
+    const W best = Keys<W>::value(top);
+    long long code = -1;
+    if (best > (W)-INFINITY) {
+      if (set.top_k == 1) {
+        unsigned index = n;
+#pragma unroll
+        for (int r = EACH - 1; r >= 0; --r)
+          if (group.key[r] == top) index = lane * EACH + r;
+        code = warp_min(index);
+      } else {
+        const Weights weights(s_table, set.inv_t, q);
+#pragma unroll
+        for (int r = 0; r < EACH; ++r) group.mass[r] = weights.of(v[r], best);
+        u64 total = 0;
+        Cut<Key> cut{0, n, 0};
+        if (set.top_k < n) cut = group.cut(Want{true, set.top_k, 0.0}, top, s_few[warp]);
+        if (set.top_p < 1) {
+          if (set.top_k >= n) {
+#pragma unroll
+            for (int r = 0; r < EACH; ++r) cut.mass += group.mass[r];
+            cut.mass = warp_sum(cut.mass);
+          }
+          cut = group.cut(Want{false, 0, set.top_p * (double)cut.mass}, top, s_few[warp]);
+        }
+        const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
+#pragma unroll
+        for (int r = 0; r < EACH; ++r) {
+          if (!(kept(group.key[r], lane * EACH + r, cut) && (group.mass[r] >= least || group.key[r] == top))) group.mass[r] = 0;
+          total += group.mass[r];
+        }
+        const u64 up_to = warp_up_to(total);
+        const u64 target = target_of(random[g], __shfl_sync(0xffffffffu, up_to, 31));
+        const unsigned who = __ffs(__ballot_sync(0xffffffffu, up_to > target)) - 1;
+        u64 run = up_to - total;
+        unsigned index = lane * EACH;
+#pragma unroll
+        for (int r = 0; r < EACH; ++r) {
+          run += group.mass[r];
+          index += run <= target;
+        }
+        code = __shfl_sync(0xffffffffu, index, who);
+      }
+      code += (long long)(g % H) * n;
+    }
+    if (lane == 0) codes[g] = code;
+    __syncwarp();
+  }
+}
+
+// ---- a cluster per group ---------------------------------------------------
+
+constexpr int kThreads = 512, kBlockWarps = kThreads / 32, kBins = 2048, kBinsEach = kBins / kThreads, kList = 512;
+constexpr int kMostBlocks = 8;      // of a cluster
+constexpr int kStage = 128 * 1024;   // bytes of a group that a block keeps in shared memory
+
+struct Block {
+  u64 bin_mass[kBins];
+  unsigned bin_count[kBins];
+  u64 list_key[kList], list_mass[kList], sorted_mass[kList];
+  unsigned list_index[kList], sorted_index[kList];
+  double table[kTable];
+  u64 sum[kBlockWarps];
+  u64 part[4];        // what a block tells the others
+  u64 found[4];       // what the first block finds: bin, and the count, mass and units of the bin in front
+  unsigned list;      // units in the list
+  int bin;
+};
+
 __device__ __forceinline__ u64 block_sum(u64 v, u64 *s) {
   v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0;
-  for (int i = 0; i < kWarps; ++i) v += s[i];
+#pragma unroll
+  for (int i = 0; i < kBlockWarps; ++i) v += s[i];
   return v;
+}
+template <typename Key>
+__device__ __forceinline__ Key block_max(Key v, u64 *s) {
+  v = warp_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  u64 m = 0;
+#pragma unroll
+  for (int i = 0; i < kBlockWarps; ++i) m = max(m, s[i]);
+  return (Key)m;
 }
 // The sum over the threads in front, in order.
 __device__ __forceinline__ u64 block_before(u64 v, u64 *s) {
-  u64 in = v;
-  const int lane = threadIdx.x & 31;
-  for (int off = 1; off < 32; off *= 2) {
-    const u64 o = __shfl_up_sync(0xffffffffu, in, off);
-    if (lane >= off) in += o;
-  }
+  const u64 in = warp_up_to(v);
   __syncthreads();
-  if (lane == 31) s[threadIdx.x >> 5] = in;
+  if ((threadIdx.x & 31) == 31) s[threadIdx.x >> 5] = in;
   __syncthreads();
   u64 base = 0;
-  for (int i = 0; i < (int)(threadIdx.x >> 5); ++i) base += s[i];
+#pragma unroll
+  for (int i = 0; i < kBlockWarps; ++i) base += i < (int)(threadIdx.x >> 5) ? s[i] : 0;
   return base + in - v;
 }
 
-template <typename T>
-struct Group {
+// The part of a group that a block works on: units [begin, begin + size) of `n`.
+template <typename T, bool STAGED>
+struct Part {
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
-  const T *x;
-  long n;
+  static constexpr int V = STAGED ? 16 / (int)sizeof(T) : 1;
+  const T *x;   // of unit `begin`; in shared memory and filled up to a whole vector with -infinity where STAGED
+  unsigned begin, size, n;
   W best;
-  double inv_t, one;   // one: 2^q, the mass of the largest weight
+  Block &s;
+  cg::cluster_group cluster;
 
-  __device__ __forceinline__ W value(long i) const { return no_nan(widen(x[i])); }
-  __device__ __forceinline__ double weight(W v) const {
-    return v == best ? 1.0 : v == (W)-INFINITY ? 0.0 : exp(((double)v - (double)best) * inv_t);
+  __device__ __forceinline__ W value(unsigned i) const { return no_nan(widen(x[i])); }
+  // f(value, index in the part) for every unit above -infinity
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (unsigned i = threadIdx.x * V; i < size; i += kThreads * V) {
+      const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(x + i);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const W w = no_nan(widen(a.v[v]));
+        if (w > (W)-INFINITY) f(w, i + v);
+      }
+    }
   }
-  __device__ __forceinline__ u64 mass(double w) const { return __double2ull_rn(w * one); }
-  __device__ __forceinline__ u64 mass_of(W v) const { return mass(weight(v)); }
+  __device__ __forceinline__ u64 cluster_sum(u64 v) {   // of a value of each block
+    if (cluster.num_blocks() == 1) return v;
+    __syncthreads();
+    if (threadIdx.x == 0) s.part[0] = v;
+    cluster.sync();
+    v = 0;
+    for (unsigned b = 0; b < cluster.num_blocks(); ++b) v += cluster.map_shared_rank(&s, b)->part[0];
+    cluster.sync();
+    return v;
+  }
+  __device__ __forceinline__ u64 cluster_max(u64 v) {
+    if (cluster.num_blocks() == 1) return v;
+    __syncthreads();
+    if (threadIdx.x == 0) s.part[0] = v;
+    cluster.sync();
+    v = 0;
+    for (unsigned b = 0; b < cluster.num_blocks(); ++b) v = max(v, cluster.map_shared_rank(&s, b)->part[0]);
+    cluster.sync();
+    return v;
+  }
+
+  // The first unit at which the running sum of weigh(value, index) passes `target`, below the sum of all (which is `all` of this
+  // part); known to every block.
+  template <typename F>
+  __device__ unsigned locate(F weigh, u64 target) {
+    const unsigned each_warp = (size + kBlockWarps - 1) / kBlockWarps, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned lo = min(size, warp * each_warp), hi = min(size, lo + each_warp);
+    u64 mine = 0;
+    for (unsigned i = lo + lane; i < hi; i += 32) mine += weigh(value(i), begin + i);
+    mine = warp_sum(mine);
+    __syncthreads();
+    if (lane == 0) s.sum[warp] = mine;
+    __syncthreads();
+    u64 before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kBlockWarps; ++w) {
+      before += w < (int)warp ? s.sum[w] : 0;
+      all += s.sum[w];
+    }
+    if (threadIdx.x == 0) s.part[0] = all;
+    cluster.sync();
+    for (unsigned b = 0; b < cluster.block_rank(); ++b) before += cluster.map_shared_rank(&s, b)->part[0];
+    if (before <= target && target < before + mine)
+      for (unsigned i0 = lo; i0 < hi; i0 += 32) {
+        const u64 up_to = warp_up_to(i0 + lane < hi ? weigh(value(i0 + lane), begin + i0 + lane) : (u64)0);
+        const unsigned past = __ballot_sync(0xffffffffu, before + up_to > target);
+        if (past) {
+          const u64 unit = begin + i0 + __ffs(past) - 1;
+          if (lane < cluster.num_blocks()) cluster.map_shared_rank(&s, lane)->part[1] = unit;
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, up_to, 31);
+      }
+    cluster.sync();
+    return (unsigned)s.part[1];
+  }
+
+  // Fills the bins: bin_of(value, key) in [0, kBins) or -1, masses where `masses` is set; the first block gets the sums of all.
+  template <typename F>
+  __device__ void histogram(F bin_of, bool masses, const Weights &weights) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kThreads) s.bin_count[b] = 0, s.bin_mass[b] = 0;
+    __syncthreads();
+    each([&](W v, unsigned) {
+      const int b = bin_of(v);
+      if (b < 0) return;
+      atomicAdd(&s.bin_count[b], 1u);
+      if (masses) {
+        const u64 m = weights.of(v, best);
+        if (m) atomicAdd(&s.bin_mass[b], m);
+      }
+    });
+    cluster.sync();
+    if (cluster.block_rank() == 0)
+      for (int b = threadIdx.x; b < kBins; b += kThreads) {
+        unsigned c = s.bin_count[b];
+        u64 m = s.bin_mass[b];
+        for (unsigned o = 1; o < cluster.num_blocks(); ++o) {
+          const Block *const other = cluster.map_shared_rank(&s, o);
+          c += other->bin_count[b];
+          if (masses) m += other->bin_mass[b];
+        }
+        s.bin_count[b] = c;
+        s.bin_mass[b] = m;
+      }
+    __syncthreads();
+  }
+  struct Found {
+    int bin;
+    unsigned in_bin, above_count;
+    u64 above_mass;
+  };
+  // The last bin that begins inside, from the first block's sums; known to every block.
+  __device__ Found find(const Want &want, unsigned above_count, u64 above_mass) {
+    if (cluster.block_rank() == 0) {
+      if (threadIdx.x == 0) s.bin = 0;
+      u64 c = 0, m = 0;
+#pragma unroll
+      for (int j = 0; j < kBinsEach; ++j) {
+        c += s.bin_count[threadIdx.x * kBinsEach + j];
+        m += s.bin_mass[threadIdx.x * kBinsEach + j];
+      }
+      u64 cb = above_count + block_before(c, s.sum), mb = above_mass + block_before(m, s.sum);
+      const u64 c0 = cb, m0 = mb;
+#pragma unroll
+      for (int j = 0; j < kBinsEach; ++j) {
+        const int b = threadIdx.x * kBinsEach + j;
+        if (s.bin_count[b] && want.inside((unsigned)cb, mb)) atomicMax(&s.bin, b);
+        cb += s.bin_count[b];
+        mb += s.bin_mass[b];
+      }
+      __syncthreads();
+      const int bin = s.bin;
+      if (bin / kBinsEach == (int)threadIdx.x) {
+        cb = c0, mb = m0;
+        for (int b = threadIdx.x * kBinsEach; b < bin; ++b) cb += s.bin_count[b], mb += s.bin_mass[b];
+        const u64 in = s.bin_count[bin];
+        for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
+          u64 *const to = cluster.map_shared_rank(&s, o)->found;
+          to[0] = bin;
+          to[1] = cb;
+          to[2] = mb;
+          to[3] = in;
+        }
+      }
+    }
+    cluster.sync();
+    const Found f{(int)s.found[0], (unsigned)s.found[3], (unsigned)s.found[1], s.found[2]};
+    return f;
+  }
+  // Puts the units that `want`s into the first block's list, which has room for them; returns their number to that block.
+  template <typename F>
+  __device__ unsigned gather(F wanted, const Weights &weights) {
+    Block *const first = cluster.map_shared_rank(&s, 0);
+    if (cluster.block_rank() == 0 && threadIdx.x == 0) s.list = 0;
+    cluster.sync();
+    each([&](W v, unsigned i) {
+      if (!wanted(v)) return;
+      const unsigned at = atomicAdd(&first->list, 1u);
+      if (at >= kList) return;
+      first->list_key[at] = Keys<W>::of(v);
+      first->list_index[at] = begin + i;
+      first->list_mass[at] = weights.of(v, best);
+    });
+    cluster.sync();
+    return cluster.block_rank() == 0 ? s.list : 0;
+  }
+  // The first block's list in order; a thread's entry, its rank and what lies in front of it.
+  struct Ranked {
+    Key key;
+    unsigned index, rank;
+    u64 mass, before;
+  };
+  __device__ Ranked rank(unsigned count) {
+    Ranked r{};
+    r.rank = kList;
+    if (threadIdx.x < count) {
+      r.key = (Key)s.list_key[threadIdx.x];
+      r.index = s.list_index[threadIdx.x];
+      r.mass = s.list_mass[threadIdx.x];
+      r.rank = 0;
+      for (unsigned j = 0; j < count; ++j) {
+        const Key o = (Key)s.list_key[j];
+        r.rank += o > r.key || (o == r.key && s.list_index[j] < r.index);
+      }
+      s.sorted_mass[r.rank] = r.mass;
+    }
+    __syncthreads();
+    const u64 before = block_before(threadIdx.x < count ? s.sorted_mass[threadIdx.x] : 0, s.sum);
+    __syncthreads();
+    if (threadIdx.x < count) s.sorted_mass[threadIdx.x] = before;
+    __syncthreads();
+    if (threadIdx.x < count) r.before = s.sorted_mass[r.rank];
+    return r;
+  }
+
+  // The cut that `want` asks for among all units: bins of equal width in the value's distance from the largest first (`found`, by
+  // linear_bin), then, while a bin holds too many for the list, bins of its values' bits.
+  template <typename F>
+  __device__ Cut<Key> cut(const Want &want, Found found, F linear_bin, const Weights &weights) {
+    Key lo = 0, hi = ~(Key)0;
+    unsigned above_count = found.above_count, in = found.in_bin;
+    u64 above_mass = found.above_mass;
+    const int bin = found.bin;
+    auto among = [&](W v) {
+      const Key k = Keys<W>::of(v);
+      return linear_bin(v) == bin && k >= lo && k <= hi;
+    };
+    while (in > kList && lo < hi) {
+      Key low = ~(Key)0, high = 0;
+      each([&](W v, unsigned) {
+        if (among(v)) {
+          const Key k = Keys<W>::of(v);
+          low = min(low, k);
+          high = max(high, k);
+        }
+      });
+      high = (Key)cluster_max(block_max(high, s.sum));
+      low = ~(Key)cluster_max(block_max((Key)~low, s.sum));
+      lo = low, hi = high;
+      if (lo == hi) break;
+      int shift = 0;
+      while (((hi - lo) >> shift) >= (Key)kBins) ++shift;
+      histogram([&](W v) { return among(v) ? (int)((hi - Keys<W>::of(v)) >> shift) : -1; }, !want.by_count, weights);
+      const Found f = find(want, above_count, above_mass);
+      above_count = f.above_count;
+      above_mass = f.above_mass;
+      in = f.in_bin;
+      const Key width = (Key)1 << shift, top = hi - (Key)f.bin * width;
+      if (top - lo >= width) lo = top - (width - 1);
+      hi = top;
+    }
+    if (in > kList) {   // equal values
+      const u64 m = weights.of(Keys<W>::value(hi), best);
+      const unsigned take = equal_ones(want, in, m, above_count, above_mass);
+      const Key key = hi;
+      const unsigned index = locate([&](W v, unsigned) { return (u64)(Keys<W>::of(v) == key); }, take - 1);
+      return Cut<Key>{key, index, above_mass + take * m};
+    }
+    const unsigned count = gather(among, weights);
+    if (cluster.block_rank() == 0) {
+      const Ranked r = rank(count);
+      const bool keep = threadIdx.x < count && want.inside(above_count + r.rank, above_mass + r.before);
+      const u64 n_kept = block_sum(keep, s.sum);
+      if (keep && r.rank + 1 == n_kept)
+        for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
+          u64 *const to = cluster.map_shared_rank(&s, o)->found;
+          to[0] = r.key;
+          to[1] = r.index;
+          to[2] = above_mass + r.before + r.mass;
+        }
+    }
+    cluster.sync();
+    return Cut<Key>{(Key)s.found[0], (unsigned)s.found[1], s.found[2]};
+  }
 };
 
-// The last unit of a beginning of the order: `count` units where it is a count, else those with less than `limit` in front.
-template <typename Key>
-struct Cut {
-  Key key;
-  long index;
-  u64 mass;   // of the units up to it
-};
-template <typename Key>
-__device__ __forceinline__ bool kept(Key key, long i, const Cut<Key> &c) {
-  return key > c.key || (key == c.key && i <= c.index);
-}
-
-// The first unit in index order at which the running sum of weigh(i) passes `target`; the last one with a weight where none does
-// (rounding of the target).  -1 where nothing has a weight.
-template <typename F>
-__device__ long locate(long n, F weigh, u64 target, Shared &s) {
-  const long each = (n + kWarps - 1) / kWarps;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long lo = min(n, warp * each), hi = min(n, lo + each);
-  u64 mine = 0;
-  for (long i = lo + lane; i < hi; i += 32) mine += weigh(i);
-  mine = warp_sum(mine);
-  __syncthreads();
-  if (lane == 0) s.sum[warp] = mine;
-  if (threadIdx.x == 0) s.index[0] = -1;
-  __syncthreads();
-  u64 before = 0, all = 0;
-  for (int i = 0; i < kWarps; ++i) {
-    if (i < warp) before += s.sum[i];
-    all += s.sum[i];
-  }
-  if (all > 0 && target >= all) target = all - 1;
-  if (mine > 0 && before <= target && target < before + mine) {
-    for (long i0 = lo; i0 < hi; i0 += 32) {
-      u64 in = i0 + lane < hi ? weigh(i0 + lane) : 0;
-      for (int off = 1; off < 32; off *= 2) {
-        const u64 o = __shfl_up_sync(0xffffffffu, in, off);
-        if (lane >= off) in += o;
-      }
-      const unsigned past = __ballot_sync(0xffffffffu, before + in > target);
-      if (past) {
-        if (lane == 0) s.index[0] = i0 + __ffs(past) - 1;
-        break;
-      }
-      before += __shfl_sync(0xffffffffu, in, 31);
-    }
-  }
-  __syncthreads();
-  return s.index[0];
-}
-
-template <typename T>
-__device__ Cut<typename Keys<Wide<T>>::type> select(const Group<T> &g, bool by_count, u64 count, double limit, Shared &s) {
-  using W = Wide<T>;
-  using Key = typename Keys<W>::type;
-  Key lo = Keys<W>::of((W)-INFINITY), hi = Keys<W>::of(g.best);
-  u64 above_count = 0, above_mass = 0;   // of the units above hi
-  for (;;) {
-    int shift = 0;
-    while (((hi - lo) >> shift) >= (Key)kBins) ++shift;
-    for (int b = threadIdx.x; b < kBins; b += kThreads) s.count[b] = 0, s.mass[b] = 0;
-    __syncthreads();
-    for (long i = threadIdx.x; i < g.n; i += kThreads) {
-      const W v = g.value(i);
-      const Key key = Keys<W>::of(v);
-      if (key < lo || key > hi) continue;
-      const int b = (int)((hi - key) >> shift);   // bin 0 holds the largest
-      atomicAdd(&s.count[b], 1u);
-      const u64 m = g.mass_of(v);
-      if (m) atomicAdd(&s.mass[b], m);
-    }
-    __syncthreads();
-    u64 c = 0, m = 0;
-    for (int j = 0; j < kBinsEach; ++j) {
-      c += s.count[threadIdx.x * kBinsEach + j];
-      m += s.mass[threadIdx.x * kBinsEach + j];
-    }
-    u64 cb = above_count + block_before(c, s.sum), mb = above_mass + block_before(m, s.sum);
-    if (threadIdx.x == 0) s.bin = -1;
-    __syncthreads();
-    // the last bin that begins inside
-    for (int j = 0; j < kBinsEach; ++j) {
-      const int b = threadIdx.x * kBinsEach + j;
-      if (s.count[b] && (by_count ? cb < count : (double)mb < limit || cb == 0)) atomicMax(&s.bin, b);
-      cb += s.count[b];
-      mb += s.mass[b];
-    }
-    __syncthreads();
-    const int bin = s.bin;
-    if (bin / kBinsEach == (int)threadIdx.x) {
-      for (int j = kBinsEach - 1; j >= bin % kBinsEach; --j) {
-        cb -= s.count[threadIdx.x * kBinsEach + j];
-        mb -= s.mass[threadIdx.x * kBinsEach + j];
-      }
-      s.result[0] = cb;
-      s.result[1] = mb;
-      s.few = 0;
-    }
-    __syncthreads();
-    above_count = s.result[0];
-    above_mass = s.result[1];
-    const unsigned in_bin = s.count[bin];
-    const Key width = (Key)1 << shift, top = hi - (Key)bin * width;
-    if (top - lo >= width) lo = top - (width - 1);
-    hi = top;
-    if (in_bin <= kFew) break;
-    if (lo == hi) {   // equal values: so many of the lowest indices
-      Cut<Key> r;
-      r.key = hi;
-      u64 take = in_bin;
-      W v = g.best;
-      const long first = locate(g.n, [&](long i) { return (u64)(Keys<W>::of(g.value(i)) == hi); }, 0, s);
-      v = g.value(first);
-      const u64 m = g.mass_of(v);
-      if (by_count) {
-        take = min(take, count - above_count);
-      } else if (m > 0) {
-        const double q = (limit - (double)above_mass) / (double)m;
-        u64 t = q > 1 ? (q < (double)in_bin ? (u64)q : in_bin) : 1;
-        while (t > 1 && !((double)(above_mass + (t - 1) * m) < limit)) --t;
-        while (t < in_bin && (double)(above_mass + t * m) < limit) ++t;
-        take = t;
-      }
-      r.index = locate(g.n, [&](long i) { return (u64)(Keys<W>::of(g.value(i)) == hi); }, take - 1, s);
-      r.mass = above_mass + take * m;
-      return r;
-    }
-    __syncthreads();   // the histogram has been read
-  }
-  for (long i = threadIdx.x; i < g.n; i += kThreads) {
-    const W v = g.value(i);
-    const Key key = Keys<W>::of(v);
-    if (key < lo || key > hi) continue;
-    const unsigned at = atomicAdd(&s.few, 1u);
-    s.few_key[at] = key;
-    s.few_index[at] = i;
-    s.few_mass[at] = g.mass_of(v);
-  }
-  __syncthreads();
-  const int few = (int)s.few;
-  bool keep = false;
-  u64 cb = above_count, mb = above_mass;
-  if ((int)threadIdx.x < few) {
-    const u64 key = s.few_key[threadIdx.x];
-    const long index = s.few_index[threadIdx.x];
-    for (int j = 0; j < few; ++j)
-      if (s.few_key[j] > key || (s.few_key[j] == key && s.few_index[j] < index)) {
-        cb += 1;
-        mb += s.few_mass[j];
-      }
-    keep = by_count ? cb < count : (double)mb < limit || cb == 0;
-  }
-  const u64 n_kept = block_sum(keep, s.sum);
-  if (keep && cb + 1 == above_count + n_kept) {
-    s.result[2] = s.few_key[threadIdx.x];
-    s.result[3] = mb + s.few_mass[threadIdx.x];
-    s.index[1] = s.few_index[threadIdx.x];
-  }
-  __syncthreads();
-  return Cut<Key>{(Key)s.result[2], s.index[1], s.result[3]};
-}
-
-// A block per group.
-template <typename T>
+template <typename T, bool STAGED>
 __global__ void __launch_bounds__(kThreads)
-    sample_kernel(const T *__restrict__ support, const float *__restrict__ random, long H, long Mc, Sampling how, double one, long long *__restrict__ codes) {
+    sample_block_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned H, unsigned n, unsigned part, bool whole,
+                        const Sampling how, int q, long long *__restrict__ codes) {
   after_previous();
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
-  __shared__ Shared s;
-  const long g = blockIdx.x;
-  const Settings set = settings_of(how, g / H, Mc);
-  Group<T> group{support + g * Mc, Mc, (W)-INFINITY, set.inv_t, one};
-  Key top = 0;
-  for (long i = threadIdx.x; i < Mc; i += kThreads) {
-    const W v = group.value(i);
-    const Key k = Keys<W>::of(v);
-    if (k > top) top = k, group.best = v;
+  extern __shared__ uint4 s_values[];
+  __shared__ Block s;
+  cg::cluster_group cluster = cg::this_cluster();
+  const unsigned blocks = cluster.num_blocks(), g = blockIdx.x / blocks, rank = cluster.block_rank();
+  const unsigned begin = min(n, rank * part), size = min(part, n - begin);
+  const T *const from = support + (long)g * n + begin;
+  Weights::fill(s.table);
+  Key top = Keys<W>::of((W)-INFINITY);
+  Part<T, STAGED> p{from, begin, size, n, (W)0, s, cluster};
+  if constexpr (STAGED) {
+    constexpr int V = 16 / (int)sizeof(T);
+    T *const to = reinterpret_cast<T *>(s_values);
+    const unsigned vectors = whole ? size / V : 0;   // (rows and parts start on 16-byte boundaries)
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
+      const Vec<T, V> a = reinterpret_cast<const Vec<T, V> *>(from)[i];
+      reinterpret_cast<Vec<T, V> *>(to)[i] = a;
+#pragma unroll
+      for (int v = 0; v < V; ++v) top = max(top, Keys<W>::of(no_nan(widen(a.v[v]))));
+    }
+#pragma unroll 4
+    for (unsigned i = vectors * V + threadIdx.x; i < size; i += kThreads) {
+      const T a = from[i];
+      to[i] = a;
+      top = max(top, Keys<W>::of(no_nan(widen(a))));
+    }
+    for (unsigned i = size + threadIdx.x; i < (size + V - 1) / V * V; i += kThreads) to[i] = narrow_to<T>((W)-INFINITY);
+    p.x = to;
+  } else {
+    for (unsigned i = threadIdx.x; i < size; i += kThreads) top = max(top, Keys<W>::of(p.value(i)));
   }
-  for (int off = 16; off > 0; off >>= 1) group.best = fmax(group.best, __shfl_xor_sync(0xffffffffu, group.best, off));
-  if ((threadIdx.x & 31) == 0) reinterpret_cast<W *>(s.sum)[threadIdx.x >> 5] = group.best;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) group.best = fmax(group.best, reinterpret_cast<W *>(s.sum)[i]);
-  __syncthreads();
-  if (group.best == (W)-INFINITY) {
-    if (threadIdx.x == 0) codes[g] = -1;
+  top = (Key)p.cluster_max(block_max(top, s.sum));
+  const W best = p.best = Keys<W>::value(top);
+  if (!(best > (W)-INFINITY)) {
+    if (rank == 0 && threadIdx.x == 0) codes[g] = -1;
     return;
   }
-  Cut<Key> cut{0, Mc, 0};
-  if (set.top_k < Mc) cut = select(group, true, (u64)set.top_k, 0.0, s);
-  if (set.top_p < 1) {
-    u64 total = cut.mass;
-    if (set.top_k >= Mc) {
-      total = 0;
-      for (long i = threadIdx.x; i < Mc; i += kThreads) total += group.mass_of(group.value(i));
-      total = block_sum(total, s.sum);
-    }
-    cut = select(group, false, 0, set.top_p * (double)total, s);
+  const long long base = (long long)(g % H) * n;
+  const Settings set = settings_of(how, g / H, n);
+  const Weights weights(s.table, set.inv_t, q);
+  if (set.top_k == 1) {
+    const unsigned unit = p.locate([&](W v, unsigned) { return (u64)(v == best); }, 0);
+    if (rank == 0 && threadIdx.x == 0) codes[g] = base + unit;
+    return;
   }
-  auto weigh = [&](long i) -> u64 {
-    const W v = group.value(i);
-    if (!kept(Keys<W>::of(v), i, cut)) return 0;
-    const double w = group.weight(v);
-    return w >= set.min_p || v == group.best ? group.mass(w) : 0;
+  const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
+  Cut<Key> cut{0, n, 0};
+  const bool by_count = set.top_k < n;
+  if (by_count || set.top_p < 1) {
+    // bins of 1/128 in the weights' exponents; all units whose weight is below e^-16 share the last one
+    const W scale = (W)(128 * set.inv_t);
+    auto bin = [&](W v) -> int {
+      const W d = (best - v) * scale;
+      return v == best ? 0 : d < (W)(kBins - 1) ? (int)d : kBins - 1;
+    };
+    u64 total = 0;
+    if (!by_count) {
+      p.each([&](W v, unsigned) { total += weights.of(v, best); });
+      total = p.cluster_sum(block_sum(total, s.sum));
+    }
+    Want want{by_count, set.top_k, set.top_p * (double)total};
+    p.histogram(bin, !by_count, weights);
+    auto found = p.find(want, 0, 0);
+    if (found.above_count + found.in_bin <= kList) {
+      // all that may be kept fits the list: the first block goes on by itself
+      const int last = found.bin;
+      const unsigned count = p.gather([&](W v) { return bin(v) <= last; }, weights);
+      if (rank != 0) return;
+      const auto r = p.rank(count);
+      bool keep = threadIdx.x < count;
+      if (by_count) {
+        keep = keep && r.rank < set.top_k;
+        want = Want{false, 0, set.top_p * (double)block_sum(keep ? r.mass : 0, s.sum)};
+      }
+      keep = keep && (set.top_p >= 1 || want.inside(r.rank, r.before)) && (r.mass >= least || r.key == top);
+      const u64 mass = keep ? r.mass : 0, target = target_of(random[g], block_sum(mass, s.sum));
+      if (threadIdx.x < count) s.list_mass[threadIdx.x] = mass;
+      __syncthreads();
+      u64 before = 0;
+      if (keep)
+        for (unsigned j = 0; j < count; ++j)
+          if (s.list_index[j] < r.index) before += s.list_mass[j];
+      if (keep && before <= target && target < before + mass) codes[g] = base + r.index;
+      return;
+    }
+    cut = p.cut(want, found, bin, weights);
+    if (by_count && set.top_p < 1) {
+      u64 sum = 0;
+      p.each([&](W v, unsigned i) {
+        if (kept(Keys<W>::of(v), begin + i, cut)) sum += weights.of(v, best);
+      });
+      want = Want{false, 0, set.top_p * (double)p.cluster_sum(block_sum(sum, s.sum))};
+      p.histogram(bin, true, weights);
+      cut = p.cut(want, p.find(want, 0, 0), bin, weights);
+    }
+  }
+  auto weigh = [&](W v, unsigned i) -> u64 {
+    if (!(v > (W)-INFINITY) || !kept(Keys<W>::of(v), i, cut)) return 0;
+    const u64 m = weights.of(v, best);
+    return m >= least || v == best ? m : 0;
   };
   u64 total = 0;
-  for (long i = threadIdx.x; i < Mc; i += kThreads) total += weigh(i);
-  total = block_sum(total, s.sum);
-  const double at = (double)random[g] * (double)total;
-  const long unit = locate(Mc, weigh, at > 0 ? (u64)at : 0, s);
-  if (threadIdx.x == 0) codes[g] = unit < 0 ? -1 : g % H * Mc + unit;
+  p.each([&](W v, unsigned i) { total += weigh(v, begin + i); });
+  total = p.cluster_sum(block_sum(total, s.sum));
+  const unsigned unit = p.locate(weigh, target_of(random[g], total));
+  if (rank == 0 && threadIdx.x == 0) codes[g] = base + unit;
+}
+
+// 2^q: no sum of n masses passes 2^62.
+int mass_bits(long n) {
+  int q = 50;
+  while (q > 20 && (double)n * (double)(1ull << q) >= 4.6e18) --q;
+  return q;
+}
+
+template <typename T, int EACH>
+cudaError_t launch_warps(const T *support, const float *random, unsigned groups, unsigned H, unsigned n, const Sampling &s, long long *codes,
+                         cudaStream_t st) {
+  constexpr size_t piece = EACH * sizeof(T) < 16 ? EACH * sizeof(T) : 16;
+  const bool whole = n % EACH == 0 && (reinterpret_cast<uintptr_t>(support) | n * sizeof(T)) % piece == 0;
+  const unsigned most = 8 * (unsigned)sm_count(), blocks = (groups + kWarps - 1) / kWarps;
+  return launch_next(sample_warp_kernel<T, EACH>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, support, random, groups, H, n, whole, s,
+                     mass_bits(n), codes);
+}
+
+template <typename T, bool STAGED>
+cudaError_t launch_blocks(const T *support, const float *random, unsigned groups, unsigned H, unsigned n, unsigned part, unsigned cluster,
+                          const Sampling &s, long long *codes, cudaStream_t st) {
+  const size_t smem = STAGED ? ((size_t)part * sizeof(T) + 15) / 16 * 16 : 0;
+  const bool whole = (reinterpret_cast<uintptr_t>(support) | (size_t)n * sizeof(T) | (size_t)part * sizeof(T)) % 16 == 0;
+  if (smem > 0) {   // (holds for the current device)
+    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_clusters(sample_block_kernel<T, STAGED>, dim3(groups * cluster), dim3(cluster), kThreads, smem, st, support, random, H, n, part, whole,
+                         s, mass_bits(n), codes);
 }
 
 }  // namespace
 
 template <typename T>
 cudaError_t launch_sample(const T *support, const float *random, long rows, long H, long Mc, Sampling s, long long *codes, cudaStream_t st) {
-  int q = 50;
-  while (q > 20 && ((double)Mc * (double)(1ull << q)) >= 4.6e18) --q;   // no sum passes 2^62
-  const cudaError_t e = launch_next(sample_kernel<T>, dim3((unsigned)(rows * H)), kThreads, 0, st, support, random, H, Mc, s, (double)(1ull << q), codes);
+  const unsigned groups = (unsigned)(rows * H), n = (unsigned)Mc, h = (unsigned)H;
+  cudaError_t e;
+  if (n <= 32) {
+    e = launch_warps<T, 1>(support, random, groups, h, n, s, codes, st);
+  } else if (n <= 64) {
+    e = launch_warps<T, 2>(support, random, groups, h, n, s, codes, st);
+  } else if (n <= 128) {
+    e = launch_warps<T, 4>(support, random, groups, h, n, s, codes, st);
+  } else if (n <= 256) {
+    e = launch_warps<T, 8>(support, random, groups, h, n, s, codes, st);
+  } else if (n <= 512) {
+    e = launch_warps<T, 16>(support, random, groups, h, n, s, codes, st);
+  } else {
+    // the smallest cluster whose blocks hold their parts; a larger one where groups are too few for the SMs and parts long
+    const size_t bytes = (size_t)n * sizeof(T);
+    unsigned cluster = 1;
+    while (cluster < kMostBlocks && bytes > (size_t)cluster * kStage) cluster *= 2;
+    while (cluster < kMostBlocks && (size_t)groups * cluster * 2 <= (size_t)sm_count() && n / cluster > 2048) cluster *= 2;
+    constexpr unsigned V = 16 / (unsigned)sizeof(T);
+    const unsigned part = ((n + cluster - 1) / cluster + V - 1) / V * V;
+    if ((size_t)groups * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    e = (size_t)part * sizeof(T) <= kStage ? launch_blocks<T, true>(support, random, groups, h, n, part, cluster, s, codes, st)
+                                           : launch_blocks<T, false>(support, random, groups, h, n, part, cluster, s, codes, st);
+  }
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
