@@ -72,6 +72,7 @@ cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, lon
 // One unit per (row, group of Mc) drawn from the softmax of support[rows, H * Mc]; codes[rows, H] = h * Mc + unit, or -1.
 struct Sampling {
   double temperature, top_p, min_p;
+  double inv_t;   // of `temperature`, filled in by launch_sample
   long top_k;
   const float *temperature_rows, *top_p_rows, *min_p_rows;   // not null: a value per row in place of the scalar
   const int *top_k_rows;

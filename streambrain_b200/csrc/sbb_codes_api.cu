@@ -144,8 +144,8 @@ int sbb_sample_minicolumns(int dtype, const void *support_dev, const float *rand
       "sample_minicolumns: misaligned pointer");
   if (const int rc = need_device()) return rc;
   if (rows == 0) return SBB_OK;
-  const sbb::Sampling s = {how->temperature,  how->top_p,      how->min_p,     how->top_k, how->temperature_rows,
-                           how->top_p_rows, how->min_p_rows, how->top_k_rows};
+  const sbb::Sampling s = {how->temperature,      how->top_p,      how->min_p,      0, how->top_k,
+                           how->temperature_rows, how->top_p_rows, how->min_p_rows, how->top_k_rows};
   return done(with_element<int>(dtype,
                                 [&](auto t, int) {
                                   return sbb::launch_sample((const decltype(t) *)support_dev, random_dev, rows, H, Mc, s, codes_dev,

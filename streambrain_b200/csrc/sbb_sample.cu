@@ -51,15 +51,17 @@ struct Settings {
   double inv_t, top_p, min_p;
   unsigned top_k;   // n: all
 };
+__host__ __device__ __forceinline__ double inverse(double t) { return t > 1e-300 ? 1 / t : t > 0 ? 1e300 : 1; }
 __device__ __forceinline__ Settings settings_of(const Sampling &s, long row, unsigned n) {
-  const double t = s.temperature_rows ? (double)s.temperature_rows[row] : s.temperature;
+  const bool own = s.temperature_rows != nullptr;
+  const float t = own ? s.temperature_rows[row] : s.temperature > 0 ? 1 : 0;
   const long k = s.top_k_rows ? (long)s.top_k_rows[row] : s.top_k;
   Settings r;
   r.top_k = k <= 0 || k > (long)n ? n : (unsigned)k;
   r.top_p = s.top_p_rows ? (double)s.top_p_rows[row] : s.top_p;
   r.min_p = s.min_p_rows ? (double)s.min_p_rows[row] : s.min_p;
   if (!(t > 0)) r.top_k = 1;
-  r.inv_t = t > 1e-300 ? 1 / t : t > 0 ? 1e300 : 1;
+  r.inv_t = own ? inverse((double)t) : s.inv_t;
   return r;
 }
 
@@ -110,18 +112,18 @@ __device__ __forceinline__ bool kept(Key key, unsigned i, const Cut<Key> &c) {
 struct Want {
   bool by_count;
   unsigned count;
-  double limit;
-  __device__ __forceinline__ bool inside(unsigned c, u64 m) const { return by_count ? c < count : c == 0 || (double)m < limit; }
+  u64 limit;
+  __device__ __forceinline__ bool inside(unsigned c, u64 m) const { return by_count ? c < count : c == 0 || m < limit; }
 };
+__device__ __forceinline__ Want want_count(unsigned count) { return Want{true, count, 0}; }
+// less than top_p of the mass in front: integers below the product are those below the next integer
+__device__ __forceinline__ Want want_mass(double top_p, u64 mass) { return Want{false, 0, top_p > 0 ? __double2ull_ru(top_p * (double)mass) : 0}; }
 // How many of `in` equal units of mass m are kept, the first of which is.
 __device__ __forceinline__ unsigned equal_ones(const Want &w, unsigned in, u64 m, unsigned above_count, u64 above_mass) {
   if (w.by_count) return min(in, w.count - above_count);
   if (m == 0) return in;
-  const double r = (w.limit - (double)above_mass) / (double)m;
-  unsigned t = r > 1 ? (r < (double)in ? (unsigned)r : in) : 1;
-  while (t > 1 && !((double)(above_mass + (t - 1) * m) < w.limit)) --t;
-  while (t < in && (double)(above_mass + t * m) < w.limit) ++t;
-  return t;
+  if (w.limit <= above_mass) return 1;
+  return (unsigned)min((u64)in, (w.limit - above_mass + m - 1) / m);
 }
 __device__ __forceinline__ u64 target_of(float random, u64 total) {
   const double at = (double)random * (double)total;
@@ -132,6 +134,11 @@ __device__ __forceinline__ u64 target_of(float random, u64 total) {
 __device__ __forceinline__ u64 warp_sum(u64 v) {
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
+}
+// The same for values below 2^54, in two sums of 27 bits.
+__device__ __forceinline__ u64 warp_sum_54(u64 v) {
+  const unsigned lo = __reduce_add_sync(0xffffffffu, (unsigned)v & 0x7ffffffu), hi = __reduce_add_sync(0xffffffffu, (unsigned)(v >> 27));
+  return ((u64)hi << 27) + lo;
 }
 template <typename V>
 __device__ __forceinline__ V warp_up_to(V v) {   // the sum over the lanes in front and one's own
@@ -153,11 +160,12 @@ __device__ __forceinline__ u64 warp_min(u64 v) { return ~warp_max(~v); }
 // ---- a warp per group ------------------------------------------------------
 
 constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
+constexpr int kWarpBits = 48;   // q: the sum of a lane's 16 masses stays below 2^54
 
 template <typename Key>
 struct Few {   // the units a cut lies among
-  u64 mass[32];
   Key key[32];
+  u64 mass[32];
   unsigned index[32];
 };
 
@@ -170,22 +178,22 @@ struct WarpGroup {
 
   __device__ __forceinline__ unsigned first() const { return (threadIdx.x & 31) * EACH; }
 
-  __device__ Cut<Key> cut(const Want &want, Key best, Few<Key> &few) const {
+  __device__ __forceinline__ Cut<Key> cut(const Want &want, Key best, Few<Key> &few) const {
     const unsigned lane = threadIdx.x & 31;
     // units in [lo, hi], units above; those at -infinity, which are never drawn, are out of it
     const Key none = Keys<W>::of((W)-INFINITY);
     Key lo = ~(Key)0, hi = best;
-    unsigned in = 0, above_count = 0;
+    unsigned to_lo = 0, above_count = 0;   // units from lo up, from above hi up
 #pragma unroll
     for (int r = 0; r < EACH; ++r)
       if (key[r] > none) {
         lo = min(lo, key[r]);
-        in += 1;
+        to_lo += 1;
       }
     lo = warp_min(lo);
-    in = __reduce_add_sync(0xffffffffu, in);
+    to_lo = __reduce_add_sync(0xffffffffu, to_lo);
     u64 above_mass = 0;
-    for (int round = 0; in > 32 && lo < hi; ++round) {
+    for (int round = 0; to_lo - above_count > 32 && lo < hi; ++round) {
       const W mid = Keys<W>::value(lo) * (W)0.5 + Keys<W>::value(hi) * (W)0.5;
       Key pivot = round < 8 && mid == mid ? Keys<W>::of(mid) : lo + (hi - lo) / 2 + 1;   // half the values, later half the bits
       pivot = pivot <= lo ? lo + 1 : pivot > hi ? hi : pivot;
@@ -193,30 +201,32 @@ struct WarpGroup {
       u64 m = 0;
 #pragma unroll
       for (int r = 0; r < EACH; ++r)
-        if (key[r] >= pivot && key[r] <= hi) c += 1, m += mass[r];
+        if (key[r] >= pivot) c += 1, m += mass[r];
       c = __reduce_add_sync(0xffffffffu, c);
-      if (!want.by_count) m = warp_sum(m);
-      if (c < in && want.inside(above_count + c, above_mass + m)) {
-        above_count += c;
-        above_mass += m;
-        in -= c;
+      if (!want.by_count) m = warp_sum_54(m);
+      if (c < to_lo && want.inside(c, m)) {
+        above_count = c;
+        above_mass = m;
         hi = pivot - 1;
       } else {
-        in = c;
+        to_lo = c;
         lo = pivot;
       }
     }
+    const unsigned in = to_lo - above_count;
     Cut<Key> r;
+    unsigned c = 0;
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) c += key[q] >= lo && key[q] <= hi;
+    unsigned at = warp_up_to(c) - c;
     if (in > 32) {   // equal ones
-      unsigned c = 0;
       u64 m = 0;
 #pragma unroll
       for (int q = 0; q < EACH; ++q)
-        if (key[q] == lo) c += 1, m = mass[q];
-      const unsigned up_to = warp_up_to(c);
+        if (key[q] == lo) m = mass[q];
       m = warp_max(m);
       const unsigned take = equal_ones(want, in, m, above_count, above_mass);
-      unsigned at = up_to - c, index = 0;
+      unsigned index = 0;
 #pragma unroll
       for (int q = 0; q < EACH; ++q)
         if (key[q] == lo && ++at == take) index = first() + q + 1;
@@ -224,10 +234,7 @@ struct WarpGroup {
       r.index = __reduce_max_sync(0xffffffffu, index) - 1;
       r.mass = above_mass + take * m;
     } else {
-      unsigned c = 0;
-#pragma unroll
-      for (int q = 0; q < EACH; ++q) c += key[q] >= lo && key[q] <= hi;
-      unsigned at = warp_up_to(c) - c;
+      // In index order, a lane each; in the order of the values once more, for the masses in front.
 #pragma unroll
       for (int q = 0; q < EACH; ++q)
         if (key[q] >= lo && key[q] <= hi) {
@@ -237,28 +244,29 @@ struct WarpGroup {
           ++at;
         }
       __syncwarp();
-      const Key k = lane < in ? few.key[lane] : 0;
-      unsigned cb = above_count;
-      u64 mb = above_mass;
-      for (unsigned j = 0; j < in; ++j) {   // (they lie in index order)
-        const Key o = few.key[j];
-        if (o > k || (o == k && j < lane)) cb += 1, mb += few.mass[j];
-      }
-      const unsigned keep = __ballot_sync(0xffffffffu, lane < in && want.inside(cb, mb));
-      const unsigned last = __popc(keep) - 1;
-      const unsigned who = __ffs(__ballot_sync(0xffffffffu, lane < in && cb == above_count + last)) - 1;
+      const Key k = lane < in ? few.key[lane] : 0;   // (no unit's key)
+      const u64 m = lane < in ? few.mass[lane] : 0;
+      unsigned rank = 0;
+#pragma unroll 8
+      for (unsigned j = 0; j < in; ++j) rank += few.key[j] >= k + (j >= lane);
+      __syncwarp();
+      if (lane < in) few.mass[rank] = m;
+      __syncwarp();
+      const u64 by_rank = lane < in ? few.mass[lane] : 0, before = above_mass + warp_up_to(by_rank) - by_rank;
+      // (the last lane inside: every rank in front of it is inside too)
+      const unsigned last = __popc(__ballot_sync(0xffffffffu, lane < in && want.inside(above_count + lane, before))) - 1;
+      const unsigned who = __ffs(__ballot_sync(0xffffffffu, lane < in && rank == last)) - 1;
       r.key = __shfl_sync(0xffffffffu, k, who);
       r.index = few.index[who];
-      r.mass = __shfl_sync(0xffffffffu, mb, who) + few.mass[who];
+      r.mass = __shfl_sync(0xffffffffu, before + by_rank, last);
       __syncwarp();
     }
-    // by count, the masses in front have not been summed in the rounds
-    if (want.by_count) {
-      u64 m = 0;
+    if (want.by_count) {   // the masses in front have not been summed in the rounds
+      u64 all = 0;
 #pragma unroll
       for (int q = 0; q < EACH; ++q)
-        if (kept(key[q], first() + q, r)) m += mass[q];
-      r.mass = warp_sum(m);
+        if (kept(key[q], first() + q, r)) all += mass[q];
+      r.mass = warp_sum_54(all);
     }
     return r;
   }
@@ -267,7 +275,7 @@ struct WarpGroup {
 template <typename T, int EACH>
 __global__ void __launch_bounds__(kWarpThreads)
     sample_warp_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned groups, unsigned H, unsigned n, bool whole,
-                       const Sampling how, int q, long long *__restrict__ codes) {
+                       const Sampling how, long long *__restrict__ codes) {
   after_previous();
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
@@ -297,7 +305,8 @@ __global__ void __launch_bounds__(kWarpThreads)
 #pragma unroll
       for (int r = 0; r < EACH; ++r) v[r] = lane * EACH + r < n ? no_nan(widen(x[lane * EACH + r])) : (W)-INFINITY;
     }
-    const Settings set = settings_of(how, g / H, n);
+    const unsigned row = g / H;
+    const Settings set = settings_of(how, row, n);
     Key top = 0;
 #pragma unroll
     for (int r = 0; r < EACH; ++r) {
@@ -315,19 +324,19 @@ __global__ void __launch_bounds__(kWarpThreads)
           if (group.key[r] == top) index = lane * EACH + r;
         code = warp_min(index);
       } else {
-        const Weights weights(s_table, set.inv_t, q);
+        const Weights weights(s_table, set.inv_t, kWarpBits);
 #pragma unroll
         for (int r = 0; r < EACH; ++r) group.mass[r] = weights.of(v[r], best);
         u64 total = 0;
         Cut<Key> cut{0, n, 0};
-        if (set.top_k < n) cut = group.cut(Want{true, set.top_k, 0.0}, top, s_few[warp]);
+        if (set.top_k < n) cut = group.cut(want_count(set.top_k), top, s_few[warp]);
         if (set.top_p < 1) {
           if (set.top_k >= n) {
 #pragma unroll
             for (int r = 0; r < EACH; ++r) cut.mass += group.mass[r];
-            cut.mass = warp_sum(cut.mass);
+            cut.mass = warp_sum_54(cut.mass);
           }
-          cut = group.cut(Want{false, 0, set.top_p * (double)cut.mass}, top, s_few[warp]);
+          cut = group.cut(want_mass(set.top_p, cut.mass), top, s_few[warp]);
         }
         const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
 #pragma unroll
@@ -347,7 +356,7 @@ __global__ void __launch_bounds__(kWarpThreads)
         }
         code = __shfl_sync(0xffffffffu, index, who);
       }
-      code += (long long)(g % H) * n;
+      code += (long long)(g - row * H) * n;
     }
     if (lane == 0) codes[g] = code;
     __syncwarp();
@@ -358,11 +367,10 @@ __global__ void __launch_bounds__(kWarpThreads)
 
 constexpr int kThreads = 512, kBlockWarps = kThreads / 32, kBins = 2048, kBinsEach = kBins / kThreads, kList = 512;
 constexpr int kMostBlocks = 8;      // of a cluster
-constexpr int kStage = 128 * 1024;   // bytes of a group that a block keeps in shared memory
+constexpr int kStage = 64 * 1024;    // bytes of a group that a block keeps in shared memory
 
 struct Block {
-  u64 bin_mass[kBins];
-  unsigned bin_count[kBins];
+  unsigned bin_count[kBins], bin_low[kBins], bin_high[kBins];   // masses in halves
   u64 list_key[kList], list_mass[kList], sorted_mass[kList];
   unsigned list_index[kList], sorted_index[kList];
   double table[kTable];
@@ -371,6 +379,8 @@ struct Block {
   u64 found[4];       // what the first block finds: bin, and the count, mass and units of the bin in front
   unsigned list;      // units in the list
   int bin;
+
+  __device__ __forceinline__ u64 mass(int b) const { return ((u64)bin_high[b] << 32) + bin_low[b]; }
 };
 
 __device__ __forceinline__ u64 block_sum(u64 v, u64 *s) {
@@ -488,35 +498,43 @@ struct Part {
     return (unsigned)s.part[1];
   }
 
-  // Fills the bins: bin_of(value, key) in [0, kBins) or -1, masses where `masses` is set; the first block gets the sums of all.
+  // Fills the bins: bin_of(value) in [0, kBins) or -1, masses where `masses` is set; the first block gets the sums of all.  Returns
+  // this thread's sum of the masses of all units, `total` asked for.
+  // Masses are added in halves with a carry: an addition of 64 bits to shared memory is a loop, and where values are equal
+  // (16-bit types) a long one: 256 rows of 128000 bf16 units, a few of them without a top-k, 1030 us.
   template <typename F>
-  __device__ void histogram(F bin_of, bool masses, const Weights &weights) {
+  __device__ u64 histogram(F bin_of, bool masses, bool total, const Weights &weights) {
     __syncthreads();
-    for (int b = threadIdx.x; b < kBins; b += kThreads) s.bin_count[b] = 0, s.bin_mass[b] = 0;
+    for (int b = threadIdx.x; b < kBins; b += kThreads) s.bin_count[b] = 0, s.bin_low[b] = 0, s.bin_high[b] = 0;
     __syncthreads();
+    u64 all = 0;
     each([&](W v, unsigned) {
       const int b = bin_of(v);
+      u64 m = 0;
+      if (total || (masses && b >= 0)) m = weights.of(v, best);
+      all += m;
       if (b < 0) return;
       atomicAdd(&s.bin_count[b], 1u);
-      if (masses) {
-        const u64 m = weights.of(v, best);
-        if (m) atomicAdd(&s.bin_mass[b], m);
-      }
+      if (!masses || m == 0) return;
+      const unsigned low = (unsigned)m, old = atomicAdd(&s.bin_low[b], low), high = (unsigned)(m >> 32) + (old + low < low);
+      if (high) atomicAdd(&s.bin_high[b], high);
     });
     cluster.sync();
     if (cluster.block_rank() == 0)
       for (int b = threadIdx.x; b < kBins; b += kThreads) {
         unsigned c = s.bin_count[b];
-        u64 m = s.bin_mass[b];
+        u64 m = s.mass(b);
         for (unsigned o = 1; o < cluster.num_blocks(); ++o) {
           const Block *const other = cluster.map_shared_rank(&s, o);
           c += other->bin_count[b];
-          if (masses) m += other->bin_mass[b];
+          if (masses) m += other->mass(b);
         }
         s.bin_count[b] = c;
-        s.bin_mass[b] = m;
+        s.bin_low[b] = (unsigned)m;
+        s.bin_high[b] = (unsigned)(m >> 32);
       }
     __syncthreads();
+    return all;
   }
   struct Found {
     int bin;
@@ -531,7 +549,7 @@ struct Part {
 #pragma unroll
       for (int j = 0; j < kBinsEach; ++j) {
         c += s.bin_count[threadIdx.x * kBinsEach + j];
-        m += s.bin_mass[threadIdx.x * kBinsEach + j];
+        m += s.mass(threadIdx.x * kBinsEach + j);
       }
       u64 cb = above_count + block_before(c, s.sum), mb = above_mass + block_before(m, s.sum);
       const u64 c0 = cb, m0 = mb;
@@ -540,13 +558,13 @@ struct Part {
         const int b = threadIdx.x * kBinsEach + j;
         if (s.bin_count[b] && want.inside((unsigned)cb, mb)) atomicMax(&s.bin, b);
         cb += s.bin_count[b];
-        mb += s.bin_mass[b];
+        mb += s.mass(b);
       }
       __syncthreads();
       const int bin = s.bin;
       if (bin / kBinsEach == (int)threadIdx.x) {
         cb = c0, mb = m0;
-        for (int b = threadIdx.x * kBinsEach; b < bin; ++b) cb += s.bin_count[b], mb += s.bin_mass[b];
+        for (int b = threadIdx.x * kBinsEach; b < bin; ++b) cb += s.bin_count[b], mb += s.mass(b);
         const u64 in = s.bin_count[bin];
         for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
           u64 *const to = cluster.map_shared_rank(&s, o)->found;
@@ -634,7 +652,7 @@ struct Part {
       if (lo == hi) break;
       int shift = 0;
       while (((hi - lo) >> shift) >= (Key)kBins) ++shift;
-      histogram([&](W v) { return among(v) ? (int)((hi - Keys<W>::of(v)) >> shift) : -1; }, !want.by_count, weights);
+      histogram([&](W v) { return among(v) ? (int)((hi - Keys<W>::of(v)) >> shift) : -1; }, !want.by_count, false, weights);
       const Found f = find(want, above_count, above_mass);
       above_count = f.above_count;
       above_mass = f.above_mass;
@@ -730,13 +748,9 @@ __global__ void __launch_bounds__(kThreads)
       const W d = (best - v) * scale;
       return v == best ? 0 : d < (W)(kBins - 1) ? (int)d : kBins - 1;
     };
-    u64 total = 0;
-    if (!by_count) {
-      p.each([&](W v, unsigned) { total += weights.of(v, best); });
-      total = p.cluster_sum(block_sum(total, s.sum));
-    }
-    Want want{by_count, set.top_k, set.top_p * (double)total};
-    p.histogram(bin, !by_count, weights);
+    u64 total = p.histogram(bin, !by_count, !by_count, weights);
+    if (!by_count) total = p.cluster_sum(block_sum(total, s.sum));
+    Want want = by_count ? want_count(set.top_k) : want_mass(set.top_p, total);
     auto found = p.find(want, 0, 0);
     if (found.above_count + found.in_bin <= kList) {
       // all that may be kept fits the list: the first block goes on by itself
@@ -747,7 +761,7 @@ __global__ void __launch_bounds__(kThreads)
       bool keep = threadIdx.x < count;
       if (by_count) {
         keep = keep && r.rank < set.top_k;
-        want = Want{false, 0, set.top_p * (double)block_sum(keep ? r.mass : 0, s.sum)};
+        want = want_mass(set.top_p, block_sum(keep ? r.mass : 0, s.sum));
       }
       keep = keep && (set.top_p >= 1 || want.inside(r.rank, r.before)) && (r.mass >= least || r.key == top);
       const u64 mass = keep ? r.mass : 0, target = target_of(random[g], block_sum(mass, s.sum));
@@ -766,8 +780,8 @@ __global__ void __launch_bounds__(kThreads)
       p.each([&](W v, unsigned i) {
         if (kept(Keys<W>::of(v), begin + i, cut)) sum += weights.of(v, best);
       });
-      want = Want{false, 0, set.top_p * (double)p.cluster_sum(block_sum(sum, s.sum))};
-      p.histogram(bin, true, weights);
+      want = want_mass(set.top_p, p.cluster_sum(block_sum(sum, s.sum)));
+      p.histogram(bin, true, false, weights);
       cut = p.cut(want, p.find(want, 0, 0), bin, weights);
     }
   }
@@ -797,7 +811,7 @@ cudaError_t launch_warps(const T *support, const float *random, unsigned groups,
   const bool whole = n % EACH == 0 && (reinterpret_cast<uintptr_t>(support) | n * sizeof(T)) % piece == 0;
   const unsigned most = 8 * (unsigned)sm_count(), blocks = (groups + kWarps - 1) / kWarps;
   return launch_next(sample_warp_kernel<T, EACH>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, support, random, groups, H, n, whole, s,
-                     mass_bits(n), codes);
+                     codes);
 }
 
 template <typename T, bool STAGED>
@@ -818,6 +832,7 @@ cudaError_t launch_blocks(const T *support, const float *random, unsigned groups
 template <typename T>
 cudaError_t launch_sample(const T *support, const float *random, long rows, long H, long Mc, Sampling s, long long *codes, cudaStream_t st) {
   const unsigned groups = (unsigned)(rows * H), n = (unsigned)Mc, h = (unsigned)H;
+  s.inv_t = inverse(s.temperature);
   cudaError_t e;
   if (n <= 32) {
     e = launch_warps<T, 1>(support, random, groups, h, n, s, codes, st);
