@@ -163,7 +163,7 @@ constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 constexpr int kWarpBits = 48;   // q: the sum of a lane's 16 masses stays below 2^54
 
 template <typename Key>
-struct Few {   // the units a cut lies among
+struct alignas(16) Few {   // the units a cut lies among
   Key key[32];
   u64 mass[32];
   unsigned index[32];
@@ -178,7 +178,8 @@ struct WarpGroup {
 
   __device__ __forceinline__ unsigned first() const { return (threadIdx.x & 31) * EACH; }
 
-  __device__ __forceinline__ Cut<Key> cut(const Want &want, Key best, Few<Key> &few) const {
+  // `behind`: units of at most this mass are behind the cut.
+  __device__ __forceinline__ Cut<Key> cut(const Want &want, u64 behind, Key best, Few<Key> &few) const {
     const unsigned lane = threadIdx.x & 31;
     // units in [lo, hi], units above; those at -infinity, which are never drawn, are out of it
     const Key none = Keys<W>::of((W)-INFINITY);
@@ -186,11 +187,10 @@ struct WarpGroup {
     unsigned to_lo = 0, above_count = 0;   // units from lo up, from above hi up
 #pragma unroll
     for (int r = 0; r < EACH; ++r)
-      if (key[r] > none) {
-        lo = min(lo, key[r]);
-        to_lo += 1;
-      }
+      if (key[r] > none && (want.by_count || mass[r] > behind)) lo = min(lo, key[r]);
     lo = warp_min(lo);
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) to_lo += key[r] >= lo;
     to_lo = __reduce_add_sync(0xffffffffu, to_lo);
     u64 above_mass = 0;
     for (int round = 0; to_lo - above_count > 32 && lo < hi; ++round) {
@@ -243,12 +243,18 @@ struct WarpGroup {
           few.index[at] = first() + q;
           ++at;
         }
+      if (lane >= in) few.key[lane] = 0;   // (no unit's key)
       __syncwarp();
-      const Key k = lane < in ? few.key[lane] : 0;   // (no unit's key)
+      const Key k = few.key[lane];
       const u64 m = lane < in ? few.mass[lane] : 0;
-      unsigned rank = 0;
-#pragma unroll 8
-      for (unsigned j = 0; j < in; ++j) rank += few.key[j] >= k + (j >= lane);
+      unsigned rank = __popc(__match_any_sync(0xffffffffu, k) & ((1u << lane) - 1));
+      constexpr int V = 16 / (int)sizeof(Key);
+#pragma unroll
+      for (int j = 0; j < 32; j += V) {
+        const Vec<Key, V> o = *reinterpret_cast<const Vec<Key, V> *>(&few.key[j]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) rank += o.v[i] > k;
+      }
       __syncwarp();
       if (lane < in) few.mass[rank] = m;
       __syncwarp();
@@ -272,6 +278,276 @@ struct WarpGroup {
   }
 };
 
+// A lane's units, NaN as -infinity.
+template <typename T, int EACH>
+__device__ __forceinline__ void load_units(const T *x, unsigned n, bool whole, Wide<T> (&v)[EACH]) {
+  using W = Wide<T>;
+  const unsigned first = (threadIdx.x & 31) * EACH;
+  if (whole) {   // rows and lanes' parts start on boundaries, and a lane's part is the group's or not
+    constexpr int V = EACH * (int)sizeof(T) <= 16 ? EACH : 16 / (int)sizeof(T);
+#pragma unroll
+    for (int r = 0; r < EACH; r += V) {
+      if (first < n) {
+        const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(x + first + r);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[r + i] = no_nan(widen(a.v[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[r + i] = (W)-INFINITY;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) v[r] = first + r < n ? no_nan(widen(x[first + r])) : (W)-INFINITY;
+  }
+}
+
+// The unit drawn from one group, or -1; the same for all lanes.
+template <typename T, int EACH>
+__device__ __noinline__ int draw_exactly(const T *x, unsigned n, bool whole, const Settings &set, float random, const double *table,
+                                         Few<typename Keys<Wide<T>>::type> &few) {
+  using W = Wide<T>;
+  using Key = typename Keys<W>::type;
+  const unsigned lane = threadIdx.x & 31;
+  W v[EACH];
+  load_units<T, EACH>(x, n, whole, v);
+  WarpGroup<W, EACH> group;
+  Key top = 0;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    group.key[r] = Keys<W>::of(v[r]);
+    top = max(top, group.key[r]);
+  }
+  top = warp_max(top);
+  const W best = Keys<W>::value(top);
+  if (!(best > (W)-INFINITY)) return -1;
+  if (set.top_k == 1) {
+    unsigned index = n;
+#pragma unroll
+    for (int r = EACH - 1; r >= 0; --r)
+      if (group.key[r] == top) index = lane * EACH + r;
+    return (int)warp_min(index);
+  }
+  const Weights weights(table, set.inv_t, kWarpBits);
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) group.mass[r] = weights.of(v[r], best);
+  Cut<Key> cut{0, n, 0};
+  if (set.top_k < n) cut = group.cut(want_count(set.top_k), 0, top, few);
+  if (set.top_p < 1) {
+    if (set.top_k >= n) {
+#pragma unroll
+      for (int r = 0; r < EACH; ++r) cut.mass += group.mass[r];
+      cut.mass = warp_sum_54(cut.mass);
+    }
+    // Units of at most 1/n of what may be left out are, all of them together, no more than that.
+    const Want want = want_mass(set.top_p, cut.mass);
+    cut = group.cut(want, want.limit > 0 && want.limit < cut.mass ? (cut.mass - want.limit) / n : 0, top, few);
+  }
+  if (set.min_p > 0) {
+    const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+      if (group.mass[r] < least && group.key[r] != top) group.mass[r] = 0;
+  }
+  u64 total = 0;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    if (!kept(group.key[r], lane * EACH + r, cut)) group.mass[r] = 0;
+    total += group.mass[r];
+  }
+  const u64 up_to = warp_up_to(total);
+  const u64 target = target_of(random, __shfl_sync(0xffffffffu, up_to, 31));
+  const unsigned who = __ffs(__ballot_sync(0xffffffffu, up_to > target)) - 1;
+  u64 run = up_to - total;
+  unsigned index = lane * EACH;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    run += group.mass[r];
+    index += run <= target;
+  }
+  return (int)__shfl_sync(0xffffffffu, index, who);
+}
+
+// The same in 32 bits, with a bound on what that can be off: where a decision lies within the bound the draw is in doubt, and is
+// made again in 64 bits.  With 100 units that is one draw in some thousands; the others cost a third of the instructions.
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+__device__ __forceinline__ float warp_min(float v) { return -warp_max(-v); }
+__device__ __forceinline__ float warp_sum(float v) {
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+struct FewFloats {
+  float key[32], mass[32];
+  unsigned index[32];
+};
+
+template <int EACH>
+struct QuickGroup {
+  float v[EACH], w[EACH];   // w = exp((v - best) / t), the largest 1
+  float error;              // bound on a sum's
+  bool doubt;
+
+  __device__ __forceinline__ unsigned first() const { return (threadIdx.x & 31) * EACH; }
+  __device__ __forceinline__ bool kept(int r, float value, unsigned index) const { return v[r] > value || (v[r] == value && first() + r <= index); }
+  // value, index: the last unit kept; returns the mass up to it.  `limit`: by mass, else the first `count`.
+  __device__ __forceinline__ float cut(bool by_count, unsigned count, float limit, float behind, float best, FewFloats &few, float &value, unsigned &index) {
+    const unsigned lane = threadIdx.x & 31;
+    auto inside = [&](unsigned c, float m) {
+      if (by_count) return c < count;
+      doubt = doubt || fabsf(m - limit) <= error;
+      return m < limit;
+    };
+    float lo = INFINITY, hi = best, above = 0;
+    unsigned to_lo = 0, above_count = 0;
+#pragma unroll
+    for (int r = 0; r < EACH; ++r)
+      if (v[r] > -INFINITY && (by_count || w[r] > behind)) lo = fminf(lo, v[r]);
+    lo = warp_min(lo);
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) to_lo += v[r] >= lo;
+    to_lo = __reduce_add_sync(0xffffffffu, to_lo);
+    for (int round = 0; to_lo - above_count > 32 && !doubt; ++round) {
+      const float pivot = 0.5f * lo + 0.5f * hi;
+      unsigned c = 0;
+      float m = 0;
+#pragma unroll
+      for (int r = 0; r < EACH; ++r)
+        if (v[r] >= pivot) c += 1, m += w[r];
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (!by_count) m = warp_sum(m);
+      // (equal values, or values far from evenly spread, are left to the exact form)
+      doubt = doubt || !(pivot > lo && pivot < hi) || round > 8;
+      if (c < to_lo && inside(c, m)) {
+        above_count = c;
+        above = m;
+        hi = pivot;   // units at the pivot itself have been counted
+        hi = __uint_as_float(pivot > 0 ? __float_as_uint(pivot) - 1 : pivot < 0 ? __float_as_uint(pivot) + 1 : 0x80000001u);
+      } else {
+        to_lo = c;
+        lo = pivot;
+      }
+    }
+    if (doubt) return 0;
+    const unsigned in = to_lo - above_count;
+    unsigned c = 0;
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) c += v[q] >= lo && v[q] <= hi;
+    unsigned at = warp_up_to(c) - c;
+#pragma unroll
+    for (int q = 0; q < EACH; ++q)
+      if (v[q] >= lo && v[q] <= hi) {
+        few.key[at] = v[q];
+        few.mass[at] = w[q];
+        few.index[at] = first() + q;
+        ++at;
+      }
+    if (lane >= in) few.key[lane] = -INFINITY;
+    __syncwarp();
+    const float k = few.key[lane], m = lane < in ? few.mass[lane] : 0;
+    unsigned rank = __popc(__match_any_sync(0xffffffffu, k) & ((1u << lane) - 1));
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 o = *reinterpret_cast<const float4 *>(&few.key[j]);
+      rank += o.x > k;
+      rank += o.y > k;
+      rank += o.z > k;
+      rank += o.w > k;
+    }
+    __syncwarp();
+    if (lane < in) few.mass[rank] = m;
+    __syncwarp();
+    const float by_rank = lane < in ? few.mass[lane] : 0, up_to = above + warp_up_to(by_rank), before = up_to - by_rank;
+    // (the very first is kept by definition)
+    const bool in_it = lane < in && (above_count + lane == 0 || inside(above_count + lane, before));
+    const unsigned last = __popc(__ballot_sync(0xffffffffu, in_it)) - 1;
+    const unsigned who = __ffs(__ballot_sync(0xffffffffu, lane < in && rank == last)) - 1;
+    value = __shfl_sync(0xffffffffu, k, who);
+    index = few.index[who & 31];
+    const float mass = __shfl_sync(0xffffffffu, up_to, last & 31);
+    doubt = __any_sync(0xffffffffu, doubt);
+    __syncwarp();
+    if (!by_count) return mass;
+    float all = 0;
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) all += kept(q, value, index) ? w[q] : 0;
+    return warp_sum(all);
+  }
+};
+
+// The unit, or -1; -2 in doubt.
+template <int EACH>
+__device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, const Settings &set, float random, FewFloats &few) {
+  const unsigned lane = threadIdx.x & 31;
+  float best = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) best = fmaxf(best, g.v[r]);
+  best = warp_max(best);
+  if (best == -INFINITY) return -1;
+  if (set.top_k == 1) {
+    unsigned index = n;
+#pragma unroll
+    for (int r = EACH - 1; r >= 0; --r)
+      if (g.v[r] == best) index = lane * EACH + r;
+    return (int)__reduce_min_sync(0xffffffffu, index);
+  }
+  const float c = (float)(set.inv_t * 1.4426950408889634);
+  if (best == INFINITY || !(c < 1e30f)) return -2;
+  float total = 0;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(g.w[r]) : "f"((g.v[r] - best) * c));
+    total += g.w[r];
+  }
+  // A weight is off by 2^-22 of it (ex2.approx) and by 3 x 2^-24 = 1.8e-7 for every unit x of its exponent: x exp(-x) is below 0.37, so
+  // by less than 3.1e-7 of the largest weight, 1, and, where it counts at all (x < 40), by 7.4e-6 of itself.  The 21 roundings on
+  // the way through a sum are 1.3e-6 of it.  Two sums are compared, one of them times a rounded factor.
+  total = warp_sum(total);
+  g.error = 2 * fminf(1.7e-6f * n, 9e-6f * total) + 3e-7f * total;
+  g.doubt = false;
+  float value = -INFINITY, mass = total;
+  unsigned index = n;
+  if (set.top_k < n) mass = g.cut(true, set.top_k, 0, 0, best, few, value, index);
+  if (set.top_p < 1 && !g.doubt) {
+    const float limit = (float)set.top_p * mass;
+    // units of at most 1/n of what may be left out are, all of them together, no more than that
+    const float behind = fmaxf(0.f, (mass - limit - 4 * g.error) / n);
+    mass = g.cut(false, 0, limit, set.top_k < n ? 0 : behind, best, few, value, index);
+  }
+  if (g.doubt) return -2;
+  if (set.min_p > 0) {
+    const float least = fminf((float)set.min_p, 1.f);
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      g.doubt = g.doubt || (fabsf(g.w[r] - least) <= 6e-6f * least && g.v[r] != best);
+      if (g.w[r] < least && g.v[r] != best) g.w[r] = 0;
+    }
+  }
+  float own = 0;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    if (!g.kept(r, value, index)) g.w[r] = 0;
+    own += g.w[r];
+  }
+  const float up_to = warp_up_to(own), all = __shfl_sync(0xffffffffu, up_to, 31), target = random * all, error = g.error;
+  // the borders of this lane's units, the one in front of them among these
+  float run = up_to - own;
+  bool doubt = g.doubt || !(random >= 0 && random < 1) || fabsf(run - target) <= error;
+  unsigned unit = lane * EACH;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    run += g.w[r];
+    doubt = doubt || fabsf(run - target) <= error;
+    unit += run <= target;
+  }
+  if (__any_sync(0xffffffffu, doubt)) return -2;
+  const unsigned who = __ffs(__ballot_sync(0xffffffffu, up_to > target)) - 1;
+  return (int)__shfl_sync(0xffffffffu, unit, who & 31);
+}
+
 template <typename T, int EACH>
 __global__ void __launch_bounds__(kWarpThreads)
     sample_warp_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned groups, unsigned H, unsigned n, bool whole,
@@ -279,86 +555,35 @@ __global__ void __launch_bounds__(kWarpThreads)
   after_previous();
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
+  constexpr bool QUICK = sizeof(W) == 4;
   __shared__ double s_table[kTable];
   __shared__ Few<Key> s_few[kWarps];
+  static_assert(sizeof(Few<Key>) >= sizeof(FewFloats), "one place for both");
   Weights::fill(s_table);
   __syncthreads();
-  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (unsigned g = blockIdx.x * kWarps + warp; g < groups; g += gridDim.x * kWarps) {
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = gridDim.x * kWarps, rows = step / H, rest = step % H;
+  const bool own = how.temperature_rows || how.top_k_rows || how.top_p_rows || how.min_p_rows;
+  Settings set;
+  if (!own) set = settings_of(how, 0, n);
+  unsigned g = blockIdx.x * kWarps + warp, row = g / H, h = g % H;
+  if (g >= groups) return;
+  W next[EACH];
+  if constexpr (QUICK) load_units<T, EACH>(support + (long)g * n, n, whole, next);
+  for (; g < groups; g += step, row += rows, h += rest) {
+    if (h >= H) h -= H, row += 1;
     const T *const x = support + (long)g * n;
-    WarpGroup<W, EACH> group;
-    W v[EACH];
-    if (whole) {   // rows and lanes' parts start on boundaries, and a lane's part is the group's or not
-      constexpr int V = EACH * (int)sizeof(T) <= 16 ? EACH : 16 / (int)sizeof(T);
+    if (own) set = settings_of(how, row, n);
+    const float u = random[g];
+    int unit = -2;
+    if constexpr (QUICK) {
+      QuickGroup<EACH> group;
 #pragma unroll
-      for (int r = 0; r < EACH; r += V) {
-        if (lane * EACH < n) {
-          const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(x + lane * EACH + r);
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[r + i] = no_nan(widen(a.v[i]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[r + i] = (W)-INFINITY;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < EACH; ++r) v[r] = lane * EACH + r < n ? no_nan(widen(x[lane * EACH + r])) : (W)-INFINITY;
+      for (int r = 0; r < EACH; ++r) group.v[r] = next[r] + 0.f;   // (no -0)
+      if (g + step < groups) load_units<T, EACH>(x + (long)step * n, n, whole, next);   // the next group is under way
+      unit = draw_quickly(group, n, set, u, reinterpret_cast<FewFloats &>(s_few[warp]));
     }
-    const unsigned row = g / H;
-    const Settings set = settings_of(how, row, n);
-    Key top = 0;
-#pragma unroll
-    for (int r = 0; r < EACH; ++r) {
-      group.key[r] = Keys<W>::of(v[r]);
-      top = max(top, group.key[r]);
-    }
-    top = warp_max(top);
-    const W best = Keys<W>::value(top);
-    long long code = -1;
-    if (best > (W)-INFINITY) {
-      if (set.top_k == 1) {
-        unsigned index = n;
-#pragma unroll
-        for (int r = EACH - 1; r >= 0; --r)
-          if (group.key[r] == top) index = lane * EACH + r;
-        code = warp_min(index);
-      } else {
-        const Weights weights(s_table, set.inv_t, kWarpBits);
-#pragma unroll
-        for (int r = 0; r < EACH; ++r) group.mass[r] = weights.of(v[r], best);
-        u64 total = 0;
-        Cut<Key> cut{0, n, 0};
-        if (set.top_k < n) cut = group.cut(want_count(set.top_k), top, s_few[warp]);
-        if (set.top_p < 1) {
-          if (set.top_k >= n) {
-#pragma unroll
-            for (int r = 0; r < EACH; ++r) cut.mass += group.mass[r];
-            cut.mass = warp_sum_54(cut.mass);
-          }
-          cut = group.cut(want_mass(set.top_p, cut.mass), top, s_few[warp]);
-        }
-        const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
-#pragma unroll
-        for (int r = 0; r < EACH; ++r) {
-          if (!(kept(group.key[r], lane * EACH + r, cut) && (group.mass[r] >= least || group.key[r] == top))) group.mass[r] = 0;
-          total += group.mass[r];
-        }
-        const u64 up_to = warp_up_to(total);
-        const u64 target = target_of(random[g], __shfl_sync(0xffffffffu, up_to, 31));
-        const unsigned who = __ffs(__ballot_sync(0xffffffffu, up_to > target)) - 1;
-        u64 run = up_to - total;
-        unsigned index = lane * EACH;
-#pragma unroll
-        for (int r = 0; r < EACH; ++r) {
-          run += group.mass[r];
-          index += run <= target;
-        }
-        code = __shfl_sync(0xffffffffu, index, who);
-      }
-      code += (long long)(g - row * H) * n;
-    }
-    if (lane == 0) codes[g] = code;
+    if (unit == -2) unit = draw_exactly<T, EACH>(x, n, whole, set, u, s_table, s_few[warp]);
+    if (lane == 0) codes[g] = unit < 0 ? -1ll : (long long)h * n + unit;
     __syncwarp();
   }
 }
