@@ -159,6 +159,10 @@ __device__ __forceinline__ u64 warp_min(u64 v) { return ~warp_max(~v); }
 
 // ---- a warp per group ------------------------------------------------------
 
+// Blocks on an SM, as registers allow; the launch has twice as many, since some draws take longer.
+template <int EACH>
+constexpr int kWarpBlocks = EACH <= 4 ? 4 : EACH <= 8 ? 3 : 2;
+
 constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 constexpr int kWarpBits = 48;   // q: the sum of a lane's 16 masses stays below 2^54
 
@@ -278,27 +282,25 @@ struct WarpGroup {
   }
 };
 
-// A lane's units, NaN as -infinity.
+// A lane's units as they are in memory; what is done to them waits until they are used.
 template <typename T, int EACH>
-__device__ __forceinline__ void load_units(const T *x, unsigned n, bool whole, Wide<T> (&v)[EACH]) {
-  using W = Wide<T>;
+__device__ __forceinline__ void load_units(const T *x, unsigned n, bool whole, T (&v)[EACH]) {
   const unsigned first = (threadIdx.x & 31) * EACH;
+  const T none = narrow_to<T>((Wide<T>)-INFINITY);
   if (whole) {   // rows and lanes' parts start on boundaries, and a lane's part is the group's or not
     constexpr int V = EACH * (int)sizeof(T) <= 16 ? EACH : 16 / (int)sizeof(T);
 #pragma unroll
     for (int r = 0; r < EACH; r += V) {
-      if (first < n) {
-        const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(x + first + r);
+      Vec<T, V> a;
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[r + i] = no_nan(widen(a.v[i]));
-      } else {
+      for (int i = 0; i < V; ++i) a.v[i] = none;
+      if (first < n) a = *reinterpret_cast<const Vec<T, V> *>(x + first + r);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[r + i] = (W)-INFINITY;
-      }
+      for (int i = 0; i < V; ++i) v[r + i] = a.v[i];
     }
   } else {
 #pragma unroll
-    for (int r = 0; r < EACH; ++r) v[r] = first + r < n ? no_nan(widen(x[first + r])) : (W)-INFINITY;
+    for (int r = 0; r < EACH; ++r) v[r] = first + r < n ? x[first + r] : none;
   }
 }
 
@@ -309,12 +311,14 @@ __device__ __noinline__ int draw_exactly(const T *x, unsigned n, bool whole, con
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
   const unsigned lane = threadIdx.x & 31;
+  T raw[EACH];
   W v[EACH];
-  load_units<T, EACH>(x, n, whole, v);
+  load_units<T, EACH>(x, n, whole, raw);
   WarpGroup<W, EACH> group;
   Key top = 0;
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
+    v[r] = no_nan(widen(raw[r]));
     group.key[r] = Keys<W>::of(v[r]);
     top = max(top, group.key[r]);
   }
@@ -549,7 +553,7 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
 }
 
 template <typename T, int EACH>
-__global__ void __launch_bounds__(kWarpThreads)
+__global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
     sample_warp_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned groups, unsigned H, unsigned n, bool whole,
                        const Sampling how, long long *__restrict__ codes) {
   after_previous();
@@ -567,7 +571,7 @@ __global__ void __launch_bounds__(kWarpThreads)
   if (!own) set = settings_of(how, 0, n);
   unsigned g = blockIdx.x * kWarps + warp, row = g / H, h = g % H;
   if (g >= groups) return;
-  W next[EACH];
+  T next[EACH];   // the next group's units, under way
   if constexpr (QUICK) load_units<T, EACH>(support + (long)g * n, n, whole, next);
   for (; g < groups; g += step, row += rows, h += rest) {
     if (h >= H) h -= H, row += 1;
@@ -578,8 +582,8 @@ __global__ void __launch_bounds__(kWarpThreads)
     if constexpr (QUICK) {
       QuickGroup<EACH> group;
 #pragma unroll
-      for (int r = 0; r < EACH; ++r) group.v[r] = next[r] + 0.f;   // (no -0)
-      if (g + step < groups) load_units<T, EACH>(x + (long)step * n, n, whole, next);   // the next group is under way
+      for (int r = 0; r < EACH; ++r) group.v[r] = no_nan(widen(next[r])) + 0.f;   // (no -0)
+      if (g + step < groups) load_units<T, EACH>(x + (long)step * n, n, whole, next);
       unit = draw_quickly(group, n, set, u, reinterpret_cast<FewFloats &>(s_few[warp]));
     }
     if (unit == -2) unit = draw_exactly<T, EACH>(x, n, whole, set, u, s_table, s_few[warp]);
@@ -1034,7 +1038,7 @@ cudaError_t launch_warps(const T *support, const float *random, unsigned groups,
                          cudaStream_t st) {
   constexpr size_t piece = EACH * sizeof(T) < 16 ? EACH * sizeof(T) : 16;
   const bool whole = n % EACH == 0 && (reinterpret_cast<uintptr_t>(support) | n * sizeof(T)) % piece == 0;
-  const unsigned most = 8 * (unsigned)sm_count(), blocks = (groups + kWarps - 1) / kWarps;
+  const unsigned most = 2 * kWarpBlocks<EACH> * (unsigned)sm_count(), blocks = (groups + kWarps - 1) / kWarps;
   return launch_next(sample_warp_kernel<T, EACH>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, support, random, groups, H, n, whole, s,
                      codes);
 }
