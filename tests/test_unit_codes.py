@@ -479,6 +479,12 @@ def test_distill_masks(mc, t):
     assert bool(torch.isnan(loss[9, 1])) and bool(torch.isnan(gradient[9, mc:]).all())
     assert_close(loss[9, :1], want[9, :1], loss_off[9, :1])
     assert_close(gradient[9, :mc], grad[9, :mc], grad_off[9, :mc] + rounding(t, grad[9, :mc]))
+    # ... also where there is nothing else, and one of the teacher's does too
+    x[0, :mc] = math.nan
+    teacher[3, 0, :] = math.nan
+    loss, gradient = k().distill_gradient(x.cuda(), h, mc, units.cuda(), teacher.cuda(), 1.5, weight.cuda())
+    assert bool(torch.isnan(loss[0, 0])) and bool(torch.isnan(gradient[0, :mc]).all())
+    assert bool(torch.isnan(loss[3, 0])) and bool(torch.isnan(gradient[3, :mc]).any())
 
 
 @gpu
