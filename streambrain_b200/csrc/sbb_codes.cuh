@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace sbb {
 
 void count_launches(int n);   // sbb_kernels.cu
@@ -47,6 +49,64 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
+
+// All of a vector's elements: 16-bit ones two at a time.
+template <typename T, int V>
+__device__ __forceinline__ void widen_all(const Vec<T, V> &a, Wide<T> (&f)[V]) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const unsigned two = reinterpret_cast<const unsigned *>(a.v)[i];
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[2 * i] = __uint_as_float(two << 16);
+        f[2 * i + 1] = __uint_as_float(two & 0xffff0000u);
+      } else {
+        const float2 both = __half22float2(*reinterpret_cast<const __half2 *>(&two));
+        f[2 * i] = both.x;
+        f[2 * i + 1] = both.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = widen(a.v[i]);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> narrow_all(const Wide<T> (&f)[V]) {
+  Vec<T, V> a;
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        reinterpret_cast<unsigned *>(a.v)[i] = *reinterpret_cast<const unsigned *>(&two);
+      } else {
+        const __half2 two = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        reinterpret_cast<unsigned *>(a.v)[i] = *reinterpret_cast<const unsigned *>(&two);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) a.v[i] = narrow_to<T>(f[i]);
+  }
+  return a;
+}
+// The largest element; a NaN is passed over.
+template <typename T, int V>
+__device__ __forceinline__ Wide<T> max_all(const Vec<T, V> &a) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m = *reinterpret_cast<const T2 *>(a.v);
+#pragma unroll
+    for (int i = 1; i < V / 2; ++i) m = __hmax2(m, *reinterpret_cast<const T2 *>(a.v + 2 * i));
+    return fmaxf(widen(m.x), widen(m.y));
+  } else {
+    Wide<T> m = widen(a.v[0]);
+#pragma unroll
+    for (int i = 1; i < V; ++i) m = fmax(m, widen(a.v[i]));
+    return m;
+  }
+}
 
 // How many elements one access may hold: 16 bytes where all rows start on such a boundary, two 16-bit elements where they start
 // on one of four bytes (a warp's request is then a whole line), else one.

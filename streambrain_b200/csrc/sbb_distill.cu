@@ -69,42 +69,50 @@ constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 
 // Lane l holds vectors l, l + 32, ... of V units each, NV of them.
 template <typename T, int V, int NV>
-__global__ void __launch_bounds__(kWarpThreads) distill_warp_kernel(const Distill<T> p) {
+__global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2) distill_warp_kernel(const Distill<T> p) {
   after_previous();
   using W = Wide<T>;
   __shared__ Vec<W, V> s_kept[kWarps][NV * 32];   // what the teacher gives each unit
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = gridDim.x * kWarps, rows = step / p.H, rest = step % p.H;
   W *const kept = s_kept[warp][0].v;
   unsigned g = blockIdx.x * kWarps + warp, row = g / p.H, h = g % p.H;
+  // the next group's units and teacher, under way while one is worked on
+  struct Ahead {
+    Vec<T, V> raw[NV];
+    unsigned u;
+    T t;
+  } next;
+  auto fetch = [&](unsigned i) {
+    const T *const x = p.support + (long)i * p.n;
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+      if ((r * 32 + lane) * V < p.n) next.raw[r] = *reinterpret_cast<const Vec<T, V> *>(x + (r * 32 + lane) * V);
+    if (lane < p.K) {
+      next.u = p.unit(i, lane);
+      next.t = p.teacher[(long)i * p.K + lane];
+    }
+  };
+  if (g < p.groups) fetch(g);
   for (; g < p.groups; g += step, row += rows, h += rest) {
     if (h >= p.H) h -= p.H, row += 1;
     const T *const x = p.support + (long)g * p.n;
     T *const out = p.gradient + (long)g * p.n;
     const W w = p.weight ? p.weight[row] : (W)1;
-    Vec<T, V> raw[NV];
     W e[NV][V], best = -INFINITY, total = 0, tbest = -INFINITY, ttotal = 0, sum = 0;
-    unsigned u0 = p.n;
-    W t0 = -INFINITY, x0 = 0;
+#pragma unroll
+    for (int r = 0; r < NV; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v) e[r][v] = (r * 32 + lane) * V < p.n ? widen(next.raw[r].v[v]) : (W)-INFINITY;
+    const unsigned u0 = lane < p.K ? next.u : p.n;
+    const W t0 = u0 < p.n ? widen(next.t) : (W)-INFINITY, x0 = u0 < p.n ? widen(x[u0]) : (W)0;
+    if (g + step < p.groups) fetch(g + step);
     if (w != (W)0) {
 #pragma unroll
       for (int r = 0; r < NV; ++r)
-        if ((r * 32 + lane) * V < p.n) raw[r] = *reinterpret_cast<const Vec<T, V> *>(x + (r * 32 + lane) * V);
-      if (lane < p.K) {
-        u0 = p.unit(g, lane);
-        if (u0 < p.n) {
-          t0 = widen(p.teacher[(long)g * p.K + lane]);
-          x0 = widen(x[u0]);
-        }
-      }
 #pragma unroll
-      for (int r = 0; r < NV; ++r)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          e[r][v] = (r * 32 + lane) * V < p.n ? widen(raw[r].v[v]) : (W)-INFINITY;
-          best = fmax(best, e[r][v]);
-        }
+        for (int v = 0; v < V; ++v) best = fmax(best, e[r][v]);
       best = warp_max(best);
-      if (u0 < p.n) tbest = t0;
+      tbest = t0;
       for (unsigned k = lane + 32; k < p.K; k += 32)
         if (p.unit(g, k) < p.n) tbest = fmax(tbest, widen(p.teacher[(long)g * p.K + k]));
       tbest = warp_max(tbest);
@@ -211,158 +219,190 @@ constexpr int kEntries = 512;        // kept units that wait in shared memory; t
 template <typename W>
 struct Running {
   W best, sum;
-  __device__ __forceinline__ void add(const Running &o, W c) {
-    const W b = fmax(best, o.best);
-    if (b == -INFINITY) {
-      sum += o.sum;   // (0, or a NaN)
-      return;
-    }
-    sum = (best == b ? sum : sum * expo(best - b, c)) + (o.best == b ? o.sum : o.sum * expo(o.best - b, c));
-    best = b;
+  __device__ __forceinline__ void move_to(W b, W c) {   // b: no less than best
+    if (best != b) sum *= expo(best - b, c), best = b;
+  }
+  __device__ __forceinline__ void add(W v, W c) {
+    if (v > best) move_to(v, c);
+    sum += v == best && v != -INFINITY ? (W)1 : v == -INFINITY ? (W)0 : expo(v - (best == -INFINITY ? (W)0 : best), c);
   }
 };
-template <typename W>
-__device__ __forceinline__ Running<W> warp_add(Running<W> r, W c) {
-  for (int off = 16; off > 0; off >>= 1) r.add(Running<W>{__shfl_xor_sync(0xffffffffu, r.best, off), __shfl_xor_sync(0xffffffffu, r.sum, off)}, c);
-  return r;
-}
 
 template <typename W>
 struct Block {
-  Running<W> part[kBlockWarps], own;
-  W sum[kBlockWarps];
-  W kept[kEntries];
-  unsigned unit[kEntries];
+  W best[2][kBlockWarps], sum[2][kBlockWarps], loss[kBlockWarps];
+  Running<W> own;
+  Vec<W, 2> kept[kEntries];   // unit (as bits), p
 };
 
+// Two of them over all threads; all have the same bits.  (Joining maxima and sums one by one took as long as a row of 32000 units
+// itself.)
 template <typename W>
-__device__ __forceinline__ W block_sum(W v, W *s) {
-  v = warp_sum(v);
+__device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Block<W> &s) {
+  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const W r_warp = warp_max(r.best), t_warp = warp_max(t.best);
+  if (lane == 0) s.best[0][warp] = r_warp, s.best[1][warp] = t_warp;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  r.move_to(warp_max(lane < kBlockWarps ? s.best[0][lane] : (W)-INFINITY), c);
+  t.move_to(warp_max(lane < kBlockWarps ? s.best[1][lane] : (W)-INFINITY), c);
+  const W r_sum = warp_sum(r.sum), t_sum = warp_sum(t.sum);
+  if (lane == 0) s.sum[0][warp] = r_sum, s.sum[1][warp] = t_sum;
   __syncthreads();
-  v = s[0];
-#pragma unroll
-  for (int i = 1; i < kBlockWarps; ++i) v += s[i];
-  return v;
-}
-// The same for a running maximum and sum; every warp's and every lane's order is the same, so all threads have the same bits.
-template <typename W>
-__device__ __forceinline__ Running<W> block_add(Running<W> r, W c, Running<W> *s) {
-  r = warp_add(r, c);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = r;
-  __syncthreads();
-  r = s[0];
-#pragma unroll
-  for (int i = 1; i < kBlockWarps; ++i) r.add(s[i], c);
-  return r;
+  r.sum = warp_sum(lane < kBlockWarps ? s.sum[0][lane] : (W)0);
+  t.sum = warp_sum(lane < kBlockWarps ? s.sum[1][lane] : (W)0);
 }
 
 // STAGED: the part waits in shared memory between the sum and the gradient; else (no gradient, or groups beyond what a cluster
-// holds) it is read again.  V: units of an access.
-template <typename T, int V, bool STAGED>
-__global__ void __launch_bounds__(kThreads) distill_block_kernel(const Distill<T> p, unsigned part) {
+// holds) it is read again.  VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last
+// one by single threads; else (support and gradient lie differently to the boundaries) element by element.
+template <typename T, bool VECTOR, bool STAGED>
+__global__ void __launch_bounds__(kThreads, 3) distill_block_kernel(const Distill<T> p, unsigned part) {
   after_previous();
   using W = Wide<T>;
+  constexpr int V = VECTOR ? 16 / (int)sizeof(T) : 1;
   extern __shared__ uint4 s_values[];
   __shared__ Block<W> s;
   cg::cluster_group cluster = cg::this_cluster();
-  const unsigned blocks = cluster.num_blocks(), g = blockIdx.x / blocks, rank = cluster.block_rank();
-  const unsigned begin = min(p.n, rank * part), size = min(part, p.n - begin), vectors = size / V;   // (V divides both)
+  const unsigned blocks = cluster.num_blocks(), g = blockIdx.x / blocks, rank = cluster.block_rank(), lane = threadIdx.x & 31;
+  const unsigned begin = min(p.n, rank * part), size = min(part, p.n - begin);
   const T *const x = p.support + (long)g * p.n + begin;
-  T *const out = p.gradient + (long)g * p.n + begin;
+  T *const out = p.gradient ? p.gradient + (long)g * p.n + begin : nullptr;
+  const unsigned lead = VECTOR ? min(size, (unsigned)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (unsigned)sizeof(T)) : 0;
+  const unsigned vectors = (size - lead) / V, tail = size - lead - vectors * V;
+  const unsigned single = threadIdx.x < lead ? threadIdx.x : threadIdx.x >= 32 && threadIdx.x - 32 < tail ? lead + vectors * V + threadIdx.x - 32 : size;
   Vec<T, V> *const stage = reinterpret_cast<Vec<T, V> *>(s_values);
+  const Vec<T, V> *const from = reinterpret_cast<const Vec<T, V> *>(x + lead);
   const W w = p.weight ? p.weight[g / p.H] : (W)1;
   Running<W> r{-INFINITY, 0}, t{-INFINITY, 0};
+  // the thread's first kept unit, under way while the row is read
+  unsigned u0 = p.n;
+  W t0 = 0, x0 = 0, own = 0;
   if (w != (W)0) {
+    if (threadIdx.x < p.K) {
+      u0 = p.unit(g, threadIdx.x);
+      t0 = widen(p.teacher[(long)g * p.K + threadIdx.x]);
+    }
+    if (single < size) own = widen(x[single]);
     constexpr int U = 4;
     for (unsigned i = threadIdx.x; i < vectors; i += U * kThreads) {
       Vec<T, V> a[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < vectors) a[u] = reinterpret_cast<const Vec<T, V> *>(x)[i + u * kThreads];
+        if (i + u * kThreads < vectors) a[u] = from[i + u * kThreads];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < vectors) {
-          if constexpr (STAGED) stage[i + u * kThreads] = a[u];
-          W m = widen(a[u].v[0]);
+      for (int u = 0; u < U; ++u) {
+        if (i + u * kThreads >= vectors) break;
+        if constexpr (STAGED) stage[i + u * kThreads] = a[u];
+        const W m = max_all(a[u]);
+        if (m > r.best) r.move_to(m, p.c);
+        const W b = r.best == -INFINITY ? (W)0 : r.best;
+        W f[V];
+        widen_all(a[u], f);
 #pragma unroll
-          for (int v = 1; v < V; ++v) m = fmax(m, widen(a[u].v[v]));
-          if (m > r.best) {
-            r.sum *= expo(r.best - m, p.c);   // (of -infinity: the sum is 0, or a NaN)
-            r.best = m;
-          }
-          const W from = r.best == -INFINITY ? (W)0 : r.best;
-#pragma unroll
-          for (int v = 0; v < V; ++v) r.sum += expo(widen(a[u].v[v]) - from, p.c);
-        }
-    }
-    r = block_add(r, p.c, s.part);
-    for (unsigned k = threadIdx.x; k < p.K; k += kThreads)
-      if (p.unit(g, k) < p.n) {
-        const W v = widen(p.teacher[(long)g * p.K + k]);
-        t.add(Running<W>{v, v == -INFINITY ? (W)0 : v == v ? (W)1 : v}, p.c);
+        for (int v = 0; v < V; ++v) r.sum += expo(f[v] - b, p.c);
       }
-    t = block_add(t, p.c, s.part);
+    }
+    if (single < size) r.add(own, p.c);
+    if (u0 < p.n) {
+      x0 = widen(p.support[(long)g * p.n + u0]);
+      t.add(t0, p.c);
+    }
+    for (unsigned k = threadIdx.x + kThreads; k < p.K; k += kThreads)
+      if (p.unit(g, k) < p.n) t.add(widen(p.teacher[(long)g * p.K + k]), p.c);
+    block_join(r, t, p.c, s);
     if (blocks > 1) {
       if (threadIdx.x == 0) s.own = r;
       cluster.sync();
-      r = cluster.map_shared_rank(&s, 0)->own;
-      for (unsigned b = 1; b < blocks; ++b) r.add(cluster.map_shared_rank(&s, b)->own, p.c);
+      W best = r.best;
+      for (unsigned b = 0; b < blocks; ++b) best = fmax(best, cluster.map_shared_rank(&s, b)->own.best);
+      W sum = 0;
+      for (unsigned b = 0; b < blocks; ++b) {
+        Running<W> o = cluster.map_shared_rank(&s, b)->own;
+        o.move_to(best, p.c);
+        sum += o.sum;
+      }
+      r = Running<W>{best, sum};
       cluster.sync();   // (a block may go on to its end, which the others read from)
     }
   }
   if (w == (W)0 || (r.best == -INFINITY && r.sum == (W)0) || (t.best == -INFINITY && t.sum == (W)0)) {
     if (rank == 0 && threadIdx.x == 0) p.loss[g] = 0;
-    if (p.gradient) {
+    if (out) {
       Vec<T, V> zero;
 #pragma unroll
       for (int v = 0; v < V; ++v) zero.v[v] = narrow_to<T>((W)0);
-      for (unsigned i = threadIdx.x; i < vectors; i += kThreads) reinterpret_cast<Vec<T, V> *>(out)[i] = zero;
+      for (unsigned i = threadIdx.x; i < vectors; i += kThreads) reinterpret_cast<Vec<T, V> *>(out + lead)[i] = zero;
+      if (single < size) out[single] = narrow_to<T>((W)0);
     }
     return;
   }
   const W inv = (W)1 / p.temperature, shift = sbb_log(r.sum) - sbb_log(t.sum), wt = w * p.temperature, scale = wt / r.sum, share = (W)1 / t.sum;
-  auto kept = [&](unsigned k) { return expo(widen(p.teacher[(long)g * p.K + k]) - t.best, p.c) * share; };
-  if (rank == 0) {
-    W sum = 0;
-    for (unsigned k = threadIdx.x; k < p.K; k += kThreads) {
-      const unsigned u = p.unit(g, k);
-      if (u >= p.n) continue;
-      const W z = widen(p.teacher[(long)g * p.K + k]) - t.best, pk = expo(z, p.c) * share;
-      if (!(pk == (W)0)) sum += pk * ((z - (widen(p.support[(long)g * p.n + u]) - r.best)) * inv + shift);
-    }
-    sum = block_sum(sum, s.sum);
-    if (threadIdx.x == 0) p.loss[g] = w * p.temperature * p.temperature * sum;
-  }
-  if (!p.gradient) return;
+  auto p_of = [&](W v) { return expo(v - t.best, p.c) * share; };
   const bool listed = p.K <= kEntries;
-  if (listed)
-    for (unsigned k = threadIdx.x; k < p.K; k += kThreads) {
-      const unsigned u = p.unit(g, k);
-      s.unit[k] = u;
-      s.kept[k] = u < p.n ? kept(k) : (W)0;
-    }
-  for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
-    const Vec<T, V> a = STAGED ? stage[i] : reinterpret_cast<const Vec<T, V> *>(x)[i];
-    Vec<T, V> o;
-#pragma unroll
-    for (int v = 0; v < V; ++v) o.v[v] = narrow_to<T>(expo(widen(a.v[v]) - r.best, p.c) * scale);
-    reinterpret_cast<Vec<T, V> *>(out)[i] = o;
-  }
-  __syncthreads();   // the kept units' elements are written again, each by the first entry that names it
-  for (unsigned k = threadIdx.x; k < p.K; k += kThreads) {
-    const unsigned u = listed ? s.unit[k] : p.unit(g, k);
-    if (u < begin || u >= begin + size) continue;
+  {
     W sum = 0;
-    bool first = true;
-    for (unsigned j = 0; j < p.K; ++j)
-      if ((listed ? s.unit[j] : p.unit(g, j)) == u) {
-        first = first && j >= k;
-        sum += listed ? s.kept[j] : kept(j);
+    for (unsigned k = threadIdx.x; k < p.K; k += kThreads) {
+      unsigned u = u0;
+      W v = t0, xu = x0;
+      if (k >= kThreads) {
+        u = p.unit(g, k);
+        if (u < p.n) v = widen(p.teacher[(long)g * p.K + k]), xu = widen(p.support[(long)g * p.n + u]);
       }
-    if (first) out[u - begin] = narrow_to<T>(expo(widen(p.support[(long)g * p.n + u]) - r.best, p.c) * scale - wt * sum);
+      const W pk = u < p.n ? p_of(v) : (W)0;
+      if (!(pk == (W)0)) sum += pk * (((v - t.best) - (xu - r.best)) * inv + shift);
+      if (listed) {
+        s.kept[k].v[1] = pk;
+        *reinterpret_cast<unsigned *>(&s.kept[k].v[0]) = u;
+      }
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) s.loss[threadIdx.x >> 5] = sum;
+  }
+  __syncthreads();
+  if (rank == 0 && threadIdx.x < 32) {
+    const W sum = warp_sum(lane < kBlockWarps ? s.loss[lane] : (W)0);
+    if (lane == 0) p.loss[g] = w * p.temperature * p.temperature * sum;
+  }
+  if (!out) return;
+  // What the teacher gives the unit of this thread's entry, if the entry is the first that names it; the parts in order.
+  auto given = [&](unsigned k, unsigned u, W &sum) {
+    bool first = true;
+    sum = 0;
+    for (unsigned j = 0; j < p.K; ++j) {
+      unsigned o;
+      W pj;
+      if (listed) {
+        const Vec<W, 2> e = s.kept[j];
+        o = *reinterpret_cast<const unsigned *>(&e.v[0]);
+        pj = e.v[1];
+      } else {
+        o = p.unit(g, j);
+        pj = o == u ? p_of(widen(p.teacher[(long)g * p.K + j])) : (W)0;
+      }
+      if (o == u) {
+        first = first && j >= k;
+        sum += pj;
+      }
+    }
+    return first;
+  };
+  W sum0 = 0;
+  const bool mine = u0 >= begin && u0 < begin + size && given(threadIdx.x, u0, sum0);
+  for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
+    W f[V];
+    widen_all(STAGED ? stage[i] : from[i], f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = expo(f[v] - r.best, p.c) * scale;
+    reinterpret_cast<Vec<T, V> *>(out + lead)[i] = narrow_all<T, V>(f);
+  }
+  if (single < size) out[single] = narrow_to<T>(expo(own - r.best, p.c) * scale);
+  __syncthreads();   // the kept units' elements are written again
+  if (mine) out[u0 - begin] = narrow_to<T>(expo(x0 - r.best, p.c) * scale - wt * sum0);
+  for (unsigned k = threadIdx.x + kThreads; k < p.K; k += kThreads) {
+    const unsigned u = p.unit(g, k);
+    W sum;
+    if (u >= begin && u < begin + size && given(k, u, sum))
+      out[u - begin] = narrow_to<T>(expo(widen(p.support[(long)g * p.n + u]) - r.best, p.c) * scale - wt * sum);
   }
 }
 
@@ -372,18 +412,18 @@ cudaError_t launch_warps(const Distill<T> &p, cudaStream_t st) {
   return launch_next(distill_warp_kernel<T, V, NV>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, p);
 }
 
-template <typename T, int V, bool STAGED>
+template <typename T, bool VECTOR, bool STAGED>
 cudaError_t launch_blocks(const Distill<T> &p, unsigned part, unsigned cluster, cudaStream_t st) {
   const size_t smem = STAGED ? (size_t)part * sizeof(T) : 0;
   if (smem > 0) {   // (holds for the current device)
-    const cudaError_t e = cudaFuncSetAttribute(distill_block_kernel<T, V, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    const cudaError_t e = cudaFuncSetAttribute(distill_block_kernel<T, VECTOR, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
     if (e != cudaSuccess) return e;
   }
-  return launch_clusters(distill_block_kernel<T, V, STAGED>, dim3(p.groups * cluster), dim3(cluster), kThreads, smem, st, p, part);
+  return launch_clusters(distill_block_kernel<T, VECTOR, STAGED>, dim3(p.groups * cluster), dim3(cluster), kThreads, smem, st, p, part);
 }
 
 template <typename T>
-cudaError_t launch_wide(const Distill<T> &p, int vec, cudaStream_t st) {
+cudaError_t launch_wide(const Distill<T> &p, cudaStream_t st) {
   const size_t bytes = (size_t)p.n * sizeof(T);
   unsigned cluster = 1;
   // the smallest cluster whose blocks hold their parts; a larger one where groups are too few for the SMs and parts long
@@ -393,9 +433,9 @@ cudaError_t launch_wide(const Distill<T> &p, int vec, cudaStream_t st) {
   const unsigned part = ((p.n + cluster - 1) / cluster + 15) / 16 * 16;
   if ((size_t)p.groups * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const bool staged = p.gradient && (size_t)part * sizeof(T) <= kStage;
-  constexpr int V = 16 / (int)sizeof(T);
-  if (vec == V) return staged ? launch_blocks<T, V, true>(p, part, cluster, st) : launch_blocks<T, V, false>(p, part, cluster, st);
-  return staged ? launch_blocks<T, 1, true>(p, part, cluster, st) : launch_blocks<T, 1, false>(p, part, cluster, st);
+  const bool vector = !p.gradient || ((reinterpret_cast<uintptr_t>(p.support) ^ reinterpret_cast<uintptr_t>(p.gradient)) & 15) == 0;
+  if (vector) return staged ? launch_blocks<T, true, true>(p, part, cluster, st) : launch_blocks<T, true, false>(p, part, cluster, st);
+  return staged ? launch_blocks<T, false, true>(p, part, cluster, st) : launch_blocks<T, false, false>(p, part, cluster, st);
 }
 
 }  // namespace
@@ -410,7 +450,7 @@ cudaError_t launch_distill(const T *support, const I *units, const T *teacher, c
   const int vec = vector_width<T>(Mc, support, gradient);
   cudaError_t e;
   if (Mc > 512) {
-    e = launch_wide(p, vec, st);
+    e = launch_wide(p, st);
   } else if (vec == V) {
     const long vectors = (Mc + 32 * V - 1) / (32 * V);
     if constexpr (V == 8) {
