@@ -154,45 +154,55 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
         e[r][v] = expo(e[r][v] - best, p.c);
         total += e[r][v];
       }
-    total = warp_sum(total);
-    const W p0 = u0 < p.n ? expo(t0 - tbest, p.c) : (W)0;
-    ttotal = p0;
-    for (unsigned k = lane + 32; k < p.K; k += 32)
-      if (p.unit(g, k) < p.n) ttotal += expo(widen(p.teacher[(long)g * p.K + k]) - tbest, p.c);
-    ttotal = warp_sum(ttotal);
-    const W inv = (W)1 / p.temperature, shift = sbb_log(total) - sbb_log(ttotal), share = (W)1 / ttotal;
-    for (unsigned k0 = 0; k0 < p.K; k0 += 32) {
-      const unsigned k = k0 + lane;
-      unsigned u = u0;
-      W t = t0, xu = x0, pk = p0;
-      if (k0 > 0) {
-        u = k < p.K ? p.unit(g, k) : p.n;
-        pk = 0;
-        if (u < p.n) {
-          t = widen(p.teacher[(long)g * p.K + k]);
-          xu = widen(x[u]);
-          pk = expo(t - tbest, p.c);
+    const W inv = (W)1 / p.temperature;
+    // the teacher's side without its divisor, so that three sums run side by side
+    auto entry = [&](bool there, W t, W xu) {
+      const W pk = there ? expo(t - tbest, p.c) : (W)0;
+      ttotal += pk;
+      if (!(pk == (W)0)) sum += pk * (((t - tbest) - (xu - best)) * inv);
+      return pk;
+    };
+    const W p0 = entry(u0 < p.n, t0, x0);
+    for (unsigned k = lane + 32; k < p.K; k += 32) {
+      const unsigned u = p.unit(g, k);
+      if (u < p.n) entry(true, widen(p.teacher[(long)g * p.K + k]), widen(x[u]));
+    }
+    for (int off = 16; off > 0; off >>= 1) {
+      total += __shfl_xor_sync(0xffffffffu, total, off);
+      ttotal += __shfl_xor_sync(0xffffffffu, ttotal, off);
+      sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    }
+    const W share = (W)1 / ttotal;
+    sum = sum * share + (sbb_log(total) - sbb_log(ttotal));
+    if (p.gradient)
+      for (unsigned k0 = 0; k0 < p.K; k0 += 32) {
+        unsigned u = u0;
+        W pk = p0;
+        if (k0 > 0) {
+          u = k0 + lane < p.K ? p.unit(g, k0 + lane) : p.n;
+          pk = u < p.n ? expo(widen(p.teacher[(long)g * p.K + k0 + lane]) - tbest, p.c) : (W)0;
         }
-      }
-      const bool there = u < p.n;
-      pk *= share;
-      if (there && !(pk == (W)0)) sum += pk * (((t - tbest) - (xu - best)) * inv + shift);
-      if (p.gradient) {
-        // a unit named twice has both parts, added in the order of the entries
-        const unsigned same = __match_any_sync(0xffffffffu, there ? u : ~lane);
-        W part = pk;
-        if (__any_sync(0xffffffffu, (same & (same - 1)) != 0)) {
-          part = 0;
+        pk *= share;
+        // A unit named twice has both parts, added in the order of the entries: whoever reads another's mark than its own has one.
+        const bool there = u < p.n;
+        W before = 0;
+        if (there && k0 > 0) before = kept[u];
+        __syncwarp();
+        if (there) kept[u] = (W)lane;
+        __syncwarp();
+        if (__any_sync(0xffffffffu, there && kept[u] != (W)lane)) {
+          const unsigned same = __match_any_sync(0xffffffffu, there ? u : ~lane);
+          W part = 0;
           for (int j = 0; j < 32; ++j) {
             const W o = __shfl_sync(0xffffffffu, pk, j);
             if (same >> j & 1) part += o;
           }
+          pk = part;
         }
-        if (there && __ffs(same) - 1 == (int)lane) kept[u] += part;
+        __syncwarp();
+        if (there) kept[u] = before + pk;   // (those that name the same unit write the same)
         __syncwarp();
       }
-    }
-    sum = warp_sum(sum);
     if (lane == 0) p.loss[g] = w * p.temperature * p.temperature * sum;
     if (!p.gradient) continue;
     const W wt = w * p.temperature, scale = wt / total;
@@ -269,7 +279,11 @@ __global__ void __launch_bounds__(kThreads, 3) distill_block_kernel(const Distil
   T *const out = p.gradient ? p.gradient + (long)g * p.n + begin : nullptr;
   const unsigned lead = VECTOR ? min(size, (unsigned)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (unsigned)sizeof(T)) : 0;
   const unsigned vectors = (size - lead) / V, tail = size - lead - vectors * V;
-  const unsigned single = threadIdx.x < lead ? threadIdx.x : threadIdx.x >= 32 && threadIdx.x - 32 < tail ? lead + vectors * V + threadIdx.x - 32 : size;
+  unsigned single = size;   // the thread's element outside the vectors
+  if constexpr (VECTOR) {
+    if (threadIdx.x < lead) single = threadIdx.x;
+    if (threadIdx.x - 32 < tail) single = lead + vectors * V + threadIdx.x - 32;   // (a warp of its own)
+  }
   Vec<T, V> *const stage = reinterpret_cast<Vec<T, V> *>(s_values);
   const Vec<T, V> *const from = reinterpret_cast<const Vec<T, V> *>(x + lead);
   const W w = p.weight ? p.weight[g / p.H] : (W)1;

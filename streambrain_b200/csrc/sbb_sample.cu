@@ -351,7 +351,7 @@ __device__ __noinline__ int draw_exactly(const T *x, unsigned n, bool whole, con
     const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
 #pragma unroll
     for (int r = 0; r < EACH; ++r)
-      if (group.mass[r] < least && group.key[r] != top) group.mass[r] = 0;
+      if (group.mass[r] < least) group.mass[r] = 0;
   }
   u64 total = 0;
 #pragma unroll
@@ -595,17 +595,19 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
 // ---- a cluster per group ---------------------------------------------------
 
 constexpr int kThreads = 512, kBlockWarps = kThreads / 32, kBins = 2048, kBinsEach = kBins / kThreads, kList = 512;
-constexpr int kMostBlocks = 8;      // of a cluster
+constexpr int kMostBlocks = 8;       // of a cluster
 constexpr int kStage = 64 * 1024;    // bytes of a group that a block keeps in shared memory
+constexpr unsigned kQuickCount = 256;   // a top-k of up to this many goes by the threads' maxima
 
 struct Block {
   unsigned bin_count[kBins], bin_low[kBins], bin_high[kBins];   // masses in halves
   u64 list_key[kList], list_mass[kList], sorted_mass[kList];
-  unsigned list_index[kList], sorted_index[kList];
+  unsigned list_index[kList];
   double table[kTable];
   u64 sum[kBlockWarps];
-  u64 part[4];        // what a block tells the others
-  u64 found[4];       // what the first block finds: bin, and the count, mass and units of the bin in front
+  u64 swap[2][2];     // what a block tells the others, in turn
+  u64 unit;           // what one block finds for all
+  u64 found[4];       // what the first block finds: a bin, the count and mass in front of it, the units in it; or a cut
   unsigned list;      // units in the list
   int bin;
 
@@ -645,92 +647,128 @@ __device__ __forceinline__ u64 block_before(u64 v, u64 *s) {
   return base + in - v;
 }
 
-// The part of a group that a block works on: units [begin, begin + size) of `n`.
+// The part of a group that a block works on: units [begin, begin + size), as elements [lead, lead + size) of `vectors` vectors.
+// Elements around them are -infinity (in shared memory, STAGED) or do not exist (V = 1).
 template <typename T, bool STAGED>
 struct Part {
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
   static constexpr int V = STAGED ? 16 / (int)sizeof(T) : 1;
-  const T *x;   // of unit `begin`; in shared memory and filled up to a whole vector with -infinity where STAGED
-  unsigned begin, size, n;
+  const Vec<T, V> *x;
+  unsigned begin, size, lead, vectors;
   W best;
   Block &s;
   cg::cluster_group cluster;
+  int turn;
 
-  __device__ __forceinline__ W value(unsigned i) const { return no_nan(widen(x[i])); }
-  // f(value, index in the part) for every unit above -infinity
+  // f(value, unit) for every unit above -infinity (no NaN is) of vectors [lo, hi), `step` apart
+  template <typename F>
+  __device__ __forceinline__ void each(unsigned lo, unsigned hi, unsigned step, F f) const {
+    for (unsigned i = lo; i < hi; i += step) {
+      W w[V];
+      widen_all(x[i], w);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (w[v] > (W)-INFINITY) f(w[v], begin + i * V + v - lead);
+    }
+  }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    for (unsigned i = threadIdx.x * V; i < size; i += kThreads * V) {
-      const Vec<T, V> a = *reinterpret_cast<const Vec<T, V> *>(x + i);
+    each(threadIdx.x, vectors, kThreads, f);
+  }
+  // The same for units of at least `low`, where they are few.
+  template <typename F>
+  __device__ __forceinline__ void each_from(W low, F f) const {
+    for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
+      const Vec<T, V> a = x[i];
+      if (!(max_all(a) >= low)) continue;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const W w = no_nan(widen(a.v[v]));
-        if (w > (W)-INFINITY) f(w, i + v);
+        const W w = widen(a.v[v]);
+        if (w >= low && w > (W)-INFINITY) f(w, begin + i * V + v - lead);
       }
     }
-  }
-  __device__ __forceinline__ u64 cluster_sum(u64 v) {   // of a value of each block
-    if (cluster.num_blocks() == 1) return v;
-    __syncthreads();
-    if (threadIdx.x == 0) s.part[0] = v;
-    cluster.sync();
-    v = 0;
-    for (unsigned b = 0; b < cluster.num_blocks(); ++b) v += cluster.map_shared_rank(&s, b)->part[0];
-    cluster.sync();
-    return v;
-  }
-  __device__ __forceinline__ u64 cluster_max(u64 v) {
-    if (cluster.num_blocks() == 1) return v;
-    __syncthreads();
-    if (threadIdx.x == 0) s.part[0] = v;
-    cluster.sync();
-    v = 0;
-    for (unsigned b = 0; b < cluster.num_blocks(); ++b) v = max(v, cluster.map_shared_rank(&s, b)->part[0]);
-    cluster.sync();
-    return v;
   }
 
-  // The first unit at which the running sum of weigh(value, index) passes `target`, below the sum of all (which is `all` of this
-  // part); known to every block.
+  // f(a, b) of every block's two values, in the blocks' order.
+  // (Two places in turn: one is written again only behind another exchange's barrier.)
   template <typename F>
-  __device__ unsigned locate(F weigh, u64 target) {
-    const unsigned each_warp = (size + kBlockWarps - 1) / kBlockWarps, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned lo = min(size, warp * each_warp), hi = min(size, lo + each_warp);
-    u64 mine = 0;
-    for (unsigned i = lo + lane; i < hi; i += 32) mine += weigh(value(i), begin + i);
-    mine = warp_sum(mine);
-    __syncthreads();
-    if (lane == 0) s.sum[warp] = mine;
-    __syncthreads();
-    u64 before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kBlockWarps; ++w) {
-      before += w < (int)warp ? s.sum[w] : 0;
-      all += s.sum[w];
+  __device__ __forceinline__ void exchange(u64 a, u64 b, F f) {
+    if (cluster.num_blocks() == 1) {
+      f(a, b);
+      return;
     }
-    if (threadIdx.x == 0) s.part[0] = all;
+    if (threadIdx.x == 0) s.swap[turn][0] = a, s.swap[turn][1] = b;
     cluster.sync();
-    for (unsigned b = 0; b < cluster.block_rank(); ++b) before += cluster.map_shared_rank(&s, b)->part[0];
-    if (before <= target && target < before + mine)
-      for (unsigned i0 = lo; i0 < hi; i0 += 32) {
-        const u64 up_to = warp_up_to(i0 + lane < hi ? weigh(value(i0 + lane), begin + i0 + lane) : (u64)0);
-        const unsigned past = __ballot_sync(0xffffffffu, before + up_to > target);
-        if (past) {
-          const u64 unit = begin + i0 + __ffs(past) - 1;
-          if (lane < cluster.num_blocks()) cluster.map_shared_rank(&s, lane)->part[1] = unit;
-          break;
+    for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
+      const Block *const other = cluster.map_shared_rank(&s, o);
+      f(other->swap[turn][0], other->swap[turn][1]);
+    }
+    turn ^= 1;
+  }
+  __device__ __forceinline__ u64 cluster_sum(u64 v) {   // of a value of each block
+    u64 all = 0;
+    exchange(v, 0, [&](u64 a, u64) { all += a; });
+    return all;
+  }
+
+  // The first unit at which the running sum of weigh(value, unit) passes target(sum of all), which is below that sum; known to every
+  // block when all have passed a barrier of the cluster.
+  template <typename F, typename G>
+  __device__ void locate(F weigh, G target) {
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned lo = 0, hi = vectors;
+    auto by_warp = [&](u64 &all) {   // sums of the warps' shares of vectors [lo, hi)
+      const unsigned share = (hi - lo + kBlockWarps - 1) / kBlockWarps, from = min(hi, lo + warp * share);
+      u64 mine = 0;
+      each(from + lane, min(hi, from + share), 32, [&](W v, unsigned i) { mine += weigh(v, i); });
+      mine = warp_sum(mine);
+      __syncthreads();
+      if (lane == 0) s.sum[warp] = mine;
+      __syncthreads();
+      all = 0;
+#pragma unroll
+      for (int w = 0; w < kBlockWarps; ++w) all += s.sum[w];
+      return share;
+    };
+    u64 all;
+    unsigned share = by_warp(all);
+    u64 total = 0, before = 0;
+    unsigned o = 0;
+    exchange(all, 0, [&](u64 a, u64) {
+      if (o++ < cluster.block_rank()) before += a;
+      total += a;
+    });
+    const u64 at = target(total);
+    if (at < before || at >= before + all) return;
+    for (;;) {   // the share that it lies in
+      unsigned w = 0;
+      while (before + s.sum[w] <= at) before += s.sum[w++];
+      lo = min(hi, lo + w * share);
+      hi = min(hi, lo + share);
+      if (hi - lo <= kThreads) break;
+      share = by_warp(all);
+    }
+    u64 mine = 0;
+    const unsigned i = lo + threadIdx.x;
+    each(i, min(hi, i + 1), 1, [&](W v, unsigned j) { mine += weigh(v, j); });
+    u64 run = before + block_before(mine, s.sum);
+    if (run <= at && at < run + mine) {
+      bool found = false;
+      each(i, i + 1, 1, [&](W v, unsigned j) {
+        run += weigh(v, j);
+        if (!found && run > at) {
+          found = true;
+          for (unsigned b = 0; b < cluster.num_blocks(); ++b) cluster.map_shared_rank(&s, b)->unit = j;
         }
-        before += __shfl_sync(0xffffffffu, up_to, 31);
-      }
-    cluster.sync();
-    return (unsigned)s.part[1];
+      });
+    }
   }
 
   // Fills the bins: bin_of(value) in [0, kBins) or -1, masses where `masses` is set; the first block gets the sums of all.  Returns
   // this thread's sum of the masses of all units, `total` asked for.
   // Masses are added in halves with a carry: an addition of 64 bits to shared memory is a loop, and where values are equal
-  // (16-bit types) a long one: 256 rows of 128000 bf16 units, a few of them without a top-k, 1030 us.
+  // (16-bit types) a long one: 256 rows of 128000 bf16 units, a few of them without a top-k, 1030 us (560 so).
   template <typename F>
   __device__ u64 histogram(F bin_of, bool masses, bool total, const Weights &weights) {
     __syncthreads();
@@ -749,7 +787,7 @@ struct Part {
       if (high) atomicAdd(&s.bin_high[b], high);
     });
     cluster.sync();
-    if (cluster.block_rank() == 0)
+    if (cluster.block_rank() == 0 && cluster.num_blocks() > 1)
       for (int b = threadIdx.x; b < kBins; b += kThreads) {
         unsigned c = s.bin_count[b];
         u64 m = s.mass(b);
@@ -780,8 +818,8 @@ struct Part {
         c += s.bin_count[threadIdx.x * kBinsEach + j];
         m += s.mass(threadIdx.x * kBinsEach + j);
       }
-      u64 cb = above_count + block_before(c, s.sum), mb = above_mass + block_before(m, s.sum);
-      const u64 c0 = cb, m0 = mb;
+      const u64 c0 = above_count + block_before(c, s.sum), m0 = above_mass + block_before(m, s.sum);
+      u64 cb = c0, mb = m0;
 #pragma unroll
       for (int j = 0; j < kBinsEach; ++j) {
         const int b = threadIdx.x * kBinsEach + j;
@@ -808,24 +846,17 @@ struct Part {
     const Found f{(int)s.found[0], (unsigned)s.found[3], (unsigned)s.found[1], s.found[2]};
     return f;
   }
-  // Puts the units that `want`s into the first block's list, which has room for them; returns their number to that block.
-  template <typename F>
-  __device__ unsigned gather(F wanted, const Weights &weights) {
+  // Puts a unit into the first block's list while there is room; s.list there counts all.  (It is 0 at first; the first block sets it
+  // back to 0 ahead of a barrier of the cluster.)
+  __device__ __forceinline__ void put(W v, unsigned unit, const Weights &weights) {
     Block *const first = cluster.map_shared_rank(&s, 0);
-    if (cluster.block_rank() == 0 && threadIdx.x == 0) s.list = 0;
-    cluster.sync();
-    each([&](W v, unsigned i) {
-      if (!wanted(v)) return;
-      const unsigned at = atomicAdd(&first->list, 1u);
-      if (at >= kList) return;
-      first->list_key[at] = Keys<W>::of(v);
-      first->list_index[at] = begin + i;
-      first->list_mass[at] = weights.of(v, best);
-    });
-    cluster.sync();
-    return cluster.block_rank() == 0 ? s.list : 0;
+    const unsigned at = atomicAdd(&first->list, 1u);
+    if (at >= kList) return;
+    first->list_key[at] = Keys<W>::of(v);
+    first->list_index[at] = unit;
+    first->list_mass[at] = weights.of(v, best);
   }
-  // The first block's list in order; a thread's entry, its rank and what lies in front of it.
+  // The first block's list: a thread's entry, its rank in the order and what lies in front of it.
   struct Ranked {
     Key key;
     unsigned index, rank;
@@ -839,6 +870,7 @@ struct Part {
       r.index = s.list_index[threadIdx.x];
       r.mass = s.list_mass[threadIdx.x];
       r.rank = 0;
+#pragma unroll 4
       for (unsigned j = 0; j < count; ++j) {
         const Key o = (Key)s.list_key[j];
         r.rank += o > r.key || (o == r.key && s.list_index[j] < r.index);
@@ -852,6 +884,28 @@ struct Part {
     __syncthreads();
     if (threadIdx.x < count) r.before = s.sorted_mass[r.rank];
     return r;
+  }
+  // The unit drawn from the first block's list, which holds all that may be kept; by that block alone.
+  __device__ void draw(unsigned count, const Settings &set, unsigned n, u64 least, float random, long long base, long long *code) {
+    const Ranked r = rank(count);
+    bool keep = threadIdx.x < count;
+    u64 all = 0;
+    if (set.top_k < n) {
+      keep = keep && r.rank < set.top_k;
+      if (set.top_p < 1) all = block_sum(keep ? r.mass : 0, s.sum);
+    } else {
+      all = s.found[3];
+    }
+    if (set.top_p < 1) keep = keep && want_mass(set.top_p, all).inside(r.rank, r.before);
+    keep = keep && r.mass >= least;   // (the largest have 2^q, which is no less)
+    const u64 mass = keep ? r.mass : 0, target = target_of(random, block_sum(mass, s.sum));
+    if (threadIdx.x < count) s.list_mass[threadIdx.x] = mass;
+    __syncthreads();
+    if (mass == 0) return;
+    u64 before = 0;
+#pragma unroll 4
+    for (unsigned j = 0; j < count; ++j) before += s.list_index[j] < r.index ? s.list_mass[j] : 0;
+    if (before <= target && target < before + mass) *code = base + r.index;
   }
 
   // The cut that `want` asks for among all units: bins of equal width in the value's distance from the largest first (`found`, by
@@ -875,9 +929,10 @@ struct Part {
           high = max(high, k);
         }
       });
-      high = (Key)cluster_max(block_max(high, s.sum));
-      low = ~(Key)cluster_max(block_max((Key)~low, s.sum));
-      lo = low, hi = high;
+      const Key high_here = block_max(high, s.sum), low_here = block_max((Key)~low, s.sum);
+      high = 0, low = 0;
+      exchange(high_here, low_here, [&](u64 a, u64 b) { high = max(high, (Key)a), low = max(low, (Key)b); });
+      lo = (Key)~low, hi = high;
       if (lo == hi) break;
       int shift = 0;
       while (((hi - lo) >> shift) >= (Key)kBins) ++shift;
@@ -894,14 +949,21 @@ struct Part {
       const u64 m = weights.of(Keys<W>::value(hi), best);
       const unsigned take = equal_ones(want, in, m, above_count, above_mass);
       const Key key = hi;
-      const unsigned index = locate([&](W v, unsigned) { return (u64)(Keys<W>::of(v) == key); }, take - 1);
-      return Cut<Key>{key, index, above_mass + take * m};
+      locate([&](W v, unsigned) { return (u64)(Keys<W>::of(v) == key); }, [&](u64) { return (u64)(take - 1); });
+      cluster.sync();
+      return Cut<Key>{key, (unsigned)s.unit, above_mass + take * m};
     }
-    const unsigned count = gather(among, weights);
+    cluster.sync();   // (the list is empty)
+    each([&](W v, unsigned i) {
+      if (among(v)) put(v, i, weights);
+    });
+    cluster.sync();
     if (cluster.block_rank() == 0) {
+      const unsigned count = s.list;
       const Ranked r = rank(count);
       const bool keep = threadIdx.x < count && want.inside(above_count + r.rank, above_mass + r.before);
       const u64 n_kept = block_sum(keep, s.sum);
+      if (threadIdx.x == 0) s.list = 0;
       if (keep && r.rank + 1 == n_kept)
         for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
           u64 *const to = cluster.map_shared_rank(&s, o)->found;
@@ -916,114 +978,152 @@ struct Part {
 };
 
 template <typename T, bool STAGED>
-__global__ void __launch_bounds__(kThreads)
-    sample_block_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned H, unsigned n, unsigned part, bool whole,
-                        const Sampling how, int q, long long *__restrict__ codes) {
+__global__ void __launch_bounds__(kThreads, 2)
+    sample_block_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned H, unsigned n, unsigned part, const Sampling how,
+                        int q, long long *__restrict__ codes) {
   after_previous();
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
+  using P = Part<T, STAGED>;
+  constexpr int V = P::V;
   extern __shared__ uint4 s_values[];
   __shared__ Block s;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned blocks = cluster.num_blocks(), g = blockIdx.x / blocks, rank = cluster.block_rank();
   const unsigned begin = min(n, rank * part), size = min(part, n - begin);
   const T *const from = support + (long)g * n + begin;
+  const Settings set = settings_of(how, g / H, n);
   Weights::fill(s.table);
-  Key top = Keys<W>::of((W)-INFINITY);
-  Part<T, STAGED> p{from, begin, size, n, (W)0, s, cluster};
+  if (threadIdx.x == 0) s.list = 0;
+  P p{reinterpret_cast<const Vec<T, V> *>(from), begin, size, 0, size, (W)0, s, cluster, 0};
+  W mine = -INFINITY;   // the largest of the values that pass through this thread
   if constexpr (STAGED) {
-    constexpr int V = 16 / (int)sizeof(T);
-    T *const to = reinterpret_cast<T *>(s_values);
-    const unsigned vectors = whole ? size / V : 0;   // (rows and parts start on 16-byte boundaries)
-#pragma unroll 4
-    for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
-      const Vec<T, V> a = reinterpret_cast<const Vec<T, V> *>(from)[i];
-      reinterpret_cast<Vec<T, V> *>(to)[i] = a;
-#pragma unroll
-      for (int v = 0; v < V; ++v) top = max(top, Keys<W>::of(no_nan(widen(a.v[v]))));
-    }
-#pragma unroll 4
-    for (unsigned i = vectors * V + threadIdx.x; i < size; i += kThreads) {
-      const T a = from[i];
-      to[i] = a;
-      top = max(top, Keys<W>::of(no_nan(widen(a))));
-    }
-    for (unsigned i = size + threadIdx.x; i < (size + V - 1) / V * V; i += kThreads) to[i] = narrow_to<T>((W)-INFINITY);
+    Vec<T, V> *const to = reinterpret_cast<Vec<T, V> *>(s_values);
+    T *const element = reinterpret_cast<T *>(s_values);
+    const unsigned head = min(size, (unsigned)((16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15) / (unsigned)sizeof(T));   // up to the first boundary
+    const unsigned body = (size - head) / V, tail = size - head - body * V, first = head ? 1 : 0;
     p.x = to;
+    p.lead = head ? V - head : 0;
+    p.vectors = (p.lead + size + V - 1) / V;
+    const Vec<T, V> *const x = reinterpret_cast<const Vec<T, V> *>(from + head);
+    constexpr int U = 4;
+    for (unsigned i = threadIdx.x; i < body; i += U * kThreads) {
+      Vec<T, V> a[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < body) a[u] = x[i + u * kThreads];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < body) {
+          to[first + i + u * kThreads] = a[u];
+          mine = fmax(mine, max_all(a[u]));
+        }
+    }
+    const T none = narrow_to<T>((W)-INFINITY);
+    if (threadIdx.x < V) {          // the vector in front of the first boundary
+      const int j = (int)threadIdx.x - (int)p.lead;
+      if (head && (j < 0 || j < (int)head)) {
+        const T a = j < 0 ? none : from[j];
+        element[threadIdx.x] = a;
+        mine = fmax(mine, widen(a));
+      }
+    } else if (threadIdx.x >= 32 && threadIdx.x < 32 + V && tail) {   // and the one behind the last
+      const unsigned j = threadIdx.x - 32;
+      const T a = j < tail ? from[head + body * V + j] : none;
+      element[(first + body) * V + j] = a;
+      mine = fmax(mine, widen(a));
+    }
   } else {
-    for (unsigned i = threadIdx.x; i < size; i += kThreads) top = max(top, Keys<W>::of(p.value(i)));
+    for (unsigned i = threadIdx.x; i < size; i += kThreads) mine = fmax(mine, widen(from[i]));
   }
-  top = (Key)p.cluster_max(block_max(top, s.sum));
+  const Key own = Keys<W>::of(mine);
+  Key top = block_max(own, s.sum), low = 0;
+  const bool by_count = set.top_k < n, quick = by_count && set.top_k > 1 && set.top_k <= kQuickCount;
+  if (quick) {
+    // A value that at least this block's share of the k units reach: the share's largest of the threads' maxima (to 2^-13 of it).
+    const unsigned share = (set.top_k + blocks - 1) / blocks;
+    constexpr int kLow = (int)sizeof(Key) * 8 - 32;
+    const unsigned bits = (unsigned)(own >> kLow);
+    unsigned reached = 0;
+    for (int b = 31; b >= 10; --b)
+      if (__syncthreads_count(bits >= (reached | 1u << b)) >= (int)share) reached |= 1u << b;
+    low = (Key)reached << kLow;
+  }
+  {
+    Key best = 0, lowest = ~(Key)0;
+    p.exchange(top, low, [&](u64 a, u64 b) { best = max(best, (Key)a), lowest = min(lowest, (Key)b); });
+    top = best, low = lowest;
+  }
   const W best = p.best = Keys<W>::value(top);
   if (!(best > (W)-INFINITY)) {
     if (rank == 0 && threadIdx.x == 0) codes[g] = -1;
+    cluster.sync();   // (a block's place is there while others read it)
     return;
   }
   const long long base = (long long)(g % H) * n;
-  const Settings set = settings_of(how, g / H, n);
   const Weights weights(s.table, set.inv_t, q);
-  if (set.top_k == 1) {
-    const unsigned unit = p.locate([&](W v, unsigned) { return (u64)(v == best); }, 0);
-    if (rank == 0 && threadIdx.x == 0) codes[g] = base + unit;
-    return;
-  }
   const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
-  Cut<Key> cut{0, n, 0};
-  const bool by_count = set.top_k < n;
-  if (by_count || set.top_p < 1) {
-    // bins of 1/128 in the weights' exponents; all units whose weight is below e^-16 share the last one
-    const W scale = (W)(128 * set.inv_t);
-    auto bin = [&](W v) -> int {
-      const W d = (best - v) * scale;
-      return v == best ? 0 : d < (W)(kBins - 1) ? (int)d : kBins - 1;
-    };
-    u64 total = p.histogram(bin, !by_count, !by_count, weights);
-    if (!by_count) total = p.cluster_sum(block_sum(total, s.sum));
-    Want want = by_count ? want_count(set.top_k) : want_mass(set.top_p, total);
-    auto found = p.find(want, 0, 0);
-    if (found.above_count + found.in_bin <= kList) {
-      // all that may be kept fits the list: the first block goes on by itself
-      const int last = found.bin;
-      const unsigned count = p.gather([&](W v) { return bin(v) <= last; }, weights);
-      if (rank != 0) return;
-      const auto r = p.rank(count);
-      bool keep = threadIdx.x < count;
-      if (by_count) {
-        keep = keep && r.rank < set.top_k;
-        want = want_mass(set.top_p, block_sum(keep ? r.mass : 0, s.sum));
-      }
-      keep = keep && (set.top_p >= 1 || want.inside(r.rank, r.before)) && (r.mass >= least || r.key == top);
-      const u64 mass = keep ? r.mass : 0, target = target_of(random[g], block_sum(mass, s.sum));
-      if (threadIdx.x < count) s.list_mass[threadIdx.x] = mass;
-      __syncthreads();
-      u64 before = 0;
-      if (keep)
-        for (unsigned j = 0; j < count; ++j)
-          if (s.list_index[j] < r.index) before += s.list_mass[j];
-      if (keep && before <= target && target < before + mass) codes[g] = base + r.index;
+  if (quick) {
+    const W from_here = low > Keys<W>::of((W)-INFINITY) ? Keys<W>::value(low) : (W)-INFINITY;
+    p.each_from(from_here, [&](W v, unsigned i) { p.put(v, i, weights); });
+    cluster.sync();
+    const unsigned count = cluster.map_shared_rank(&s, 0)->list;
+    cluster.sync();
+    if (count <= kList) {
+      if (rank == 0) p.draw(count, set, n, least, random[g], base, codes + g);
       return;
     }
-    cut = p.cut(want, found, bin, weights);
-    if (by_count && set.top_p < 1) {
-      u64 sum = 0;
-      p.each([&](W v, unsigned i) {
-        if (kept(Keys<W>::of(v), begin + i, cut)) sum += weights.of(v, best);
-      });
-      want = want_mass(set.top_p, p.cluster_sum(block_sum(sum, s.sum)));
-      p.histogram(bin, true, false, weights);
-      cut = p.cut(want, p.find(want, 0, 0), bin, weights);
-    }
+    if (rank == 0 && threadIdx.x == 0) s.list = 0;   // (values that lie unevenly over the threads, or many equal ones)
   }
-  auto weigh = [&](W v, unsigned i) -> u64 {
-    if (!(v > (W)-INFINITY) || !kept(Keys<W>::of(v), i, cut)) return 0;
-    const u64 m = weights.of(v, best);
-    return m >= least || v == best ? m : 0;
-  };
-  u64 total = 0;
-  p.each([&](W v, unsigned i) { total += weigh(v, begin + i); });
-  total = p.cluster_sum(block_sum(total, s.sum));
-  const unsigned unit = p.locate(weigh, target_of(random[g], total));
-  if (rank == 0 && threadIdx.x == 0) codes[g] = base + unit;
+  Cut<Key> cut{0, n, 0};
+  if (set.top_k == 1) {
+    p.locate([&](W v, unsigned) { return (u64)(v == best); }, [](u64) { return (u64)0; });
+  } else {
+    if (by_count || set.top_p < 1) {
+      // bins of 1/128 in the weights' exponents; all units whose weight is below e^-16 share the last one
+      const W scale = (W)(128 * set.inv_t);
+      auto bin = [&](W v) -> int {
+        const W d = (best - v) * scale;
+        return v == best ? 0 : d < (W)(kBins - 1) ? (int)d : kBins - 1;
+      };
+      u64 total = p.histogram(bin, !by_count, !by_count, weights);
+      if (!by_count) total = p.cluster_sum(block_sum(total, s.sum));
+      Want want = by_count ? want_count(set.top_k) : want_mass(set.top_p, total);
+      const auto found = p.find(want, 0, 0);
+      if (!by_count && found.above_count + found.in_bin <= kList) {
+        // all that may be kept fits the list: the first block goes on by itself
+        p.each([&](W v, unsigned i) {
+          if (bin(v) <= found.bin) p.put(v, i, weights);
+        });
+        cluster.sync();
+        if (rank != 0) return;
+        const unsigned count = s.list;
+        if (threadIdx.x == 0) s.found[3] = total;
+        __syncthreads();
+        p.draw(count, set, n, least, random[g], base, codes + g);
+        return;
+      }
+      cut = p.cut(want, found, bin, weights);
+      if (by_count && set.top_p < 1) {
+        u64 sum = 0;
+        p.each([&](W v, unsigned i) {
+          if (kept(Keys<W>::of(v), i, cut)) sum += weights.of(v, best);
+        });
+        want = want_mass(set.top_p, p.cluster_sum(block_sum(sum, s.sum)));
+        p.histogram(bin, true, false, weights);
+        cut = p.cut(want, p.find(want, 0, 0), bin, weights);
+      }
+    }
+    p.locate(
+        [&](W v, unsigned i) -> u64 {
+          if (!kept(Keys<W>::of(v), i, cut)) return 0;
+          const u64 m = weights.of(v, best);
+          return m >= least ? m : 0;
+        },
+        [&](u64 total) { return target_of(random[g], total); });
+  }
+  cluster.sync();
+  if (rank == 0 && threadIdx.x == 0) codes[g] = base + (long long)s.unit;
 }
 
 // 2^q: no sum of n masses passes 2^62.
@@ -1046,14 +1146,13 @@ cudaError_t launch_warps(const T *support, const float *random, unsigned groups,
 template <typename T, bool STAGED>
 cudaError_t launch_blocks(const T *support, const float *random, unsigned groups, unsigned H, unsigned n, unsigned part, unsigned cluster,
                           const Sampling &s, long long *codes, cudaStream_t st) {
-  const size_t smem = STAGED ? ((size_t)part * sizeof(T) + 15) / 16 * 16 : 0;
-  const bool whole = (reinterpret_cast<uintptr_t>(support) | (size_t)n * sizeof(T) | (size_t)part * sizeof(T)) % 16 == 0;
+  const size_t smem = STAGED ? (size_t)part * sizeof(T) + 32 : 0;   // (a vector in front and one behind)
   if (smem > 0) {   // (holds for the current device)
-    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage + 32);
     if (e != cudaSuccess) return e;
   }
-  return launch_clusters(sample_block_kernel<T, STAGED>, dim3(groups * cluster), dim3(cluster), kThreads, smem, st, support, random, H, n, part, whole,
-                         s, mass_bits(n), codes);
+  return launch_clusters(sample_block_kernel<T, STAGED>, dim3(groups * cluster), dim3(cluster), kThreads, smem, st, support, random, H, n, part, s,
+                         mass_bits(n), codes);
 }
 
 }  // namespace
