@@ -33,12 +33,15 @@ int fail(int code, const char *fmt, ...) {
   } while (0)
 
 int need_device() {
+  static bool found = false;   // (a device that is there stays)
+  if (found) return SBB_OK;
   int n = 0;
   if (cudaGetDeviceCount(&n) != cudaSuccess) {
     (void)cudaGetLastError();
     n = 0;
   }
   if (n <= 0) return fail(SBB_ERR_NO_DEVICE, "no CUDA device is available; this library has no CPU path");
+  found = true;
   return SBB_OK;
 }
 

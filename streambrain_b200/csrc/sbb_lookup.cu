@@ -7,37 +7,136 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A block has `lanes` threads across V columns each, and its other threads split the row's codes; the parts are added in order.
+// `lanes` threads take V columns each of a row's tile; `parts` such groups of a block split the row's codes and the parts are added in
+// order; the block's other groups take other rows or tiles.  Codes are read eight at a time, so that as many weight rows are in
+// flight, and the next eight while these are.
 template <typename T, typename I, int V>
 __global__ void __launch_bounds__(kThreads)
-    lookup_kernel(const T *__restrict__ weights, const I *__restrict__ codes, long L, long N, long M, Wide<T> scale, T *__restrict__ out, int lanes) {
+    lookup_kernel(const T *__restrict__ weights, const I *__restrict__ codes, long rows, long L, long N, long M, Wide<T> scale, T *__restrict__ out,
+                  int lanes, int parts, unsigned tiles) {
   after_previous();
   using W = Wide<T>;
-  __shared__ W s_part[kThreads * V];
-  const int parts = kThreads / lanes, part = threadIdx.x / lanes;
-  const long r = blockIdx.x, col = ((long)blockIdx.y * lanes + threadIdx.x % lanes) * V;
+  extern __shared__ unsigned char s_raw[];
+  W *const s_part = reinterpret_cast<W *>(s_raw);   // [threads][V], where parts > 1
+  const int group = threadIdx.x / lanes, part = group % parts;
+  const long item = (long)blockIdx.x * (kThreads / (lanes * parts)) + group / parts, r = item / tiles;
+  const long col = (item % tiles * lanes + threadIdx.x % lanes) * V;
+  const bool here = r < rows && col < M;
   W acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = (W)0;
-  if (col < M)
-    for (long l = part; l < L; l += parts) {
-      const long code = (long)codes[r * L + l];
-      if (code < 0 || code >= N) continue;
-      const Vec<T, V> w = *reinterpret_cast<const Vec<T, V> *>(weights + code * M + col);
+  if (here) {
+    constexpr int U = 8;
+    const I *const code = codes + r * L;
+    const T *const from = weights + col;
+    I c[U];
+    auto read = [&](long l) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] += widen(w.v[v]);
+      for (int u = 0; u < U; ++u) c[u] = l + u * parts < L ? code[l + u * parts] : (I)-1;
+    };
+    read(part);
+    for (long l = part; l < L; l += U * parts) {
+      Vec<T, V> x[U];
+      bool named[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        named[u] = c[u] >= 0 && (long)c[u] < N;
+        if (named[u]) x[u] = *reinterpret_cast<const Vec<T, V> *>(from + (long)c[u] * M);
+      }
+      if (l + U * parts < L) read(l + U * parts);
+      // the eight among themselves first: a chain of L additions loses digits that one of L / 8 keeps
+      W eight[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) eight[v] = (W)0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (named[u]) {
+          W f[V];
+          widen_all(x[u], f);
+#pragma unroll
+          for (int v = 0; v < V; ++v) eight[v] += f[v];
+        }
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += eight[v];
     }
+  }
+  if (parts > 1) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) s_part[threadIdx.x * V + v] = acc[v];
-  __syncthreads();
-  if (part != 0 || col >= M) return;
-  for (int p = 1; p < parts; ++p)
+    for (int v = 0; v < V; ++v) s_part[threadIdx.x * V + v] = acc[v];
+    __syncthreads();
+    if (part != 0) return;
+    for (int p = 1; p < parts; ++p)
 #pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] += s_part[(p * lanes + threadIdx.x) * V + v];
-  Vec<T, V> o;
+      for (int v = 0; v < V; ++v) acc[v] += s_part[(p * lanes + threadIdx.x) * V + v];
+  }
+  if (!here) return;
 #pragma unroll
-  for (int v = 0; v < V; ++v) o.v[v] = narrow_to<T>(acc[v] * scale);
-  *reinterpret_cast<Vec<T, V> *>(out + r * M + col) = o;
+  for (int v = 0; v < V; ++v) acc[v] *= scale;
+  *reinterpret_cast<Vec<T, V> *>(out + r * M + col) = narrow_all<T, V>(acc);
+}
+
+// One code a row: copies of weight rows, U under way per thread.  A block takes whole pieces of kThreads * U vectors of the result.
+template <typename T, typename I, int V, int U>
+__global__ void __launch_bounds__(kThreads)
+    lookup_one_kernel(const T *__restrict__ weights, const I *__restrict__ codes, long rows, long N, long M, Wide<T> scale, T *__restrict__ out,
+                      unsigned across) {
+  after_previous();
+  using W = Wide<T>;
+  const long first = (long)blockIdx.x * (kThreads * U), row0 = first / across;
+  const unsigned at0 = (unsigned)(first - row0 * across) + threadIdx.x;   // (the one division of 64 bits)
+  Vec<T, V> x[U];
+  unsigned r[U], col[U];
+  I c[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned at = at0 + u * kThreads;
+    r[u] = at / across;
+    col[u] = (at - r[u] * across) * V;
+    c[u] = row0 + r[u] < rows ? codes[row0 + r[u]] : (I)-1;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (c[u] >= 0 && (long)c[u] < N) {
+      x[u] = *reinterpret_cast<const Vec<T, V> *>(weights + (long)c[u] * M + col[u]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[u].v[v] = narrow_to<T>((W)0);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (row0 + r[u] >= rows) continue;
+    W f[V];
+    widen_all(x[u], f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] *= scale;
+    *reinterpret_cast<Vec<T, V> *>(out + (row0 + r[u]) * M + col[u]) = narrow_all<T, V>(f);
+  }
+}
+
+template <typename T, typename I, int V>
+cudaError_t launch_lookup_as(const T *weights, const I *codes, long rows, long L, long N, long M, double scale, T *out, cudaStream_t st) {
+  const long across = M / V;
+  if (L == 1) {
+    constexpr int U = V == 1 ? 8 : 4;
+    const long blocks = (rows * across + kThreads * U - 1) / (kThreads * U);
+    if (blocks > 0x7fffffffl) return cudaErrorInvalidConfiguration;
+    return launch_next(lookup_one_kernel<T, I, V, U>, dim3((unsigned)blocks), kThreads, 0, st, weights, codes, rows, N, M, (Wide<T>)scale, out,
+                       (unsigned)across);
+  }
+  // Few rows of many codes: narrow tiles (of a line of 128 bytes and more) and the codes split until the SMs have work, four codes or
+  // more a part.
+  const long want = 1024l * sm_count();
+  int lanes = 1;
+  while (lanes < 32 && lanes < across) lanes *= 2;
+  while (lanes > 8 && rows * across * (L / 16) < want && rows * ((across + lanes - 1) / lanes) < 2 * sm_count()) lanes /= 2;
+  int parts = 1;
+  while (parts * lanes < kThreads && parts * 8 <= L && rows * across * parts < want) parts *= 2;
+  const long tiles = (across + lanes - 1) / lanes, each = kThreads / (lanes * parts), blocks = (rows * tiles + each - 1) / each;
+  if (blocks > 0x7fffffffl) return cudaErrorInvalidConfiguration;
+  const size_t smem = parts > 1 ? kThreads * V * sizeof(Wide<T>) : 0;
+  return launch_next(lookup_kernel<T, I, V>, dim3((unsigned)blocks), kThreads, smem, st, weights, codes, rows, L, N, M, (Wide<T>)scale, out, lanes, parts,
+                     (unsigned)tiles);
 }
 
 // ---- gradient --------------------------------------------------------------
@@ -433,18 +532,16 @@ cudaError_t launch_sums(Sums<T, V> p, unsigned chunks, cudaStream_t st) {
 template <typename T, typename I>
 cudaError_t launch_lookup(const T *weights, const I *codes, long rows, long L, long N, long M, double scale, T *out, cudaStream_t st) {
   const int vec = vector_width<T>(M, weights, out);
-  const long across = (M + vec - 1) / vec;
-  int lanes = 8;
-  while (lanes < kThreads && lanes < across) lanes *= 2;
-  const dim3 grid((unsigned)rows, (unsigned)((across + lanes - 1) / lanes));
-  const Wide<T> s = (Wide<T>)scale;
   cudaError_t e;
-  if (vec == 16 / (int)sizeof(T))
-    e = launch_next(lookup_kernel<T, I, 16 / (int)sizeof(T)>, grid, kThreads, 0, st, weights, codes, L, N, M, s, out, lanes);
-  else if (sizeof(T) == 2 && vec == 2)
-    e = launch_next(lookup_kernel<T, I, 2>, grid, kThreads, 0, st, weights, codes, L, N, M, s, out, lanes);
-  else
-    e = launch_next(lookup_kernel<T, I, 1>, grid, kThreads, 0, st, weights, codes, L, N, M, s, out, lanes);
+  if (vec == 16 / (int)sizeof(T)) {
+    e = launch_lookup_as<T, I, 16 / (int)sizeof(T)>(weights, codes, rows, L, N, M, scale, out, st);
+  } else {
+    if constexpr (sizeof(T) == 2)
+      e = vec == 2 ? launch_lookup_as<T, I, 2>(weights, codes, rows, L, N, M, scale, out, st)
+                   : launch_lookup_as<T, I, 1>(weights, codes, rows, L, N, M, scale, out, st);
+    else
+      e = launch_lookup_as<T, I, 1>(weights, codes, rows, L, N, M, scale, out, st);
+  }
   if (e == cudaSuccess) count_launches(1);
   return e;
 }

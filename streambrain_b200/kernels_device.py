@@ -16,7 +16,6 @@ Nothing here records for autograd: the gradients are calls of their own.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 
 import torch
 
@@ -31,27 +30,31 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
-def _dense(t, name, dim, dtypes, like=None):
-    """``t`` as a contiguous CUDA tensor of one of ``dtypes``, on the device of ``like``."""
+def _dense(t, name, dim, dtypes, device=None):
+    """``t`` as a contiguous CUDA tensor of one of ``dtypes``, on ``device`` (a number)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError("%s must be a CUDA tensor" % name)
     if t.dtype not in dtypes:
         raise TypeError("%s has dtype %s, expected %s" % (name, t.dtype, " or ".join(str(d) for d in dtypes)))
     if t.dim() != dim:
         raise ValueError("%s must have %d dimensions, got shape %s" % (name, dim, tuple(t.shape)))
-    if like is not None and t.device != like.device:
-        raise ValueError("%s is on %s, not on %s" % (name, t.device, like.device))
+    if device is not None and t.get_device() != device:
+        raise ValueError("%s is on cuda:%d, not on cuda:%d" % (name, t.get_device(), device))
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _on(t):
-    """Makes the device of ``t`` current while the work is queued."""
-    index = t.device.index
-    return nullcontext() if _current_device is not None and _current_device() == index else torch.cuda.device(index)
-
-
-def _stream(t):
-    return _raw_stream(t.device.index) if _raw_stream is not None else torch.cuda.current_stream(t.device).cuda_stream
+def _call(entry, device, *arguments):
+    """``entry(*arguments, stream)`` on torch's current stream of ``device``, with that device current."""
+    if _raw_stream is None or _current_device is None:
+        with torch.cuda.device(device):
+            rc = entry(*arguments, torch.cuda.current_stream(device).cuda_stream)
+    elif _current_device() == device:
+        rc = entry(*arguments, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*arguments, _raw_stream(device))
+    if rc:
+        check(rc)
 
 
 def _wide(dtype):
@@ -63,13 +66,13 @@ def lookup(weights, codes, scale=1.0):
     weights' dtype.  With L = 1 an embedding lookup.  Codes outside ``0 .. N - 1`` (-1 by convention) name nothing; a row
     of such codes, or with L = 0, gives zeros."""
     weights = _dense(weights, "weights", 2, _DTYPES)
-    codes = _dense(codes, "codes", 2, _INDEX_BYTES, weights)
+    device = weights.get_device()
+    codes = _dense(codes, "codes", 2, _INDEX_BYTES, device)
     rows, length = codes.shape
     n, m = weights.shape
     out = weights.new_empty((rows, m))
-    with _on(weights):
-        check(lib.sbb_lookup(_DTYPES[weights.dtype], weights.data_ptr(), codes.data_ptr(), _INDEX_BYTES[codes.dtype], rows,
-                             length, n, m, float(scale), out.data_ptr(), _stream(weights)))
+    _call(lib.sbb_lookup, device, _DTYPES[weights.dtype], weights.data_ptr(), codes.data_ptr(), _INDEX_BYTES[codes.dtype], rows,
+          length, n, m, scale, out.data_ptr())
     return out
 
 
@@ -79,7 +82,8 @@ def lookup_gradient(grad, codes, in_features, scale=1.0, out=None, accumulate=Fa
     zero.  ``out`` (contiguous) receives it; with ``accumulate=True`` the sums are added to what it holds, and rows that no
     code names are left alone."""
     grad = _dense(grad, "grad", 2, _DTYPES)
-    codes = _dense(codes, "codes", 2, _INDEX_BYTES, grad)
+    device = grad.get_device()
+    codes = _dense(codes, "codes", 2, _INDEX_BYTES, device)
     rows, length = codes.shape
     n, m = int(in_features), grad.shape[1]
     if grad.shape[0] != rows:
@@ -91,24 +95,22 @@ def lookup_gradient(grad, codes, in_features, scale=1.0, out=None, accumulate=Fa
             raise ValueError("in_features must be above 0")
         out = grad.new_empty((n, m))
     else:
-        if _dense(out, "out", 2, (grad.dtype,), grad) is not out:
+        if _dense(out, "out", 2, (grad.dtype,), device) is not out:
             raise ValueError("out must be contiguous")
         if out.shape != (n, m):
             raise ValueError("out must have shape %s, got %s" % ((n, m), tuple(out.shape)))
     code = _DTYPES[grad.dtype]
-    size = int(lib.sbb_lookup_gradient_workspace(code, rows, length, n, m))
-    work = torch.empty(size, dtype=torch.uint8, device=grad.device) if size else None
-    with _on(grad):
-        check(lib.sbb_lookup_gradient(code, grad.data_ptr(), codes.data_ptr(), _INDEX_BYTES[codes.dtype], rows, length, n, m,
-                                      float(scale), 1 if accumulate else 0, out.data_ptr(),
-                                      None if work is None else work.data_ptr(), size, _stream(grad)))
+    size = lib.sbb_lookup_gradient_workspace(code, rows, length, n, m)
+    work = grad.new_empty(size, dtype=torch.uint8) if size else None
+    _call(lib.sbb_lookup_gradient, device, code, grad.data_ptr(), codes.data_ptr(), _INDEX_BYTES[codes.dtype], rows, length, n, m,
+          scale, 1 if accumulate else 0, out.data_ptr(), None if work is None else work.data_ptr(), size)
     return out
 
 
-def _setting(value, name, rows, dtype, like):
+def _setting(value, name, rows, dtype, device):
     """A sampling setting: (number, tensor of a value per row or None)."""
     if isinstance(value, torch.Tensor):
-        t = _dense(value, name, 1, (dtype,), like)
+        t = _dense(value, name, 1, (dtype,), device)
         if t.shape[0] != rows:
             raise ValueError("%s must be a number or have %d values, got %d" % (name, rows, t.shape[0]))
         return None, t
@@ -127,49 +129,48 @@ def sample_minicolumns(support, hypercolumns, minicolumns, random, temperature=1
     equal ones.  NaN counts as -infinity.  Each setting is a number or a CUDA tensor with a value per row (``top_k`` int32,
     the others float32; values out of range act as the nearest in range)."""
     support = _dense(support, "support", 2, _DTYPES)
+    device = support.get_device()
     h, mc = int(hypercolumns), int(minicolumns)
-    rows = support.shape[0]
-    if support.shape[1] != h * mc:
-        raise ValueError("support has %d columns, expected %d hypercolumns of %d units" % (support.shape[1], h, mc))
-    random = _dense(random, "random", 2, (torch.float32,), support)
+    rows, columns = support.shape
+    if columns != h * mc:
+        raise ValueError("support has %d columns, expected %d hypercolumns of %d units" % (columns, h, mc))
+    random = _dense(random, "random", 2, (torch.float32,), device)
     if random.shape != (rows, h):
         raise ValueError("random must have shape %s, got %s" % ((rows, h), tuple(random.shape)))
-    t, t_rows = _setting(temperature, "temperature", rows, torch.float32, support)
-    k, k_rows = _setting(top_k, "top_k", rows, torch.int32, support)
-    p, p_rows = _setting(top_p, "top_p", rows, torch.float32, support)
-    low, low_rows = _setting(min_p, "min_p", rows, torch.float32, support)
-    how = Sampling(1.0 if t is None else float(t), 1.0 if p is None else float(p), 0.0 if low is None else float(low),
-                   0 if k is None else int(k), *(None if a is None else a.data_ptr() for a in (t_rows, p_rows, low_rows, k_rows)))
-    codes = torch.empty((rows, h), dtype=torch.int64, device=support.device)
-    with _on(support):
-        check(lib.sbb_sample_minicolumns(_DTYPES[support.dtype], support.data_ptr(), random.data_ptr(), rows, h, mc,
-                                         ctypes.byref(how), codes.data_ptr(), _stream(support)))
+    t, t_rows = _setting(temperature, "temperature", rows, torch.float32, device)
+    k, k_rows = _setting(top_k, "top_k", rows, torch.int32, device)
+    p, p_rows = _setting(top_p, "top_p", rows, torch.float32, device)
+    low, low_rows = _setting(min_p, "min_p", rows, torch.float32, device)
+    how = Sampling(1.0 if t is None else t, 1.0 if p is None else p, 0.0 if low is None else low, 0 if k is None else int(k),
+                   *[None if a is None else a.data_ptr() for a in (t_rows, p_rows, low_rows, k_rows)])
+    codes = support.new_empty((rows, h), dtype=torch.int64)
+    _call(lib.sbb_sample_minicolumns, device, _DTYPES[support.dtype], support.data_ptr(), random.data_ptr(), rows, h, mc,
+          ctypes.byref(how), codes.data_ptr())
     return codes
 
 
 def _distill(support, hypercolumns, minicolumns, teacher_units, teacher_support, temperature, weight, want_gradient):
     support = _dense(support, "support", 2, _DTYPES)
+    device = support.get_device()
     h, mc = int(hypercolumns), int(minicolumns)
-    rows = support.shape[0]
-    if support.shape[1] != h * mc:
-        raise ValueError("support has %d columns, expected %d hypercolumns of %d units" % (support.shape[1], h, mc))
-    units = _dense(teacher_units, "teacher_units", 3, _INDEX_BYTES, support)
-    teacher = _dense(teacher_support, "teacher_support", 3, (support.dtype,), support)
+    rows, columns = support.shape
+    if columns != h * mc:
+        raise ValueError("support has %d columns, expected %d hypercolumns of %d units" % (columns, h, mc))
+    units = _dense(teacher_units, "teacher_units", 3, _INDEX_BYTES, device)
+    teacher = _dense(teacher_support, "teacher_support", 3, (support.dtype,), device)
     if units.shape != teacher.shape or units.shape[:2] != (rows, h):
         raise ValueError("teacher_units and teacher_support must both be [%d, %d, k], got %s and %s" % (
             rows, h, tuple(units.shape), tuple(teacher.shape)))
     wide = _wide(support.dtype)
     if weight is not None:
-        weight = _dense(weight, "weight", 1, (wide,), support)
+        weight = _dense(weight, "weight", 1, (wide,), device)
         if weight.shape[0] != rows:
             raise ValueError("weight has %d values for %d rows" % (weight.shape[0], rows))
-    loss = torch.empty((rows, h), dtype=wide, device=support.device)
-    gradient = torch.empty_like(support) if want_gradient else None
-    with _on(support):
-        check(lib.sbb_distill(_DTYPES[support.dtype], support.data_ptr(), units.data_ptr(), _INDEX_BYTES[units.dtype],
-                              teacher.data_ptr(), None if weight is None else weight.data_ptr(), rows, h, mc, units.shape[2],
-                              float(temperature), loss.data_ptr(), None if gradient is None else gradient.data_ptr(),
-                              _stream(support)))
+    loss = support.new_empty((rows, h), dtype=wide)
+    gradient = support.new_empty((rows, columns)) if want_gradient else None
+    _call(lib.sbb_distill, device, _DTYPES[support.dtype], support.data_ptr(), units.data_ptr(), _INDEX_BYTES[units.dtype],
+          teacher.data_ptr(), None if weight is None else weight.data_ptr(), rows, h, mc, units.shape[2], temperature,
+          loss.data_ptr(), None if gradient is None else gradient.data_ptr())
     return loss, gradient
 
 
