@@ -2,6 +2,11 @@
 #include "sbb_codes.cuh"
 #include "sbb_launch.cuh"
 
+#include <cooperative_groups.h>
+#include <cstdlib>
+
+namespace cg = cooperative_groups;
+
 namespace sbb {
 namespace {
 
@@ -143,12 +148,32 @@ cudaError_t launch_lookup_as(const T *weights, const I *codes, long rows, long L
 //
 // The codes are sorted (stably, so that the sums of a weight row run in the order of the samples whatever the schedule), and
 // then every weight row is the sum of a run of the gradient's rows.  Runs may be of any length, so the sorted entries are cut
-// into equal chunks: a chunk writes the runs that lie in it and leaves the part of a run that crosses its border in the
-// workspace, from where join_kernel adds the parts in order.
+// into equal chunks and these joined to spans: a block writes the runs that lie in its span and leaves the part of a run that
+// crosses the span's border in the workspace, from where join_kernel adds the parts in order.
 
 constexpr unsigned kRankMost = 8192;   // entries that are ranked by comparing all with all
 
 __device__ __forceinline__ unsigned key_of(long code, long N) { return code >= 0 && code < N ? (unsigned)code : (unsigned)N; }
+
+// Bytes [begin, begin + bytes) of the result that a launch of the sort sets to zero beside its own work, which leaves most SMs and
+// all of the memory's bandwidth idle.  Rows that codes name are written again later; knowing them and leaving them out, in the
+// launch that sums, took 78 us for 65536 codes of 50000 x 1024 bf16.
+struct Zero {
+  unsigned char *begin;
+  size_t bytes;
+};
+constexpr size_t kZeroBlock = 64 * 1024;
+inline unsigned zero_blocks(const Zero &z) { return (unsigned)((z.bytes + kZeroBlock - 1) / kZeroBlock); }
+__device__ __forceinline__ void set_zero(const Zero &z, unsigned block) {
+  unsigned char *const from = z.begin + block * kZeroBlock;
+  const size_t bytes = min(kZeroBlock, z.bytes - block * kZeroBlock);
+  const size_t head = min(bytes, (size_t)((16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15)), body = (bytes - head) / 16;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (size_t i = threadIdx.x; i < body; i += blockDim.x) reinterpret_cast<uint4 *>(from + head)[i] = zero;
+  const size_t rest = bytes - body * 16;   // bytes at either end, an even number of them
+  for (size_t i = threadIdx.x * 2; i < rest; i += blockDim.x * 2)
+    *reinterpret_cast<unsigned short *>(from + (i < head ? i : body * 16 + i)) = 0;
+}
 
 // a < b for numbers of up to 2^31 (the difference's sign: an instruction less than a comparison and a choice)
 __device__ __forceinline__ unsigned below(unsigned a, unsigned b) { return (a - b) >> 31; }
@@ -158,8 +183,9 @@ __device__ __forceinline__ unsigned below(unsigned a, unsigned b) { return (a - 
 template <typename I>
 __global__ void __launch_bounds__(kThreads)
     rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, unsigned *__restrict__ key, unsigned *__restrict__ row,
-                unsigned *__restrict__ some) {
+                unsigned blocks, const Zero zero) {
   after_previous();
+  if (blockIdx.x >= blocks) return set_zero(zero, blockIdx.x - blocks);
   __shared__ uint4 s_key[kRankMost / 4];
   unsigned *const s = reinterpret_cast<unsigned *>(s_key);
   const unsigned padded = (entries + 3) & ~3u;
@@ -195,7 +221,6 @@ __global__ void __launch_bounds__(kThreads)
     if (lane == 0 && e0 + q < entries) {
       key[r] = k[q];
       row[r] = (e0 + q) / L;
-      if (some != nullptr && k[q] < (unsigned)N) some[k[q]] = r;
     }
   }
 }
@@ -211,8 +236,9 @@ __device__ __forceinline__ unsigned sort_key(const I *codes, const unsigned *key
 template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
     digits_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, unsigned entries, long N, int shift, unsigned tile,
-                  unsigned *__restrict__ counts) {
+                  unsigned *__restrict__ counts, unsigned blocks, const Zero zero) {
   after_previous();
+  if (blockIdx.x >= blocks) return set_zero(zero, blockIdx.x - blocks);
   __shared__ unsigned s_count[kDigits];
   for (int d = threadIdx.x; d < kDigits; d += kSortThreads) s_count[d] = 0;
   __syncthreads();
@@ -229,8 +255,9 @@ template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
     move_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, const unsigned *__restrict__ row, unsigned entries, unsigned L, long N,
                 int shift, unsigned tile, const unsigned *__restrict__ counts, unsigned *__restrict__ key_to, unsigned *__restrict__ row_to,
-                unsigned *__restrict__ some) {
+                unsigned blocks, const Zero zero) {
   after_previous();
+  if (blockIdx.x >= blocks) return set_zero(zero, blockIdx.x - blocks);
   static_assert(kDigits == kSortThreads, "a thread per digit");
   __shared__ unsigned s_at[kSortWarps][kDigits];
   __shared__ unsigned s_warp[kSortWarps];
@@ -241,7 +268,7 @@ __global__ void __launch_bounds__(kSortThreads)
   for (unsigned i = lo + lane; i < hi; i += 32) atomicAdd(&s_at[warp][(sort_key<I, FIRST>(codes, key, i, N) >> shift) & (kDigits - 1)], 1u);
   unsigned all = 0, before = 0;
 #pragma unroll 16
-  for (unsigned b = 0; b < gridDim.x; ++b) {
+  for (unsigned b = 0; b < blocks; ++b) {
     const unsigned c = counts[b * kDigits + threadIdx.x];
     all += c;
     before += b < blockIdx.x ? c : 0;
@@ -270,7 +297,6 @@ __global__ void __launch_bounds__(kSortThreads)
       const unsigned to = s_at[warp][digit] + __popc(same & ((1u << lane) - 1));
       key_to[to] = kk;
       row_to[to] = FIRST ? (i0 + lane) / L : row[i0 + lane];
-      if (some != nullptr && kk < (unsigned)N) some[kk] = to;
     }
     __syncwarp();
     if (there && (same >> lane) == 1u) s_at[warp][digit] += __popc(same);   // the last of its kind
@@ -278,20 +304,122 @@ __global__ void __launch_bounds__(kSortThreads)
   }
 }
 
+// The same sort by one cluster in one launch, for as many entries as its threads hold: an entry's place is found in registers and
+// shared memory, and the entries move between the blocks' shared memories.
+constexpr int kClusterThreads = 1024, kClusterWarps = kClusterThreads / 32, kClusterBlocks = 16;
+
+struct SortSpace {
+  unsigned short at[kClusterWarps][kDigits];
+  unsigned all[kDigits], base[kDigits], warp[kClusterWarps];
+};
+
+// EACH entries a thread.  `hold`: two words for each of the block's entries, where there is more than one pass.
+template <typename I, int EACH>
+__device__ void cluster_sort(cg::cluster_group cluster, SortSpace &s, unsigned *hold, const I *codes, unsigned entries, unsigned L, long N, int passes,
+                             int digit_bits, unsigned *key_to, unsigned *row_to) {
+  constexpr unsigned kHere = kClusterThreads * EACH;
+  const unsigned rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1u << digit_bits;
+  const unsigned slot0 = warp * (32 * EACH) + lane, first = rank * kHere + slot0;   // a warp's entries lie together
+  unsigned key[EACH], row[EACH];
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) key[r] = first + r * 32 < entries ? key_of((long)codes[first + r * 32], N) : ~0u;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) row[r] = (first + r * 32) / L;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    for (unsigned i = threadIdx.x; i < kClusterWarps * kDigits / 2; i += kClusterThreads) reinterpret_cast<unsigned *>(s.at)[i] = 0;
+    __syncthreads();
+    unsigned short place[EACH];   // among the warp's entries of the same digit
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      const bool there = first + r * 32 < entries;
+      const unsigned digit = there ? (key[r] >> shift) & (digits - 1) : kDigits + 1;
+      const unsigned same = __match_any_sync(0xffffffffu, digit), front = __popc(same & ((1u << lane) - 1));
+      if (there) place[r] = (unsigned short)(s.at[warp][digit] + front);
+      __syncwarp();
+      if (there && (same >> lane) == 1u) s.at[warp][digit] = (unsigned short)(place[r] + 1);   // the last of its kind
+      __syncwarp();
+    }
+    __syncthreads();
+    if (threadIdx.x < digits) {
+      unsigned run = 0;
+#pragma unroll 8
+      for (int w = 0; w < kClusterWarps; ++w) {
+        const unsigned c = s.at[w][threadIdx.x];
+        s.at[w][threadIdx.x] = (unsigned short)run;
+        run += c;
+      }
+      s.all[threadIdx.x] = run;
+    }
+    cluster.sync();   // (and every block has read what it holds)
+    unsigned all = 0, before = 0;
+    if (threadIdx.x < digits)
+#pragma unroll
+      for (unsigned o = 0; o < kClusterBlocks; ++o) {
+        const unsigned c = cluster.map_shared_rank(&s, o)->all[threadIdx.x];
+        all += c;
+        before += o < rank ? c : 0;
+      }
+    unsigned in = all;
+    for (int off = 1; off < 32; off *= 2) {
+      const unsigned o = __shfl_up_sync(0xffffffffu, in, off);
+      if (lane >= off) in += o;
+    }
+    if (lane == 31) s.warp[warp] = in;
+    __syncthreads();
+    if (threadIdx.x < digits) {
+      unsigned base = before + in - all;
+      for (unsigned w = 0; w < warp; ++w) base += s.warp[w];
+      s.base[threadIdx.x] = base;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      if (first + r * 32 >= entries) continue;
+      const unsigned digit = (key[r] >> shift) & (digits - 1), to = s.base[digit] + s.at[warp][digit] + place[r];
+      if (pass + 1 == passes) {
+        key_to[to] = key[r];
+        row_to[to] = row[r];
+      } else {
+        unsigned *const there = cluster.map_shared_rank(hold, to / kHere) + to % kHere;
+        there[0] = key[r];
+        there[kHere] = row[r];
+      }
+    }
+    cluster.sync();
+    if (pass + 1 < passes) {
+#pragma unroll
+      for (int r = 0; r < EACH; ++r) key[r] = hold[slot0 + r * 32], row[r] = hold[kHere + slot0 + r * 32];
+    }
+  }
+}
+
+template <typename I, int EACH>
+__global__ void __launch_bounds__(kClusterThreads, 1)
+    sort_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, int passes, int digit_bits, unsigned *__restrict__ key,
+                unsigned *__restrict__ row, const Zero zero) {
+  after_previous();
+  if (blockIdx.x >= kClusterBlocks) {   // (whole clusters; those behind the last piece have none)
+    if (blockIdx.x - kClusterBlocks < (zero.bytes + kZeroBlock - 1) / kZeroBlock) set_zero(zero, blockIdx.x - kClusterBlocks);
+    return;
+  }
+  extern __shared__ unsigned s_hold[];
+  __shared__ SortSpace s;
+  cluster_sort<I, EACH>(cg::this_cluster(), s, s_hold, codes, entries, L, N, passes, digit_bits, key, row);
+}
+
 template <typename T, int V>
 struct Sums {
   const T *grad;
   const unsigned *key, *row;   // sorted
-  const unsigned *some;        // per weight row: the position of a code that names it, or anything where none does
-  unsigned entries, chunk;
+  unsigned entries, chunk, span;   // of a group of threads, of a block
   long N, M;
   Wide<T> scale;
   bool accumulate;
   T *out;
-  Wide<T> *partial;   // [chunk][run from the chunk before, run into the next][M]
+  Wide<T> *partial;   // [span][run from the span before, run into the next][M]
   int lanes;
   unsigned tiles;     // of `lanes` vectors
-  int zero_rows;      // of a block
 
   using W = Wide<T>;
   __device__ __forceinline__ void write(unsigned i, long col, const W (&acc)[V]) const {
@@ -305,42 +433,16 @@ struct Sums {
   __device__ __forceinline__ W *part(unsigned c, int which, long col) const { return partial + (2l * c + which) * M + col; }
 };
 
-constexpr int kZeroRows = 128;   // most rows of a block that sets rows to zero
-
-// `lanes` threads take a chunk and a tile of columns.  Among the `sum_blocks` blocks that do so lie `zero_blocks` that set rows
-// without a code to zero, evenly, so that memory is read and written at the same time.
+// `lanes` threads take a chunk and a tile of columns, a block the chunks of a span.  A run inside a chunk is written; the others'
+// parts wait in shared memory and the group in which a run begins (the first one, for a run from the span before) adds them up.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p, unsigned sum_blocks, unsigned zero_blocks) {
+__global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p) {
   after_previous();
   using W = Wide<T>;
-  const unsigned zero_before = (unsigned)((unsigned long long)blockIdx.x * zero_blocks / gridDim.x);
-  if ((unsigned)((unsigned long long)(blockIdx.x + 1) * zero_blocks / gridDim.x) != zero_before) {
-    __shared__ bool s_absent[kZeroRows];
-    const long n0 = (long)zero_before * p.zero_rows;
-    const int rows = (int)min((long)p.zero_rows, p.N - n0);
-    if ((int)threadIdx.x < rows) {
-      const unsigned n = (unsigned)n0 + threadIdx.x, at = p.some[n];   // (nothing has written it where no code names the row)
-      s_absent[threadIdx.x] = at >= p.entries || p.key[at] != n;
-    }
-    __syncthreads();
-    Vec<T, V> zero;
-#pragma unroll
-    for (int v = 0; v < V; ++v) zero.v[v] = narrow_to<T>((W)0);
-    const unsigned across = (unsigned)(p.M / V);
-    unsigned r = threadIdx.x / across, c = threadIdx.x % across;
-    const unsigned dr = kThreads / across, dc = kThreads % across;
-    while ((int)r < rows) {
-      if (s_absent[r]) *reinterpret_cast<Vec<T, V> *>(p.out + (n0 + r) * p.M + (long)c * V) = zero;
-      r += dr;
-      c += dc;
-      if (c >= across) c -= across, ++r;
-    }
-    return;
-  }
+  __shared__ Vec<W, V> s_head[kThreads], s_tail[kThreads];
   // the block's sorted entries, with one more at either end
   extern __shared__ unsigned s_entry[];
-  const unsigned groups = kThreads / p.lanes, g0 = (blockIdx.x - zero_before) * groups, g = g0 + threadIdx.x / p.lanes, c = g / p.tiles;
-  const unsigned first = g0 / p.tiles * p.chunk, end = min(p.entries, ((g0 + groups - 1) / p.tiles + 1) * p.chunk), size = end > first ? end - first : 0;
+  const unsigned span = blockIdx.x / p.tiles, first = span * p.span, size = min(p.span, p.entries - first);
   unsigned *const s_key = s_entry + 1, *const s_row = s_entry + size + 2;
   for (unsigned i = threadIdx.x; i < size + 2; i += kThreads) {
     const unsigned at = first + i - 1;   // (wraps below zero)
@@ -348,65 +450,108 @@ __global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p, u
   }
   for (unsigned i = threadIdx.x; i < size; i += kThreads) s_row[i] = p.row[first + i];
   __syncthreads();
-  const long col = ((long)(g % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
-  const unsigned b = c * p.chunk, e = min(p.entries, b + p.chunk);
-  if (b >= p.entries || col >= p.M) return;
+  const unsigned group = threadIdx.x / p.lanes, b = group * p.chunk, e = min(size, b + p.chunk);
+  const long col = ((long)(blockIdx.x % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
+  const bool here = b < size && col < p.M && s_key[b] < (unsigned)p.N;   // (codes that name nothing are the last ones)
   W acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = (W)0;
-  const unsigned *key = s_key + (b - first), *row = s_row + (b - first);
-  unsigned n = e - b;
-  while (n > 0 && key[n - 1] >= (unsigned)p.N) --n;   // codes that name nothing are the last ones
-  if (n == 0) return;
-  unsigned cur = key[0];
-  bool head = s_entry[b - first] == cur;
-  auto flush = [&](int which) {   // 2: the run lies in the chunk
-    if (which == 2) {
-      p.write(cur, col, acc);
-    } else {
-      W *const to = p.part(c, which, col);
+  bool begins = false;   // a run begins in this chunk and goes on behind it
+  if (here) {
+    const unsigned *const key = s_key + b, *const row = s_row + b;
+    unsigned n = e - b;
+    while (key[n - 1] >= (unsigned)p.N) --n;
+    unsigned cur = key[0];
+    bool head = s_entry[b] == cur;   // the key in front
+    auto keep = [&](Vec<W, V> &to) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) to[v] = acc[v];
-    }
-  };
-  // Four loads without conditions in flight, four blocks on an SM.  65536 rows of 1024 bf16 elements, us a call: with conditions
-  // between the loads 117, eight loads and three blocks 78, two pairs of four in turn 79 to 90 (registers), this 79.
-  constexpr int U = 4;
-  const T *const from = p.grad + col;
-  for (unsigned i = 0; i < n; i += U) {
-    Vec<T, V> x[U];
+      for (int v = 0; v < V; ++v) to.v[v] = acc[v];
+    };
+    // Four loads without conditions in flight, four blocks on an SM.  65536 rows of 1024 bf16 elements, us a call: with conditions
+    // between the loads 117, eight loads and three blocks 78, two pairs of four in turn 79 to 90 (registers), this 79.
+    constexpr int U = 4;
+    const T *const from = p.grad + col;
+    for (unsigned i = 0; i < n; i += U) {
+      Vec<T, V> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Vec<T, V> *>(from + (long)row[min(i + u, n - 1)] * p.M);
+      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const Vec<T, V> *>(from + (long)row[min(i + u, n - 1)] * p.M);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i + u >= n) break;
-      const unsigned k = key[i + u];
-      if (k != cur) {
-        flush(head ? 0 : 2);
-        cur = k;
-        head = false;
+      for (int u = 0; u < U; ++u) {
+        if (i + u >= n) break;
+        const unsigned k = key[i + u];
+        if (k != cur) {
+          if (head)
+            keep(s_head[threadIdx.x]);
+          else
+            p.write(cur, col, acc);
+          cur = k;
+          head = false;
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = (W)0;
+          for (int v = 0; v < V; ++v) acc[v] = (W)0;
+        }
+        W f[V];
+        widen_all(x[u], f);
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] += f[v];
       }
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] += widen(x[u].v[v]);
+    }
+    if (head) {
+      keep(s_head[threadIdx.x]);
+    } else if (key[n] == cur) {
+      keep(s_tail[threadIdx.x]);
+      begins = true;
+    } else {
+      p.write(cur, col, acc);
     }
   }
-  flush(head ? 0 : key[n] == cur ? 1 : 2);
+  __syncthreads();
+  if (!here) return;
+  auto collect = [&](unsigned cur, unsigned from, int which) {   // the groups' parts from `from` on, while the run goes on
+    unsigned end = from * p.chunk;
+    while (end < size && s_key[end] == cur) {
+      const Vec<W, V> more = s_head[threadIdx.x % p.lanes + from * p.lanes];
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += more.v[v];
+      end = min(size, end + p.chunk);
+      ++from;
+      if (s_key[end - 1] != cur) break;
+    }
+    if (which == 0 || (end == size && s_key[size - 1] == cur && s_key[size] == cur)) {
+      W *const to = p.part(span, which, col);
+#pragma unroll
+      for (int v = 0; v < V; ++v) to[v] = acc[v];
+    } else {
+      p.write(cur, col, acc);
+    }
+  };
+  if (begins) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = s_tail[threadIdx.x].v[v];
+    collect(s_key[e - 1], group + 1, 1);
+  }
+  if (group == 0 && s_entry[0] == s_key[0]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = (W)0;
+    collect(s_key[0], 0, 0);
+  }
 }
 
-// Adds the parts of the runs that cross the end of a chunk and begin in it: a group of `lanes` threads for each chunk and tile
-// of columns, all groups of the block together for runs of many parts (of which a block, with chunks that follow one another,
+// Adds the parts of the runs that cross the end of a span and begin in it: a group of `lanes` threads for each span and tile
+// of columns, all groups of the block together for runs of many parts (of which a block, with spans that follow one another,
 // has few).
 constexpr unsigned kLongRun = 32;
-template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
-  after_previous();
+template <typename T, int V, int THREADS>
+struct JoinSpace {
+  unsigned last[THREADS / 4];   // of each group's run, 0: none or short
+  Wide<T> sum[THREADS * V];
+};
+template <typename T, int V, int THREADS>
+__device__ __forceinline__ void join_runs(const Sums<T, V> &p, unsigned block, JoinSpace<T, V, THREADS> &s) {
   using W = Wide<T>;
-  __shared__ unsigned s_last[kThreads / 4];   // of each group's run, 0: none or short
-  __shared__ W s_sum[kThreads * V];
-  const unsigned groups = kThreads / p.lanes, own = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
-  const unsigned chunks = (p.entries + p.chunk - 1) / p.chunk;
+  unsigned *const s_last = s.last;
+  W *const s_sum = s.sum;
+  const unsigned groups = THREADS / p.lanes, own = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
+  const unsigned spans = (p.entries + p.span - 1) / p.span;
   auto sum = [&](W(&acc)[V], unsigned from, unsigned to, unsigned step, long col) {   // parts [from, to], four in flight
     for (; from <= to; from += 4 * step) {
       Vec<W, V> x[4];
@@ -420,20 +565,20 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
           for (int v = 0; v < V; ++v) acc[v] += x[u].v[v];
     }
   };
-  const unsigned blocks = (chunks + groups - 1) / groups, c0 = blockIdx.x % blocks * groups, c = c0 + own;
-  const long col = ((long)(blockIdx.x / blocks) * p.lanes + lane) * V;
+  const unsigned blocks = (spans + groups - 1) / groups, c0 = block % blocks * groups, c = c0 + own;
+  const long col = ((long)(block / blocks) * p.lanes + lane) * V;
   unsigned cur = 0, last = 0;
-  if (c + 1 < chunks) {
-    const unsigned b = c * p.chunk, e = b + p.chunk;
+  if (c + 1 < spans) {
+    const unsigned b = c * p.span, e = b + p.span;
     cur = p.key[e - 1];
     if (p.key[e] == cur && cur < (unsigned)p.N && !(b > 0 && p.key[b] == cur && p.key[b - 1] == cur)) {
-      // the last chunk that begins inside the run: the group's threads try that many places at a time
+      // the last span that begins inside the run: the group's threads try that many places at a time
       last = c + 1;
-      unsigned end = chunks;
+      unsigned end = spans;
       const unsigned mask = (p.lanes == 32 ? ~0u : (1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
-      for (unsigned step = 1; last + 1 < end; step = (end - last - 1 + p.lanes - 1) / p.lanes) {   // first the chunks that follow
+      for (unsigned step = 1; last + 1 < end; step = (end - last - 1 + p.lanes - 1) / p.lanes) {   // first those that follow
         const unsigned at = last + (lane + 1) * step;
-        const int in = __popc(__ballot_sync(mask, at < end && p.key[at * p.chunk] == cur));
+        const int in = __popc(__ballot_sync(mask, at < end && p.key[at * p.span] == cur));
         last += in * step;
         if (in < p.lanes) end = min(end, last + step);
       }
@@ -471,31 +616,88 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
   }
 }
 
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
+  after_previous();
+  __shared__ JoinSpace<T, V, kThreads> s;
+  join_runs(p, blockIdx.x, s);
+}
+
+// Whether the device takes a cluster of sixteen blocks (eight are what every device takes).
+template <typename I, int EACH>
+cudaError_t sort_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[2], int passes, cudaStream_t st) {
+  const size_t smem = passes > 1 ? 2 * sizeof(unsigned) * kClusterThreads * EACH : 0;
+  cudaError_t e = cudaFuncSetAttribute(sort_kernel<I, EACH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(sort_kernel<I, EACH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kClusterBlocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg = {};
+  cfg.gridDim = dim3(kClusterBlocks);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return e;
+}
+bool cluster_fits() {
+  static const bool fits = [] {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    int clusters = 0;
+    cudaError_t e = sort_config<int64_t, 8>(cfg, attr, 2, nullptr);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, sort_kernel<int64_t, 8>, &cfg);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return e == cudaSuccess && clusters > 0;
+  }();
+  return fits;
+}
+unsigned cl_most() {
+  static const unsigned most = getenv("SBB_CL") ? atoi(getenv("SBB_CL")) : 8 * kClusterThreads * kClusterBlocks;
+  return most;
+}
+unsigned rank_most() {
+  static const unsigned most = getenv("SBB_RANK") ? atoi(getenv("SBB_RANK")) : kRankMost;
+  return most;
+}
+
 // Sizes of a gradient call.
 struct GradientPlan {
-  unsigned entries, chunk, chunks;
-  bool rank;
-  unsigned tile, blocks;   // of the sort's passes
-  int passes;
-  size_t padded, counts, some, partial;   // elements: a key or row array, the digits' counts, a position per row, the parts of runs
+  unsigned entries, chunk, span, spans;
+  int lanes;
+  unsigned tiles;
+  bool rank, cluster;      // how the codes are sorted; else by launches for every pass
+  unsigned tile, blocks;   // of these passes
+  int passes, digit_bits;
+  size_t padded, counts, partial;   // elements: a key or row array, the digits' counts, the parts of runs
 };
-GradientPlan gradient_plan(long rows, long L, long N, long M) {
+// `vec`: units of an access
+GradientPlan gradient_plan(long rows, long L, long N, long M, int vec) {
   GradientPlan p = {};
   p.entries = (unsigned)(rows * L);
-  p.rank = p.entries <= kRankMost;
-  // as many chunks as keep all threads busy with a vector of 16 bytes each, of 8 to 64 entries
-  const long want = 2048l * sm_count() * 4;
-  long chunk = (long)p.entries * M / want / 8 * 8;
+  p.rank = p.entries <= rank_most();
+  p.cluster = !p.rank && p.entries <= cl_most() && cluster_fits();
+  const long across = M / vec;
+  p.lanes = 4;
+  while (p.lanes < 32 && p.lanes < across) p.lanes *= 2;
+  p.tiles = (unsigned)((across + p.lanes - 1) / p.lanes);
+  // as many chunks as keep all threads busy, of 8 to 64 entries
+  const long want = 2048l * sm_count() / p.lanes;
+  long chunk = (long)p.entries * p.tiles / want / 8 * 8;
   chunk = chunk < 8 ? 8 : chunk > 64 ? 64 : chunk;
   p.chunk = (unsigned)chunk;
-  p.chunks = (p.entries + p.chunk - 1) / p.chunk;
+  p.span = p.chunk * (kThreads / p.lanes);
+  p.spans = (p.entries + p.span - 1) / p.span;
   p.padded = ((size_t)p.entries + 7) / 8 * 8;
-  p.some = ((size_t)N + 7) / 8 * 8;
-  p.partial = p.chunks > 1 ? 2 * (size_t)p.chunks * (size_t)M : 0;
-  if (!p.rank) {
-    int bits = 1;
-    while (bits < 32 && (N >> bits) != 0) ++bits;   // N stands for codes that name nothing
-    p.passes = (bits + kDigitBits - 1) / kDigitBits;
+  p.partial = p.spans > 1 ? 2 * (size_t)p.spans * (size_t)M : 0;
+  int bits = 1;
+  while (bits < 32 && (N >> bits) != 0) ++bits;   // N stands for codes that name nothing
+  p.passes = (bits + kDigitBits - 1) / kDigitBits;
+  p.digit_bits = (bits + p.passes - 1) / p.passes;
+  if (!p.rank && !p.cluster) {
     // up to 128 tiles: every block of a pass reads the counts of all
     p.tile = ((p.entries + 127) / 128 + kSortThreads - 1) / kSortThreads * kSortThreads;
     if (p.tile < 1024) p.tile = 1024;
@@ -505,24 +707,27 @@ GradientPlan gradient_plan(long rows, long L, long N, long M) {
   return p;
 }
 
+template <typename I, int EACH>
+cudaError_t launch_sort(const I *codes, const GradientPlan &p, long L, long N, unsigned *key, unsigned *row, const Zero &zero, cudaStream_t st) {
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr[2];
+  const cudaError_t e = sort_config<I, EACH>(cfg, attr, p.passes, st);
+  if (e != cudaSuccess) return e;
+  cfg.gridDim = dim3(kClusterBlocks * (1 + (zero_blocks(zero) + kClusterBlocks - 1) / kClusterBlocks));
+  return cudaLaunchKernelEx(&cfg, sort_kernel<I, EACH>, codes, p.entries, (unsigned)L, N, p.passes, p.digit_bits, key, row, zero);
+}
+
 template <typename T, int V>
-cudaError_t launch_sums(Sums<T, V> p, unsigned chunks, cudaStream_t st) {
-  const long across = p.M / V;
-  p.lanes = 4;
-  while (p.lanes < 32 && p.lanes < across) p.lanes *= 2;
-  p.tiles = (unsigned)((across + p.lanes - 1) / p.lanes);
-  const unsigned per = kThreads / p.lanes;
-  const long zero_rows = 32768 / (p.M * (long)sizeof(T));   // 32 KB a block
-  p.zero_rows = (int)(zero_rows < 1 ? 1 : zero_rows > kZeroRows ? kZeroRows : zero_rows);
-  const size_t blocks = ((size_t)chunks * p.tiles + per - 1) / per, zero = p.accumulate ? 0 : ((size_t)p.N + p.zero_rows - 1) / p.zero_rows;
-  if (blocks + zero > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  const size_t smem = (2 * ((per + p.tiles - 1) / p.tiles + 1) * (size_t)p.chunk + 2) * sizeof(unsigned);
-  cudaError_t e = launch_next(sums_kernel<T, V>, dim3((unsigned)(blocks + zero)), kThreads, smem, st, p, (unsigned)blocks, (unsigned)zero);
+cudaError_t launch_sums(const Sums<T, V> &p, unsigned spans, cudaStream_t st) {
+  const size_t blocks = (size_t)spans * p.tiles;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const size_t smem = (2 * (size_t)p.span + 2) * sizeof(unsigned);
+  cudaError_t e = launch_next(sums_kernel<T, V>, dim3((unsigned)blocks), kThreads, smem, st, p);
   if (e != cudaSuccess) return e;
   count_launches(1);
-  if (chunks == 1) return e;
-  const size_t join = (((size_t)chunks + per - 1) / per) * p.tiles;
-  e = launch_next(join_kernel<T, V>, dim3((unsigned)join), kThreads, 0, st, p);
+  if (spans == 1) return e;
+  const unsigned per = kThreads / p.lanes;
+  e = launch_next(join_kernel<T, V>, dim3((spans + per - 1) / per * p.tiles), kThreads, 0, st, p);
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
@@ -547,18 +752,41 @@ cudaError_t launch_lookup(const T *weights, const I *codes, long rows, long L, l
 }
 
 size_t lookup_gradient_workspace(long rows, long L, long N, long M, size_t wide) {
-  const GradientPlan p = gradient_plan(rows, L, N, M);
-  return ((p.rank ? 2 : 4) * p.padded + p.counts + p.some) * sizeof(unsigned) + 64 + p.partial * wide;
+  GradientPlan p = gradient_plan(rows, L, N, M, 1);
+  for (int vec = 2; vec <= 8 && M % vec == 0; vec *= 2) {   // the width of the accesses depends on addresses
+    const size_t partial = gradient_plan(rows, L, N, M, vec).partial;
+    if (partial > p.partial) p.partial = partial;
+  }
+  return ((p.rank || p.cluster ? 2 : 4) * p.padded + p.counts) * sizeof(unsigned) + 64 + p.partial * wide;
 }
 
 template <typename T, typename I>
 cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, long L, long N, long M, double scale, bool accumulate, T *out,
                                    void *workspace, cudaStream_t st) {
-  const GradientPlan p = gradient_plan(rows, L, N, M);
-  unsigned *key = static_cast<unsigned *>(workspace), *row = key + p.padded, *const some = accumulate ? nullptr : row + p.padded, *end = row + p.padded + p.some;
+  const int vec = vector_width<T>(M, grad, out);
+  const GradientPlan p = gradient_plan(rows, L, N, M, vec);
+  unsigned *key = static_cast<unsigned *>(workspace), *row = key + p.padded, *end = row + p.padded;
+  // the result's bytes over the sort's launches
+  const size_t bytes = accumulate ? 0 : (size_t)N * (size_t)M * sizeof(T);
+  auto zero = [&](int launch, int launches) {
+    const size_t from = bytes / launches / 256 * 256 * launch, to = launch + 1 == launches ? bytes : bytes / launches / 256 * 256 * (launch + 1);
+    return Zero{reinterpret_cast<unsigned char *>(out) + from, to - from};
+  };
+  if (bytes / kZeroBlock > 0x40000000) return cudaErrorInvalidConfiguration;
   cudaError_t e;
   if (p.rank) {
-    e = launch_next(rank_kernel<I>, dim3((p.entries + kThreads / 8 - 1) / (kThreads / 8)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, key, row, some);
+    const Zero z = zero(0, 1);
+    const unsigned blocks = (p.entries + kThreads / 8 - 1) / (kThreads / 8);
+    e = launch_next(rank_kernel<I>, dim3(blocks + zero_blocks(z)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, key, row, blocks, z);
+    if (e != cudaSuccess) return e;
+    count_launches(1);
+  } else if (p.cluster) {
+    const unsigned each = (p.entries + kClusterThreads * kClusterBlocks - 1) / (kClusterThreads * kClusterBlocks);
+    const Zero z = zero(0, 1);
+    e = each <= 1   ? launch_sort<I, 1>(codes, p, L, N, key, row, z, st)
+        : each <= 2 ? launch_sort<I, 2>(codes, p, L, N, key, row, z, st)
+        : each <= 4 ? launch_sort<I, 4>(codes, p, L, N, key, row, z, st)
+                    : launch_sort<I, 8>(codes, p, L, N, key, row, z, st);
     if (e != cudaSuccess) return e;
     count_launches(1);
   } else {
@@ -566,15 +794,13 @@ cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, lon
     end = counts + p.counts;
     for (int pass = 0; pass < p.passes; ++pass) {
       const int shift = pass * kDigitBits;
-      const bool first = pass == 0;
-      unsigned *const last = pass + 1 == p.passes ? some : nullptr;
-      e = first ? launch_next(digits_kernel<I, true>, dim3(p.blocks), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts)
-                : launch_next(digits_kernel<I, false>, dim3(p.blocks), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts);
+      const Zero z = zero(2 * pass, 2 * p.passes), z2 = zero(2 * pass + 1, 2 * p.passes);
+      auto digits = pass == 0 ? digits_kernel<I, true> : digits_kernel<I, false>;
+      auto move = pass == 0 ? move_kernel<I, true> : move_kernel<I, false>;
+      e = launch_next(digits, dim3(p.blocks + zero_blocks(z)), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts, p.blocks, z);
       if (e != cudaSuccess) return e;
-      e = first ? launch_next(move_kernel<I, true>, dim3(p.blocks), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile,
-                              counts, key2, row2, last)
-                : launch_next(move_kernel<I, false>, dim3(p.blocks), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile,
-                              counts, key2, row2, last);
+      e = launch_next(move, dim3(p.blocks + zero_blocks(z2)), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile, counts, key2,
+                      row2, p.blocks, z2);
       if (e != cudaSuccess) return e;
       count_launches(2);
       unsigned *const k = key, *const r = row;
@@ -582,13 +808,12 @@ cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, lon
     }
   }
   Wide<T> *const partial = reinterpret_cast<Wide<T> *>((reinterpret_cast<uintptr_t>(end) + 63) / 64 * 64);   // (read 32 bytes at a time)
-  const int vec = vector_width<T>(M, grad, out);
   const Wide<T> s = (Wide<T>)scale;
-  constexpr int V = 16 / (int)sizeof(T);
-  if (vec == V) return launch_sums(Sums<T, V>{grad, key, row, some, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+#define SBB_SUMS(V) launch_sums(Sums<T, V>{grad, key, row, p.entries, p.chunk, p.span, N, M, s, accumulate, out, partial, p.lanes, p.tiles}, p.spans, st)
   if constexpr (sizeof(T) == 2)
-    if (vec == 2) return launch_sums(Sums<T, 2>{grad, key, row, some, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
-  return launch_sums(Sums<T, 1>{grad, key, row, some, p.entries, p.chunk, N, M, s, accumulate, out, partial, 0, 0}, p.chunks, st);
+    if (vec == 2) return SBB_SUMS(2);
+  return vec == 1 ? SBB_SUMS(1) : SBB_SUMS(16 / (int)sizeof(T));
+#undef SBB_SUMS
 }
 
 #define SBB_INSTANCE(T, I)                                                                                              \
