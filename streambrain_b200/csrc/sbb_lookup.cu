@@ -3,7 +3,6 @@
 #include "sbb_launch.cuh"
 
 #include <cooperative_groups.h>
-#include <cstdlib>
 
 namespace cg = cooperative_groups;
 
@@ -151,7 +150,9 @@ cudaError_t launch_lookup_as(const T *weights, const I *codes, long rows, long L
 // into equal chunks and these joined to spans: a block writes the runs that lie in its span and leaves the part of a run that
 // crosses the span's border in the workspace, from where join_kernel adds the parts in order.
 
-constexpr unsigned kRankMost = 8192;   // entries that are ranked by comparing all with all
+// Entries that are ranked by comparing all with all, and that a cluster sorts.  Codes of 30000 x 64 float32, us a call: 4000 12.0 and
+// (cluster) 15.0, 5000 14.4 and 15.4, 8000 22.9 and 15.5; 64000 (cluster) 27 and (launches for every pass) 37, 130000 46 and 61.
+constexpr unsigned kRankMost = 5120, kClusterMost = 131072;
 
 __device__ __forceinline__ unsigned key_of(long code, long N) { return code >= 0 && code < N ? (unsigned)code : (unsigned)N; }
 
@@ -162,8 +163,8 @@ struct Zero {
   unsigned char *begin;
   size_t bytes;
 };
-constexpr size_t kZeroBlock = 64 * 1024;
-inline unsigned zero_blocks(const Zero &z) { return (unsigned)((z.bytes + kZeroBlock - 1) / kZeroBlock); }
+constexpr size_t kZeroBlock = 64 * 1024;   // bytes of a block
+__host__ __device__ __forceinline__ unsigned zero_blocks(const Zero &z) { return (unsigned)((z.bytes + kZeroBlock - 1) / kZeroBlock); }
 __device__ __forceinline__ void set_zero(const Zero &z, unsigned block) {
   unsigned char *const from = z.begin + block * kZeroBlock;
   const size_t bytes = min(kZeroBlock, z.bytes - block * kZeroBlock);
@@ -182,8 +183,7 @@ __device__ __forceinline__ unsigned below(unsigned a, unsigned b) { return (a - 
 // one launch where a radix sort is four.
 template <typename I>
 __global__ void __launch_bounds__(kThreads)
-    rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, unsigned *__restrict__ key, unsigned *__restrict__ row,
-                unsigned blocks, const Zero zero) {
+    rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, uint2 *__restrict__ to, unsigned blocks, const Zero zero) {
   after_previous();
   if (blockIdx.x >= blocks) return set_zero(zero, blockIdx.x - blocks);
   __shared__ uint4 s_key[kRankMost / 4];
@@ -219,8 +219,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
     for (int o = 0; o < 4; ++o) r += o < q ? k[o] <= k[q] : k[o] < k[q];
     if (lane == 0 && e0 + q < entries) {
-      key[r] = k[q];
-      row[r] = (e0 + q) / L;
+      to[r] = make_uint2(k[q], (e0 + q) / L);
     }
   }
 }
@@ -229,13 +228,13 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kDigitBits = 9, kDigits = 1 << kDigitBits;
 
 template <typename I, bool FIRST>
-__device__ __forceinline__ unsigned sort_key(const I *codes, const unsigned *key, unsigned i, long N) {
-  return FIRST ? key_of((long)codes[i], N) : key[i];
+__device__ __forceinline__ unsigned sort_key(const I *codes, const uint2 *from, unsigned i, long N) {
+  return FIRST ? key_of((long)codes[i], N) : from[i].x;
 }
 
 template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
-    digits_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, unsigned entries, long N, int shift, unsigned tile,
+    digits_kernel(const I *__restrict__ codes, const uint2 *__restrict__ key, unsigned entries, long N, int shift, unsigned tile,
                   unsigned *__restrict__ counts, unsigned blocks, const Zero zero) {
   after_previous();
   if (blockIdx.x >= blocks) return set_zero(zero, blockIdx.x - blocks);
@@ -253,9 +252,8 @@ __global__ void __launch_bounds__(kSortThreads)
 // in its own warp in front.
 template <typename I, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads)
-    move_kernel(const I *__restrict__ codes, const unsigned *__restrict__ key, const unsigned *__restrict__ row, unsigned entries, unsigned L, long N,
-                int shift, unsigned tile, const unsigned *__restrict__ counts, unsigned *__restrict__ key_to, unsigned *__restrict__ row_to,
-                unsigned blocks, const Zero zero) {
+    move_kernel(const I *__restrict__ codes, const uint2 *__restrict__ key, unsigned entries, unsigned L, long N, int shift, unsigned tile,
+                const unsigned *__restrict__ counts, uint2 *__restrict__ to_entry, unsigned blocks, const Zero zero) {
   after_previous();
   if (blockIdx.x >= blocks) return set_zero(zero, blockIdx.x - blocks);
   static_assert(kDigits == kSortThreads, "a thread per digit");
@@ -290,13 +288,13 @@ __global__ void __launch_bounds__(kSortThreads)
   __syncthreads();
   for (unsigned i0 = lo; i0 < hi; i0 += 32) {
     const bool there = i0 + lane < hi;
-    const unsigned kk = there ? sort_key<I, FIRST>(codes, key, i0 + lane, N) : 0;
+    const uint2 own = !there ? make_uint2(0, 0) : FIRST ? make_uint2(key_of((long)codes[i0 + lane], N), (i0 + lane) / L) : key[i0 + lane];
+    const unsigned kk = own.x;
     const unsigned digit = there ? (kk >> shift) & (kDigits - 1) : kDigits;
     const unsigned same = __match_any_sync(0xffffffffu, digit);
     if (there) {
       const unsigned to = s_at[warp][digit] + __popc(same & ((1u << lane) - 1));
-      key_to[to] = kk;
-      row_to[to] = FIRST ? (i0 + lane) / L : row[i0 + lane];
+      to_entry[to] = own;
     }
     __syncwarp();
     if (there && (same >> lane) == 1u) s_at[warp][digit] += __popc(same);   // the last of its kind
@@ -305,26 +303,31 @@ __global__ void __launch_bounds__(kSortThreads)
 }
 
 // The same sort by one cluster in one launch, for as many entries as its threads hold: an entry's place is found in registers and
-// shared memory, and the entries move between the blocks' shared memories.
+// shared memory, and the entries move between the blocks' shared memories.  They are put in order within the block first, so that
+// neighbours go to neighbouring places (one by one, each store was 32 requests, and 65536 entries took 24 us).
 constexpr int kClusterThreads = 1024, kClusterWarps = kClusterThreads / 32, kClusterBlocks = 16;
 
 struct SortSpace {
   unsigned short at[kClusterWarps][kDigits];
-  unsigned all[kDigits], base[kDigits], warp[kClusterWarps];
+  unsigned all[kDigits];               // the block's entries of each digit
+  unsigned own[kDigits], base[kDigits];  // where a digit begins in the block, and where its entries go
+  unsigned warp[2][kClusterWarps];
 };
 
-// EACH entries a thread.  `hold`: two words for each of the block's entries, where there is more than one pass.
+// EACH entries a thread.  `space`: two entries' room for each of the block's.
 template <typename I, int EACH>
-__device__ void cluster_sort(cg::cluster_group cluster, SortSpace &s, unsigned *hold, const I *codes, unsigned entries, unsigned L, long N, int passes,
-                             int digit_bits, unsigned *key_to, unsigned *row_to) {
+__device__ void cluster_sort(cg::cluster_group cluster, SortSpace &s, uint2 *space, const I *codes, unsigned entries, unsigned L, long N, int passes,
+                             int digit_bits, uint2 *result) {
   constexpr unsigned kHere = kClusterThreads * EACH;
+  uint2 *const hold = space, *const order = space + kHere;
   const unsigned rank = cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1u << digit_bits;
   const unsigned slot0 = warp * (32 * EACH) + lane, first = rank * kHere + slot0;   // a warp's entries lie together
-  unsigned key[EACH], row[EACH];
+  const unsigned here = entries > rank * kHere ? min(kHere, entries - rank * kHere) : 0;
+  uint2 entry[EACH];
 #pragma unroll
-  for (int r = 0; r < EACH; ++r) key[r] = first + r * 32 < entries ? key_of((long)codes[first + r * 32], N) : ~0u;
+  for (int r = 0; r < EACH; ++r) entry[r].x = first + r * 32 < entries ? key_of((long)codes[first + r * 32], N) : ~0u;
 #pragma unroll
-  for (int r = 0; r < EACH; ++r) row[r] = (first + r * 32) / L;
+  for (int r = 0; r < EACH; ++r) entry[r].y = (first + r * 32) / L;
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
     for (unsigned i = threadIdx.x; i < kClusterWarps * kDigits / 2; i += kClusterThreads) reinterpret_cast<unsigned *>(s.at)[i] = 0;
@@ -333,7 +336,7 @@ __device__ void cluster_sort(cg::cluster_group cluster, SortSpace &s, unsigned *
 #pragma unroll
     for (int r = 0; r < EACH; ++r) {
       const bool there = first + r * 32 < entries;
-      const unsigned digit = there ? (key[r] >> shift) & (digits - 1) : kDigits + 1;
+      const unsigned digit = there ? (entry[r].x >> shift) & (digits - 1) : kDigits + 1;
       const unsigned same = __match_any_sync(0xffffffffu, digit), front = __popc(same & ((1u << lane) - 1));
       if (there) place[r] = (unsigned short)(s.at[warp][digit] + front);
       __syncwarp();
@@ -341,8 +344,8 @@ __device__ void cluster_sort(cg::cluster_group cluster, SortSpace &s, unsigned *
       __syncwarp();
     }
     __syncthreads();
+    unsigned run = 0;
     if (threadIdx.x < digits) {
-      unsigned run = 0;
 #pragma unroll 8
       for (int w = 0; w < kClusterWarps; ++w) {
         const unsigned c = s.at[w][threadIdx.x];
@@ -360,58 +363,64 @@ __device__ void cluster_sort(cg::cluster_group cluster, SortSpace &s, unsigned *
         all += c;
         before += o < rank ? c : 0;
       }
-    unsigned in = all;
+    unsigned in = all, in_own = run;
     for (int off = 1; off < 32; off *= 2) {
-      const unsigned o = __shfl_up_sync(0xffffffffu, in, off);
-      if (lane >= off) in += o;
+      const unsigned o = __shfl_up_sync(0xffffffffu, in, off), p = __shfl_up_sync(0xffffffffu, in_own, off);
+      if (lane >= off) in += o, in_own += p;
     }
-    if (lane == 31) s.warp[warp] = in;
+    if (lane == 31) s.warp[0][warp] = in, s.warp[1][warp] = in_own;
     __syncthreads();
     if (threadIdx.x < digits) {
-      unsigned base = before + in - all;
-      for (unsigned w = 0; w < warp; ++w) base += s.warp[w];
+      unsigned base = before + in - all, own = in_own - run;
+      for (unsigned w = 0; w < warp; ++w) base += s.warp[0][w], own += s.warp[1][w];
       s.base[threadIdx.x] = base;
+      s.own[threadIdx.x] = own;
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < EACH; ++r) {
-      if (first + r * 32 >= entries) continue;
-      const unsigned digit = (key[r] >> shift) & (digits - 1), to = s.base[digit] + s.at[warp][digit] + place[r];
-      if (pass + 1 == passes) {
-        key_to[to] = key[r];
-        row_to[to] = row[r];
-      } else {
-        unsigned *const there = cluster.map_shared_rank(hold, to / kHere) + to % kHere;
-        there[0] = key[r];
-        there[kHere] = row[r];
+    for (int r = 0; r < EACH; ++r)
+      if (first + r * 32 < entries) {
+        const unsigned digit = (entry[r].x >> shift) & (digits - 1);
+        order[s.own[digit] + s.at[warp][digit] + place[r]] = entry[r];
       }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+      const unsigned i = threadIdx.x + r * kClusterThreads;
+      if (i >= here) continue;
+      const uint2 e = order[i];
+      const unsigned digit = (e.x >> shift) & (digits - 1), to = s.base[digit] + i - s.own[digit];
+      if (pass + 1 == passes)
+        result[to] = e;
+      else
+        cluster.map_shared_rank(hold, to / kHere)[to % kHere] = e;
     }
     cluster.sync();
     if (pass + 1 < passes) {
 #pragma unroll
-      for (int r = 0; r < EACH; ++r) key[r] = hold[slot0 + r * 32], row[r] = hold[kHere + slot0 + r * 32];
+      for (int r = 0; r < EACH; ++r) entry[r] = hold[slot0 + r * 32];
     }
   }
 }
 
 template <typename I, int EACH>
 __global__ void __launch_bounds__(kClusterThreads, 1)
-    sort_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, int passes, int digit_bits, unsigned *__restrict__ key,
-                unsigned *__restrict__ row, const Zero zero) {
+    sort_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, int passes, int digit_bits, uint2 *__restrict__ result,
+                const Zero zero) {
   after_previous();
   if (blockIdx.x >= kClusterBlocks) {   // (whole clusters; those behind the last piece have none)
-    if (blockIdx.x - kClusterBlocks < (zero.bytes + kZeroBlock - 1) / kZeroBlock) set_zero(zero, blockIdx.x - kClusterBlocks);
+    if (blockIdx.x - kClusterBlocks < zero_blocks(zero)) set_zero(zero, blockIdx.x - kClusterBlocks);
     return;
   }
-  extern __shared__ unsigned s_hold[];
+  extern __shared__ uint2 s_space[];
   __shared__ SortSpace s;
-  cluster_sort<I, EACH>(cg::this_cluster(), s, s_hold, codes, entries, L, N, passes, digit_bits, key, row);
+  cluster_sort<I, EACH>(cg::this_cluster(), s, s_space, codes, entries, L, N, passes, digit_bits, result);
 }
 
 template <typename T, int V>
 struct Sums {
   const T *grad;
-  const unsigned *key, *row;   // sorted
+  const uint2 *entry;   // sorted: code, row of the gradient
   unsigned entries, chunk, span;   // of a group of threads, of a block
   long N, M;
   Wide<T> scale;
@@ -446,9 +455,10 @@ __global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p) {
   unsigned *const s_key = s_entry + 1, *const s_row = s_entry + size + 2;
   for (unsigned i = threadIdx.x; i < size + 2; i += kThreads) {
     const unsigned at = first + i - 1;   // (wraps below zero)
-    s_entry[i] = at < p.entries ? p.key[at] : ~0u;
+    const uint2 own = at < p.entries ? p.entry[at] : make_uint2(~0u, 0);
+    s_entry[i] = own.x;
+    if (i > 0 && i <= size) s_row[i - 1] = own.y;
   }
-  for (unsigned i = threadIdx.x; i < size; i += kThreads) s_row[i] = p.row[first + i];
   __syncthreads();
   const unsigned group = threadIdx.x / p.lanes, b = group * p.chunk, e = min(size, b + p.chunk);
   const long col = ((long)(blockIdx.x % p.tiles) * p.lanes + threadIdx.x % p.lanes) * V;
@@ -570,15 +580,15 @@ __device__ __forceinline__ void join_runs(const Sums<T, V> &p, unsigned block, J
   unsigned cur = 0, last = 0;
   if (c + 1 < spans) {
     const unsigned b = c * p.span, e = b + p.span;
-    cur = p.key[e - 1];
-    if (p.key[e] == cur && cur < (unsigned)p.N && !(b > 0 && p.key[b] == cur && p.key[b - 1] == cur)) {
+    cur = p.entry[e - 1].x;
+    if (p.entry[e].x == cur && cur < (unsigned)p.N && !(b > 0 && p.entry[b].x == cur && p.entry[b - 1].x == cur)) {
       // the last span that begins inside the run: the group's threads try that many places at a time
       last = c + 1;
       unsigned end = spans;
       const unsigned mask = (p.lanes == 32 ? ~0u : (1u << p.lanes) - 1) << (threadIdx.x & 31 & ~(p.lanes - 1));
       for (unsigned step = 1; last + 1 < end; step = (end - last - 1 + p.lanes - 1) / p.lanes) {   // first those that follow
         const unsigned at = last + (lane + 1) * step;
-        const int in = __popc(__ballot_sync(mask, at < end && p.key[at * p.span] == cur));
+        const int in = __popc(__ballot_sync(mask, at < end && p.entry[at * p.span].x == cur));
         last += in * step;
         if (in < p.lanes) end = min(end, last + step);
       }
@@ -625,8 +635,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Sums<T, V> p) {
 
 // Whether the device takes a cluster of sixteen blocks (eight are what every device takes).
 template <typename I, int EACH>
-cudaError_t sort_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[2], int passes, cudaStream_t st) {
-  const size_t smem = passes > 1 ? 2 * sizeof(unsigned) * kClusterThreads * EACH : 0;
+cudaError_t sort_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute (&attr)[2], cudaStream_t st) {
+  const size_t smem = 2 * sizeof(uint2) * kClusterThreads * EACH;
   cudaError_t e = cudaFuncSetAttribute(sort_kernel<I, EACH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(sort_kernel<I, EACH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -648,22 +658,13 @@ bool cluster_fits() {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
     int clusters = 0;
-    cudaError_t e = sort_config<int64_t, 8>(cfg, attr, 2, nullptr);
+    cudaError_t e = sort_config<int64_t, 8>(cfg, attr, nullptr);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, sort_kernel<int64_t, 8>, &cfg);
     if (e != cudaSuccess) (void)cudaGetLastError();
     return e == cudaSuccess && clusters > 0;
   }();
   return fits;
 }
-unsigned cl_most() {
-  static const unsigned most = getenv("SBB_CL") ? atoi(getenv("SBB_CL")) : 8 * kClusterThreads * kClusterBlocks;
-  return most;
-}
-unsigned rank_most() {
-  static const unsigned most = getenv("SBB_RANK") ? atoi(getenv("SBB_RANK")) : kRankMost;
-  return most;
-}
-
 // Sizes of a gradient call.
 struct GradientPlan {
   unsigned entries, chunk, span, spans;
@@ -672,14 +673,14 @@ struct GradientPlan {
   bool rank, cluster;      // how the codes are sorted; else by launches for every pass
   unsigned tile, blocks;   // of these passes
   int passes, digit_bits;
-  size_t padded, counts, partial;   // elements: a key or row array, the digits' counts, the parts of runs
+  size_t counts, partial;   // elements: the digits' counts, the parts of runs
 };
 // `vec`: units of an access
 GradientPlan gradient_plan(long rows, long L, long N, long M, int vec) {
   GradientPlan p = {};
   p.entries = (unsigned)(rows * L);
-  p.rank = p.entries <= rank_most();
-  p.cluster = !p.rank && p.entries <= cl_most() && cluster_fits();
+  p.rank = p.entries <= kRankMost;
+  p.cluster = !p.rank && p.entries <= kClusterMost && cluster_fits();
   const long across = M / vec;
   p.lanes = 4;
   while (p.lanes < 32 && p.lanes < across) p.lanes *= 2;
@@ -691,7 +692,6 @@ GradientPlan gradient_plan(long rows, long L, long N, long M, int vec) {
   p.chunk = (unsigned)chunk;
   p.span = p.chunk * (kThreads / p.lanes);
   p.spans = (p.entries + p.span - 1) / p.span;
-  p.padded = ((size_t)p.entries + 7) / 8 * 8;
   p.partial = p.spans > 1 ? 2 * (size_t)p.spans * (size_t)M : 0;
   int bits = 1;
   while (bits < 32 && (N >> bits) != 0) ++bits;   // N stands for codes that name nothing
@@ -708,13 +708,13 @@ GradientPlan gradient_plan(long rows, long L, long N, long M, int vec) {
 }
 
 template <typename I, int EACH>
-cudaError_t launch_sort(const I *codes, const GradientPlan &p, long L, long N, unsigned *key, unsigned *row, const Zero &zero, cudaStream_t st) {
+cudaError_t launch_sort(const I *codes, const GradientPlan &p, long L, long N, uint2 *entry, const Zero &zero, cudaStream_t st) {
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  const cudaError_t e = sort_config<I, EACH>(cfg, attr, p.passes, st);
+  const cudaError_t e = sort_config<I, EACH>(cfg, attr, st);
   if (e != cudaSuccess) return e;
   cfg.gridDim = dim3(kClusterBlocks * (1 + (zero_blocks(zero) + kClusterBlocks - 1) / kClusterBlocks));
-  return cudaLaunchKernelEx(&cfg, sort_kernel<I, EACH>, codes, p.entries, (unsigned)L, N, p.passes, p.digit_bits, key, row, zero);
+  return cudaLaunchKernelEx(&cfg, sort_kernel<I, EACH>, codes, p.entries, (unsigned)L, N, p.passes, p.digit_bits, entry, zero);
 }
 
 template <typename T, int V>
@@ -757,7 +757,7 @@ size_t lookup_gradient_workspace(long rows, long L, long N, long M, size_t wide)
     const size_t partial = gradient_plan(rows, L, N, M, vec).partial;
     if (partial > p.partial) p.partial = partial;
   }
-  return ((p.rank || p.cluster ? 2 : 4) * p.padded + p.counts) * sizeof(unsigned) + 64 + p.partial * wide;
+  return (p.rank || p.cluster ? 1 : 2) * (size_t)p.entries * sizeof(uint2) + p.counts * sizeof(unsigned) + 64 + p.partial * wide;
 }
 
 template <typename T, typename I>
@@ -765,7 +765,8 @@ cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, lon
                                    void *workspace, cudaStream_t st) {
   const int vec = vector_width<T>(M, grad, out);
   const GradientPlan p = gradient_plan(rows, L, N, M, vec);
-  unsigned *key = static_cast<unsigned *>(workspace), *row = key + p.padded, *end = row + p.padded;
+  uint2 *entry = static_cast<uint2 *>(workspace);
+  void *end = entry + p.entries;
   // the result's bytes over the sort's launches
   const size_t bytes = accumulate ? 0 : (size_t)N * (size_t)M * sizeof(T);
   auto zero = [&](int launch, int launches) {
@@ -777,39 +778,40 @@ cudaError_t launch_lookup_gradient(const T *grad, const I *codes, long rows, lon
   if (p.rank) {
     const Zero z = zero(0, 1);
     const unsigned blocks = (p.entries + kThreads / 8 - 1) / (kThreads / 8);
-    e = launch_next(rank_kernel<I>, dim3(blocks + zero_blocks(z)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, key, row, blocks, z);
+    e = launch_next(rank_kernel<I>, dim3(blocks + zero_blocks(z)), kThreads, 0, st, codes, p.entries, (unsigned)L, N, entry, blocks, z);
     if (e != cudaSuccess) return e;
     count_launches(1);
   } else if (p.cluster) {
     const unsigned each = (p.entries + kClusterThreads * kClusterBlocks - 1) / (kClusterThreads * kClusterBlocks);
     const Zero z = zero(0, 1);
-    e = each <= 1   ? launch_sort<I, 1>(codes, p, L, N, key, row, z, st)
-        : each <= 2 ? launch_sort<I, 2>(codes, p, L, N, key, row, z, st)
-        : each <= 4 ? launch_sort<I, 4>(codes, p, L, N, key, row, z, st)
-                    : launch_sort<I, 8>(codes, p, L, N, key, row, z, st);
+    e = each <= 1   ? launch_sort<I, 1>(codes, p, L, N, entry, z, st)
+        : each <= 2 ? launch_sort<I, 2>(codes, p, L, N, entry, z, st)
+        : each <= 4 ? launch_sort<I, 4>(codes, p, L, N, entry, z, st)
+                    : launch_sort<I, 8>(codes, p, L, N, entry, z, st);
     if (e != cudaSuccess) return e;
     count_launches(1);
   } else {
-    unsigned *key2 = end, *row2 = key2 + p.padded, *counts = row2 + p.padded;
+    uint2 *other = entry + p.entries;
+    unsigned *const counts = reinterpret_cast<unsigned *>(other + p.entries);
     end = counts + p.counts;
     for (int pass = 0; pass < p.passes; ++pass) {
       const int shift = pass * kDigitBits;
       const Zero z = zero(2 * pass, 2 * p.passes), z2 = zero(2 * pass + 1, 2 * p.passes);
       auto digits = pass == 0 ? digits_kernel<I, true> : digits_kernel<I, false>;
       auto move = pass == 0 ? move_kernel<I, true> : move_kernel<I, false>;
-      e = launch_next(digits, dim3(p.blocks + zero_blocks(z)), kSortThreads, 0, st, codes, key, p.entries, N, shift, p.tile, counts, p.blocks, z);
+      e = launch_next(digits, dim3(p.blocks + zero_blocks(z)), kSortThreads, 0, st, codes, entry, p.entries, N, shift, p.tile, counts, p.blocks, z);
       if (e != cudaSuccess) return e;
-      e = launch_next(move, dim3(p.blocks + zero_blocks(z2)), kSortThreads, 0, st, codes, key, row, p.entries, (unsigned)L, N, shift, p.tile, counts, key2,
-                      row2, p.blocks, z2);
+      e = launch_next(move, dim3(p.blocks + zero_blocks(z2)), kSortThreads, 0, st, codes, entry, p.entries, (unsigned)L, N, shift, p.tile, counts, other,
+                      p.blocks, z2);
       if (e != cudaSuccess) return e;
       count_launches(2);
-      unsigned *const k = key, *const r = row;
-      key = key2, row = row2, key2 = k, row2 = r;
+      uint2 *const moved = other;
+      other = entry, entry = moved;
     }
   }
   Wide<T> *const partial = reinterpret_cast<Wide<T> *>((reinterpret_cast<uintptr_t>(end) + 63) / 64 * 64);   // (read 32 bytes at a time)
   const Wide<T> s = (Wide<T>)scale;
-#define SBB_SUMS(V) launch_sums(Sums<T, V>{grad, key, row, p.entries, p.chunk, p.span, N, M, s, accumulate, out, partial, p.lanes, p.tiles}, p.spans, st)
+#define SBB_SUMS(V) launch_sums(Sums<T, V>{grad, entry, p.entries, p.chunk, p.span, N, M, s, accumulate, out, partial, p.lanes, p.tiles}, p.spans, st)
   if constexpr (sizeof(T) == 2)
     if (vec == 2) return SBB_SUMS(2);
   return vec == 1 ? SBB_SUMS(1) : SBB_SUMS(16 / (int)sizeof(T));

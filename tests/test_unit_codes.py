@@ -63,10 +63,11 @@ def plain_gradient(grad, codes, n, scale):
     out = torch.zeros((n, g.shape[1]), dtype=F64)
     size, count = torch.zeros_like(out), np.zeros(n, dtype=int)
     for r in range(c.shape[0]):
+        row, row_size = g[r], g[r].abs()
         for code in c[r].tolist():
             if 0 <= code < n:
-                out[code] += g[r]
-                size[code] += g[r].abs()
+                out[code] += row
+                size[code] += row_size
                 count[code] += 1
     return out * scale, size * abs(scale), int(count.max()) if n else 0
 
@@ -192,7 +193,8 @@ def test_lookup(rows, length, n, m, kind, scale, t):
 
 GRADIENTS = LOOKUPS + [  # long runs of equal codes, runs that end anywhere, few and many codes for the table
     (700, 1, 3, 20, "any", 1.0), (1000, 3, 5000, 33, "few", 1.0), (40, 300, 50, 16, "same", 1.0), (5000, 2, 300, 9, "few", 1.0),
-    (9001, 1, 20011, 8, "few", 1.0), (3, 1, 70001, 3, "any", 1.0), (130, 130, 700, 40, "absent", 1.0), (20000, 1, 9, 5, "any", 1.0),
+    (9001, 1, 20011, 8, "few", 1.0), (6000, 3, 100, 6, "any", 1.0), (36000, 1, 300, 4, "few", 1.0), (900, 99, 70001, 3, "absent", 1.0),
+    (140001, 1, 1000, 2, "any", 1.0), (133, 1000, 40, 3, "any", 1.0), (70000, 2, 300, 1, "same", 1.0), (3, 1, 70001, 3, "any", 1.0), (130, 130, 700, 40, "absent", 1.0), (20000, 1, 9, 5, "any", 1.0),
 ]
 
 
