@@ -601,8 +601,9 @@ constexpr unsigned kQuickCount = 256;   // a top-k of up to this many goes by th
 
 struct Block {
   unsigned bin_count[kBins], bin_low[kBins], bin_high[kBins];   // masses in halves
-  u64 list_key[kList], list_mass[kList], sorted_mass[kList];
+  u64 list_key[kList];
   unsigned list_index[kList];
+  u64 sorted_mass[kList];
   double table[kTable];
   u64 sum[kBlockWarps];
   u64 swap[2][2];     // what a block tells the others, in turn
@@ -648,12 +649,13 @@ __device__ __forceinline__ u64 block_before(u64 v, u64 *s) {
 }
 
 // The part of a group that a block works on: units [begin, begin + size), as elements [lead, lead + size) of `vectors` vectors.
-// Elements around them are -infinity (in shared memory, STAGED) or do not exist (V = 1).
+// Elements around them are -infinity: in shared memory, STAGED, they are there; else the first and the last vector are put
+// together from the elements that exist.
 template <typename T, bool STAGED>
 struct Part {
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
-  static constexpr int V = STAGED ? 16 / (int)sizeof(T) : 1;
+  static constexpr int V = 16 / (int)sizeof(T);
   const Vec<T, V> *x;
   unsigned begin, size, lead, vectors;
   W best;
@@ -661,33 +663,65 @@ struct Part {
   cg::cluster_group cluster;
   int turn;
 
-  // f(value, unit) for every unit above -infinity (no NaN is) of vectors [lo, hi), `step` apart
+  // whole vectors: [first_whole(), end_whole())
+  __device__ __forceinline__ unsigned first_whole() const { return STAGED || lead == 0 ? 0 : 1; }
+  __device__ __forceinline__ unsigned end_whole() const { return STAGED ? vectors : (lead + size) / V; }
+  __device__ __forceinline__ Vec<T, V> load(unsigned i) const {
+    if (i >= first_whole() && i < end_whole()) return x[i];
+    Vec<T, V> a;
+    const T *const element = reinterpret_cast<const T *>(x);
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.v[v] = i * V + v >= lead && i * V + v < lead + size ? element[i * V + v] : narrow_to<T>((W)-INFINITY);
+    return a;
+  }
+  // f(vector, its number) for every vector, a thread's in rising order but for the first and the last one where they are not whole
+  // (threads 0 and 32); U in flight, their loads without conditions among them.
+  template <int U, typename F>
+  __device__ __forceinline__ void vectors_of_thread(F f) const {
+    const unsigned end = end_whole();
+    for (unsigned i = first_whole() + threadIdx.x; i < end; i += U * kThreads) {
+      Vec<T, V> a[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < end) a[u] = x[i + u * kThreads];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * kThreads < end) f(a[u], i + u * kThreads);
+    }
+    if constexpr (!STAGED) {
+      if (threadIdx.x == 0 && vectors > 0 && lead > 0) f(load(0), 0);
+      if (threadIdx.x == 32 && vectors > first_whole() && end < vectors) f(load(vectors - 1), vectors - 1);
+    }
+  }
+  // f(value, unit) for the units above -infinity (no NaN is) of a vector
+  template <typename F>
+  __device__ __forceinline__ void units(const Vec<T, V> &a, unsigned i, F f) const {
+    W w[V];
+    widen_all(a, w);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (w[v] > (W)-INFINITY) f(w[v], begin + i * V + v - lead);
+  }
+  // ... of vectors [lo, hi), `step` apart; of all
   template <typename F>
   __device__ __forceinline__ void each(unsigned lo, unsigned hi, unsigned step, F f) const {
-    for (unsigned i = lo; i < hi; i += step) {
-      W w[V];
-      widen_all(x[i], w);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (w[v] > (W)-INFINITY) f(w[v], begin + i * V + v - lead);
-    }
+    for (unsigned i = lo; i < hi; i += step) units(load(i), i, f);
   }
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    each(threadIdx.x, vectors, kThreads, f);
+    vectors_of_thread<STAGED ? 1 : 2>([&](const Vec<T, V> &a, unsigned i) { units(a, i, f); });
   }
   // The same for units of at least `low`, where they are few.
   template <typename F>
   __device__ __forceinline__ void each_from(W low, F f) const {
-    for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
-      const Vec<T, V> a = x[i];
-      if (!(max_all(a) >= low)) continue;
+    vectors_of_thread<STAGED ? 1 : 4>([&](const Vec<T, V> &a, unsigned i) {
+      if (!(max_all(a) >= low)) return;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const W w = widen(a.v[v]);
         if (w >= low && w > (W)-INFINITY) f(w, begin + i * V + v - lead);
       }
-    }
+    });
   }
 
   // f(a, b) of every block's two values, in the blocks' order.
@@ -848,13 +882,31 @@ struct Part {
   }
   // Puts a unit into the first block's list while there is room; s.list there counts all.  (It is 0 at first; the first block sets it
   // back to 0 ahead of a barrier of the cluster.)
-  __device__ __forceinline__ void put(W v, unsigned unit, const Weights &weights) {
-    Block *const first = cluster.map_shared_rank(&s, 0);
+  __device__ __forceinline__ void put(W v, unsigned unit) {
+    Block *const first = cluster.num_blocks() == 1 ? &s : cluster.map_shared_rank(&s, 0);
     const unsigned at = atomicAdd(&first->list, 1u);
     if (at >= kList) return;
-    first->list_key[at] = Keys<W>::of(v);
+    reinterpret_cast<Key *>(first->list_key)[at] = Keys<W>::of(v);
     first->list_index[at] = unit;
-    first->list_mass[at] = weights.of(v, best);
+  }
+  // How many of the first `count` numbers of a list are above (below) one's own: four a step.
+  template <bool ABOVE, typename N>
+  __device__ __forceinline__ unsigned count_of(const N *list, unsigned count, N own, unsigned &equal) const {
+    constexpr int E = 16 / (int)sizeof(N);
+    unsigned c = 0, e = 0;
+#pragma unroll 4
+    for (unsigned j = 0; j < count; j += E) {
+      const Vec<N, E> o = reinterpret_cast<const Vec<N, E> *>(list)[j / E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (j + i < count) {
+          c += ABOVE ? o.v[i] > own : o.v[i] < own;
+          e += o.v[i] == own;
+        }
+      }
+    }
+    equal = e;
+    return c;
   }
   // The first block's list: a thread's entry, its rank in the order and what lies in front of it.
   struct Ranked {
@@ -862,50 +914,52 @@ struct Part {
     unsigned index, rank;
     u64 mass, before;
   };
-  __device__ Ranked rank(unsigned count) {
+  __device__ Ranked rank(unsigned count, const Weights &weights) {
     Ranked r{};
     r.rank = kList;
     if (threadIdx.x < count) {
-      r.key = (Key)s.list_key[threadIdx.x];
+      const Key *const keys = reinterpret_cast<const Key *>(s.list_key);
+      r.key = keys[threadIdx.x];
       r.index = s.list_index[threadIdx.x];
-      r.mass = s.list_mass[threadIdx.x];
-      r.rank = 0;
-#pragma unroll 4
-      for (unsigned j = 0; j < count; ++j) {
-        const Key o = (Key)s.list_key[j];
-        r.rank += o > r.key || (o == r.key && s.list_index[j] < r.index);
-      }
+      r.mass = weights.of(Keys<W>::value(r.key), best);
+      unsigned equal;
+      r.rank = count_of<true>(keys, count, r.key, equal);
+      if (equal > 1)
+        for (unsigned j = 0; j < count; ++j) r.rank += keys[j] == r.key && s.list_index[j] < r.index;
       s.sorted_mass[r.rank] = r.mass;
     }
+    r.before = sum_in_front(count, r.rank);
+    return r;
+  }
+  // Of s.sorted_mass[0 .. count), the sum in front of entry `at`.
+  __device__ __forceinline__ u64 sum_in_front(unsigned count, unsigned at) {
     __syncthreads();
     const u64 before = block_before(threadIdx.x < count ? s.sorted_mass[threadIdx.x] : 0, s.sum);
     __syncthreads();
     if (threadIdx.x < count) s.sorted_mass[threadIdx.x] = before;
     __syncthreads();
-    if (threadIdx.x < count) r.before = s.sorted_mass[r.rank];
-    return r;
+    return threadIdx.x < count ? s.sorted_mass[at] : 0;
   }
-  // The unit drawn from the first block's list, which holds all that may be kept; by that block alone.
-  __device__ void draw(unsigned count, const Settings &set, unsigned n, u64 least, float random, long long base, long long *code) {
-    const Ranked r = rank(count);
+  // The unit drawn from the first block's list, which holds all that may be kept; by that block alone.  `total`: the mass of all
+  // units, where there is no top-k.
+  __device__ void draw(unsigned count, const Settings &set, unsigned n, u64 total, u64 least, const Weights &weights, float random, long long base,
+                       long long *code) {
+    const Ranked r = rank(count, weights);
     bool keep = threadIdx.x < count;
-    u64 all = 0;
     if (set.top_k < n) {
       keep = keep && r.rank < set.top_k;
-      if (set.top_p < 1) all = block_sum(keep ? r.mass : 0, s.sum);
-    } else {
-      all = s.found[3];
+      if (set.top_p < 1) total = block_sum(keep ? r.mass : 0, s.sum);
     }
-    if (set.top_p < 1) keep = keep && want_mass(set.top_p, all).inside(r.rank, r.before);
+    if (set.top_p < 1) keep = keep && want_mass(set.top_p, total).inside(r.rank, r.before);
     keep = keep && r.mass >= least;   // (the largest have 2^q, which is no less)
     const u64 mass = keep ? r.mass : 0, target = target_of(random, block_sum(mass, s.sum));
-    if (threadIdx.x < count) s.list_mass[threadIdx.x] = mass;
-    __syncthreads();
-    if (mass == 0) return;
-    u64 before = 0;
-#pragma unroll 4
-    for (unsigned j = 0; j < count; ++j) before += s.list_index[j] < r.index ? s.list_mass[j] : 0;
-    if (before <= target && target < before + mass) *code = base + r.index;
+    unsigned equal, at = 0;
+    if (threadIdx.x < count) {
+      at = count_of<false>(s.list_index, count, r.index, equal);
+      s.sorted_mass[at] = mass;
+    }
+    const u64 before = sum_in_front(count, at);
+    if (mass > 0 && before <= target && target < before + mass) *code = base + r.index;
   }
 
   // The cut that `want` asks for among all units: bins of equal width in the value's distance from the largest first (`found`, by
@@ -955,12 +1009,12 @@ struct Part {
     }
     cluster.sync();   // (the list is empty)
     each([&](W v, unsigned i) {
-      if (among(v)) put(v, i, weights);
+      if (among(v)) put(v, i);
     });
     cluster.sync();
     if (cluster.block_rank() == 0) {
       const unsigned count = s.list;
-      const Ranked r = rank(count);
+      const Ranked r = rank(count, weights);
       const bool keep = threadIdx.x < count && want.inside(above_count + r.rank, above_mass + r.before);
       const u64 n_kept = block_sum(keep, s.sum);
       if (threadIdx.x == 0) s.list = 0;
@@ -995,57 +1049,28 @@ __global__ void __launch_bounds__(kThreads, 2)
   const Settings set = settings_of(how, g / H, n);
   Weights::fill(s.table);
   if (threadIdx.x == 0) s.list = 0;
-  P p{reinterpret_cast<const Vec<T, V> *>(from), begin, size, 0, size, (W)0, s, cluster, 0};
-  W mine = -INFINITY;   // the largest of the values that pass through this thread
-  if constexpr (STAGED) {
-    Vec<T, V> *const to = reinterpret_cast<Vec<T, V> *>(s_values);
-    T *const element = reinterpret_cast<T *>(s_values);
-    const unsigned head = min(size, (unsigned)((16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15) / (unsigned)sizeof(T));   // up to the first boundary
-    const unsigned body = (size - head) / V, tail = size - head - body * V, first = head ? 1 : 0;
-    p.x = to;
-    p.lead = head ? V - head : 0;
-    p.vectors = (p.lead + size + V - 1) / V;
-    const Vec<T, V> *const x = reinterpret_cast<const Vec<T, V> *>(from + head);
-    constexpr int U = 4;
-    for (unsigned i = threadIdx.x; i < body; i += U * kThreads) {
-      Vec<T, V> a[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < body) a[u] = x[i + u * kThreads];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < body) {
-          to[first + i + u * kThreads] = a[u];
-          mine = fmax(mine, max_all(a[u]));
-        }
-    }
-    const T none = narrow_to<T>((W)-INFINITY);
-    if (threadIdx.x < V) {          // the vector in front of the first boundary
-      const int j = (int)threadIdx.x - (int)p.lead;
-      if (head && (j < 0 || j < (int)head)) {
-        const T a = j < 0 ? none : from[j];
-        element[threadIdx.x] = a;
-        mine = fmax(mine, widen(a));
-      }
-    } else if (threadIdx.x >= 32 && threadIdx.x < 32 + V && tail) {   // and the one behind the last
-      const unsigned j = threadIdx.x - 32;
-      const T a = j < tail ? from[head + body * V + j] : none;
-      element[(first + body) * V + j] = a;
-      mine = fmax(mine, widen(a));
-    }
-  } else {
-    for (unsigned i = threadIdx.x; i < size; i += kThreads) mine = fmax(mine, widen(from[i]));
-  }
+  // vectors begin on 16-byte boundaries of memory, in shared memory too
+  const unsigned lead = (unsigned)(reinterpret_cast<uintptr_t>(from) & 15) / (unsigned)sizeof(T), vectors = size ? (lead + size + V - 1) / V : 0;
+  const Vec<T, V> *const memory = reinterpret_cast<const Vec<T, V> *>(from - lead);
+  W mine = -INFINITY;   // the largest of the values that pass through this thread, and the first vector that has it
+  unsigned where = 0;
+  Part<T, false>{memory, begin, size, lead, vectors, (W)0, s, cluster, 0}.template vectors_of_thread<STAGED ? 4 : 8>([&](const Vec<T, V> &a, unsigned i) {
+    if constexpr (STAGED) reinterpret_cast<Vec<T, V> *>(s_values)[i] = a;
+    const W m = max_all(a);
+    if (m > mine || (m == mine && i < where)) mine = m, where = i;
+  });
+  P p{STAGED ? reinterpret_cast<const Vec<T, V> *>(s_values) : memory, begin, size, lead, vectors, (W)0, s, cluster, 0};
   const Key own = Keys<W>::of(mine);
   Key top = block_max(own, s.sum), low = 0;
   const bool by_count = set.top_k < n, quick = by_count && set.top_k > 1 && set.top_k <= kQuickCount;
   if (quick) {
-    // A value that at least this block's share of the k units reach: the share's largest of the threads' maxima (to 2^-13 of it).
+    // A value that at least this block's share of the k units reach: the share's largest of the threads' maxima, in its first bits.
     const unsigned share = (set.top_k + blocks - 1) / blocks;
     constexpr int kLow = (int)sizeof(Key) * 8 - 32;
     const unsigned bits = (unsigned)(own >> kLow);
     unsigned reached = 0;
-    for (int b = 31; b >= 10; --b)
+    constexpr int kBits = sizeof(T) == 2 ? 16 : 20;   // (those of a 16-bit element)
+    for (int b = 31; b > 31 - kBits; --b)
       if (__syncthreads_count(bits >= (reached | 1u << b)) >= (int)share) reached |= 1u << b;
     low = (Key)reached << kLow;
   }
@@ -1065,20 +1090,34 @@ __global__ void __launch_bounds__(kThreads, 2)
   const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
   if (quick) {
     const W from_here = low > Keys<W>::of((W)-INFINITY) ? Keys<W>::value(low) : (W)-INFINITY;
-    p.each_from(from_here, [&](W v, unsigned i) { p.put(v, i, weights); });
+    p.each_from(from_here, [&](W v, unsigned i) { p.put(v, i); });
     cluster.sync();
     const unsigned count = cluster.map_shared_rank(&s, 0)->list;
     cluster.sync();
     if (count <= kList) {
-      if (rank == 0) p.draw(count, set, n, least, random[g], base, codes + g);
+      if (rank == 0) p.draw(count, set, n, 0, least, weights, random[g], base, codes + g);
       return;
     }
     if (rank == 0 && threadIdx.x == 0) s.list = 0;   // (values that lie unevenly over the threads, or many equal ones)
   }
+  if (set.top_k == 1) {   // the first of the largest; vectors that lie behind one another in a thread lie so in the group
+    u64 last = 0;
+    if (mine == best) {
+      unsigned unit = ~0u;
+      p.each(where, where + 1, 1, [&](W v, unsigned i) {
+        if (v == best) unit = min(unit, i);
+      });
+      last = ~unit;
+    }
+    last = block_max(last, s.sum);
+    u64 of_all = 0;
+    p.exchange(last, 0, [&](u64 a, u64) { of_all = max(of_all, a); });
+    if (rank == 0 && threadIdx.x == 0) codes[g] = base + (long long)(unsigned)~of_all;
+    cluster.sync();
+    return;
+  }
   Cut<Key> cut{0, n, 0};
-  if (set.top_k == 1) {
-    p.locate([&](W v, unsigned) { return (u64)(v == best); }, [](u64) { return (u64)0; });
-  } else {
+  {
     if (by_count || set.top_p < 1) {
       // bins of 1/128 in the weights' exponents; all units whose weight is below e^-16 share the last one
       const W scale = (W)(128 * set.inv_t);
@@ -1093,14 +1132,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (!by_count && found.above_count + found.in_bin <= kList) {
         // all that may be kept fits the list: the first block goes on by itself
         p.each([&](W v, unsigned i) {
-          if (bin(v) <= found.bin) p.put(v, i, weights);
+          if (bin(v) <= found.bin) p.put(v, i);
         });
         cluster.sync();
-        if (rank != 0) return;
-        const unsigned count = s.list;
-        if (threadIdx.x == 0) s.found[3] = total;
-        __syncthreads();
-        p.draw(count, set, n, least, random[g], base, codes + g);
+        if (rank == 0) p.draw(s.list, set, n, total, least, weights, random[g], base, codes + g);
         return;
       }
       cut = p.cut(want, found, bin, weights);
@@ -1146,9 +1181,9 @@ cudaError_t launch_warps(const T *support, const float *random, unsigned groups,
 template <typename T, bool STAGED>
 cudaError_t launch_blocks(const T *support, const float *random, unsigned groups, unsigned H, unsigned n, unsigned part, unsigned cluster,
                           const Sampling &s, long long *codes, cudaStream_t st) {
-  const size_t smem = STAGED ? (size_t)part * sizeof(T) + 32 : 0;   // (a vector in front and one behind)
+  const size_t smem = STAGED ? (size_t)part * sizeof(T) + 16 : 0;   // (a vector more where the part begins inside one)
   if (smem > 0) {   // (holds for the current device)
-    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage + 32);
+    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage + 16);
     if (e != cudaSuccess) return e;
   }
   return launch_clusters(sample_block_kernel<T, STAGED>, dim3(groups * cluster), dim3(cluster), kThreads, smem, st, support, random, H, n, part, s,
@@ -1173,16 +1208,20 @@ cudaError_t launch_sample(const T *support, const float *random, long rows, long
   } else if (n <= 512) {
     e = launch_warps<T, 16>(support, random, groups, h, n, s, codes, st);
   } else {
-    // the smallest cluster whose blocks hold their parts; a larger one where groups are too few for the SMs and parts long
+    // With a group for every SM, a block each, which reads its group again where it has to (it is in L2 by then).  Fewer: the smallest
+    // cluster whose blocks hold their parts in shared memory, and a larger one while there are SMs and parts are long.
     const size_t bytes = (size_t)n * sizeof(T);
     unsigned cluster = 1;
-    while (cluster < kMostBlocks && bytes > (size_t)cluster * kStage) cluster *= 2;
-    while (cluster < kMostBlocks && (size_t)groups * cluster * 2 <= (size_t)sm_count() && n / cluster > 2048) cluster *= 2;
+    const bool alone = groups >= (unsigned)sm_count();
+    if (!alone) {
+      while (cluster < kMostBlocks && bytes > (size_t)cluster * kStage) cluster *= 2;
+      while (cluster < kMostBlocks && (size_t)groups * cluster * 2 <= (size_t)sm_count() && n / cluster > 2048) cluster *= 2;
+    }
     constexpr unsigned V = 16 / (unsigned)sizeof(T);
     const unsigned part = ((n + cluster - 1) / cluster + V - 1) / V * V;
     if ((size_t)groups * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    e = (size_t)part * sizeof(T) <= kStage ? launch_blocks<T, true>(support, random, groups, h, n, part, cluster, s, codes, st)
-                                           : launch_blocks<T, false>(support, random, groups, h, n, part, cluster, s, codes, st);
+    e = !alone && (size_t)part * sizeof(T) <= kStage ? launch_blocks<T, true>(support, random, groups, h, n, part, cluster, s, codes, st)
+                                                     : launch_blocks<T, false>(support, random, groups, h, n, part, cluster, s, codes, st);
   }
   if (e == cudaSuccess) count_launches(1);
   return e;
