@@ -149,6 +149,11 @@ int sbb_layer_state_ptr(sbb_layer *layer, int which, void **device_ptr);
  * compute_activation: BCPNN/backend/_cpu_base_backend.py:44-51, 126-133. */
 int sbb_layer_forward(sbb_layer *layer, const void *x_dev, long B, void *y_dev, void *stream);
 
+/* The same for coded inputs (see the operators on unit codes below): codes_dev[B, codes_per_row] name the active
+ * inputs of each sample, int32 or int64 (code_bytes 4 or 8); with softmax == 0, y receives the support. */
+int sbb_layer_forward_codes(sbb_layer *layer, const void *codes_dev, int code_bytes, long B, long codes_per_row,
+                            int softmax, void *y_dev, void *stream);
+
 /* One train step from device buffers x[B,N] (layer input) and y[B,M] (layer
  * output, or the one-hot labels for the classifier).  `hypercolumn` >= 0 also
  * runs the mask update for that hypercolumn (plastic only); pass -1 for none.

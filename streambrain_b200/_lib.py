@@ -80,6 +80,7 @@ SIGNATURES = {
     "sbb_layer_get_state": (c_int, [c_void_p, c_int, c_void_p, c_size_t]),
     "sbb_layer_state_ptr": (c_int, [c_void_p, c_int, POINTER(c_void_p)]),
     "sbb_layer_forward": (c_int, [c_void_p, c_void_p, c_long, c_void_p, c_void_p]),
+    "sbb_layer_forward_codes": (c_int, [c_void_p, c_void_p, c_int, c_long, c_long, c_int, c_void_p, c_void_p]),
     "sbb_layer_train_step": (c_int, [c_void_p, c_void_p, c_void_p, c_long, c_long, c_void_p]),
     "sbb_layer_train_finalize": (c_int, [c_void_p, c_void_p]),
     "sbb_layer_forward_host": (c_int, [c_void_p, c_void_p, c_long, c_void_p]),

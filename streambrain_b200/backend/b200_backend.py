@@ -118,8 +118,11 @@ class _DeviceLayer:
 
     # -- reference API ---------------------------------------------------
     def compute_activation(self, inputs):
-        """softmax_minicolumns(inputs . weights + bias): _cpu_base_backend.py:44-51, 126-133."""
+        """softmax_minicolumns(inputs . weights + bias): _cpu_base_backend.py:44-51, 126-133.  An int32 or int64 CUDA
+        tensor [B, L] holds codes: the positions of each sample's active inputs (:mod:`streambrain_b200.kernels_device`)."""
         if _is_tensor(inputs):
+            if inputs.dtype in (torch.int32, torch.int64):
+                return self._forward_codes(inputs, 1)
             x = self._dev_input(inputs, self.in_features)
             B = x.shape[0]
             y = x.new_empty((B, self.out_features))
@@ -134,6 +137,25 @@ class _DeviceLayer:
         y = np.empty((B, self.out_features), dtype=self.dtype)
         check(lib.sbb_layer_forward_host(self._handle, host_ptr(x), B, host_ptr(y)))
         return y
+
+    def _forward_codes(self, codes, softmax):
+        if not codes.is_cuda:
+            raise TypeError("torch inputs must be CUDA tensors (pass numpy arrays for host data)")
+        if codes.dim() != 2:
+            raise TypeError("expected a [B, L] tensor of codes")
+        c = codes if codes.is_contiguous() else codes.contiguous()
+        y = torch.empty((c.shape[0], self.out_features), dtype=self._tdtype, device=c.device)
+        check(lib.sbb_layer_forward_codes(self._handle, c.data_ptr(), c.element_size(), c.shape[0], c.shape[1], softmax,
+                                          y.data_ptr(), _stream_ptr()))
+        return y
+
+    def sample_units(self, codes, random, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """The codes [B, hypercolumns] of one unit per hypercolumn, drawn from the softmax of the support that coded inputs
+        (as in :meth:`compute_activation`) give; ``random`` and the settings as in
+        :func:`streambrain_b200.kernels_device.sample_minicolumns`.  They are the next layer's coded inputs."""
+        from ..kernels_device import sample_minicolumns
+        return sample_minicolumns(self._forward_codes(codes, 0), self.hypercolumns, self.minicolumns, random, temperature,
+                                  top_k, top_p, min_p)
 
     def _dev_input(self, t, cols):
         if not t.is_cuda:

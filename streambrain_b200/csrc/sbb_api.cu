@@ -1060,6 +1060,23 @@ int sbb_layer_forward(sbb_layer *L, const void *x_dev, long B, void *y_dev, void
                   layer_forward<double>(L, (const double *)x_dev, B, (double *)y_dev, st));
 }
 
+int sbb_layer_forward_codes(sbb_layer *L, const void *codes_dev, int code_bytes, long B, long codes_per_row, int softmax, void *y_dev,
+                            void *stream) {
+  SBB_TRY(check_layer(L));
+  ARG(y_dev != nullptr, "layer_forward_codes: null pointer");
+  SBB_TRY(check_batch(L, B));
+  // (its checks are the lookup's: codes, their number and width)
+  SBB_TRY(sbb_lookup(L->desc.dtype, L->state[SBB_STATE_WEIGHTS], codes_dev, code_bytes, B, codes_per_row, L->N, L->M, 1.0, y_dev, stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (L->desc.dtype == SBB_F32)
+    SBB_CUDA(sbb::launch_reduce_bias_softmax<float>((float *)y_dev, 1, (const float *)L->state[SBB_STATE_BIAS], (float *)y_dev, B, L->H, L->Mc,
+                                                    softmax != 0, st));
+  else
+    SBB_CUDA(sbb::launch_reduce_bias_softmax<double>((double *)y_dev, 1, (const double *)L->state[SBB_STATE_BIAS], (double *)y_dev, B, L->H, L->Mc,
+                                                     softmax != 0, st));
+  return SBB_OK;
+}
+
 int sbb_layer_train_step(sbb_layer *L, const void *x_dev, const void *y_dev, long B, long hypercolumn, void *stream) {
   SBB_TRY(check_layer(L));
   ARG(x_dev && y_dev, "layer_train_step: null pointer");

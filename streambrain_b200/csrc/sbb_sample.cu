@@ -674,23 +674,28 @@ struct Part {
     for (int v = 0; v < V; ++v) a.v[v] = i * V + v >= lead && i * V + v < lead + size ? element[i * V + v] : narrow_to<T>((W)-INFINITY);
     return a;
   }
-  // f(vector, its number) for every vector, a thread's in rising order but for the first and the last one where they are not whole
-  // (threads 0 and 32); U in flight, their loads without conditions among them.
+  // f(vector, its number) for vectors lo, lo + step, ... below hi, in rising order; U in flight, their loads without conditions among
+  // them.  A first and a last vector that are not whole are put together by themselves.
   template <int U, typename F>
-  __device__ __forceinline__ void vectors_of_thread(F f) const {
-    const unsigned end = end_whole();
-    for (unsigned i = first_whole() + threadIdx.x; i < end; i += U * kThreads) {
+  __device__ __forceinline__ void range(unsigned lo, unsigned hi, unsigned step, F f) const {
+    unsigned i = lo;
+    if (!STAGED && i < first_whole() && i < hi) {
+      f(load(i), i);
+      i += step;
+    }
+    const unsigned end = min(hi, end_whole());
+    for (; i < end; i += U * step) {
       Vec<T, V> a[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < end) a[u] = x[i + u * kThreads];
+        if (i + u * step < end) a[u] = x[i + u * step];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (i + u * kThreads < end) f(a[u], i + u * kThreads);
+        if (i + u * step < end) f(a[u], i + u * step);
     }
     if constexpr (!STAGED) {
-      if (threadIdx.x == 0 && vectors > 0 && lead > 0) f(load(0), 0);
-      if (threadIdx.x == 32 && vectors > first_whole() && end < vectors) f(load(vectors - 1), vectors - 1);
+      const unsigned last = end_whole();
+      if (last < hi && last >= first_whole() && last >= lo && (last - lo) % step == 0) f(load(last), last);
     }
   }
   // f(value, unit) for the units above -infinity (no NaN is) of a vector
@@ -702,26 +707,58 @@ struct Part {
     for (int v = 0; v < V; ++v)
       if (w[v] > (W)-INFINITY) f(w[v], begin + i * V + v - lead);
   }
-  // ... of vectors [lo, hi), `step` apart; of all
-  template <typename F>
-  __device__ __forceinline__ void each(unsigned lo, unsigned hi, unsigned step, F f) const {
-    for (unsigned i = lo; i < hi; i += step) units(load(i), i, f);
-  }
+  // ... of all vectors
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    vectors_of_thread<STAGED ? 1 : 2>([&](const Vec<T, V> &a, unsigned i) { units(a, i, f); });
+    range<1>(threadIdx.x, vectors, kThreads, [&](const Vec<T, V> &a, unsigned i) { units(a, i, f); });
   }
-  // The same for units of at least `low`, where they are few.
+  // The same for units of at least `low`, which most vectors have none of: marked in a word first, so that there is one copy of f's
+  // code (32 of them, for the vectors in flight, did not stay in the instruction cache: 39 us a pass over 128000 units, 12 so).
+  template <typename F>
+  __device__ __forceinline__ void range_from(W low, unsigned lo, unsigned hi, unsigned step, F f) const {
+    constexpr int U = 32 / V < 4 ? 32 / V : 4;
+    const T *const element = reinterpret_cast<const T *>(x);
+    auto marks = [&](const Vec<T, V> &a) {
+      unsigned m = 0;
+      if (max_all(a) >= low)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const W w = widen(a.v[v]);
+          m |= (w >= low && w > (W)-INFINITY ? 1u : 0u) << v;
+        }
+      return m;
+    };
+    auto run = [&](unsigned m, unsigned i) {
+      for (; m != 0; m &= m - 1) {
+        const unsigned bit = __ffs(m) - 1, at = (i + bit / V * step) * V + bit % V;
+        f((W)widen(element[at]), begin + at - lead);
+      }
+    };
+    const unsigned first = first_whole(), end = min(hi, end_whole()), last = end_whole();
+    unsigned i = lo, edge = 0, at = 0;
+    if (!STAGED && i < first && i < hi) {
+      edge = marks(load(i)), at = i;
+      i += step;
+    } else if (!STAGED && last < hi && last >= first && last >= lo && (last - lo) % step == 0) {
+      edge = marks(load(last)), at = last;
+    }
+    if constexpr (!STAGED) run(edge, at);
+    if (!STAGED && lo < first && lo < hi && last < hi && last >= first && (last - lo) % step == 0) run(marks(load(last)), last);   // (both ends)
+    for (; i < end; i += U * step) {
+      Vec<T, V> a[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * step < end) a[u] = x[i + u * step];
+      unsigned m = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * step < end) m |= marks(a[u]) << (u * V);
+      run(m, i);
+    }
+  }
   template <typename F>
   __device__ __forceinline__ void each_from(W low, F f) const {
-    vectors_of_thread<STAGED ? 1 : 4>([&](const Vec<T, V> &a, unsigned i) {
-      if (!(max_all(a) >= low)) return;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const W w = widen(a.v[v]);
-        if (w >= low && w > (W)-INFINITY) f(w, begin + i * V + v - lead);
-      }
-    });
+    range_from(low, threadIdx.x, vectors, kThreads, f);
   }
 
   // f(a, b) of every block's two values, in the blocks' order.
@@ -748,14 +785,18 @@ struct Part {
 
   // The first unit at which the running sum of weigh(value, unit) passes target(sum of all), which is below that sum; known to every
   // block when all have passed a barrier of the cluster.
+  // Units below `low` weigh nothing.
   template <typename F, typename G>
-  __device__ void locate(F weigh, G target) {
+  __device__ void locate(W low, F weigh, G target) {
     const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned lo = 0, hi = vectors;
     auto by_warp = [&](u64 &all) {   // sums of the warps' shares of vectors [lo, hi)
       const unsigned share = (hi - lo + kBlockWarps - 1) / kBlockWarps, from = min(hi, lo + warp * share);
       u64 mine = 0;
-      each(from + lane, min(hi, from + share), 32, [&](W v, unsigned i) { mine += weigh(v, i); });
+      if (low > (W)-INFINITY)
+        range_from(low, from + lane, min(hi, from + share), 32, [&](W v, unsigned i) { mine += weigh(v, i); });
+      else
+        range<1>(from + lane, min(hi, from + share), 32, [&](const Vec<T, V> &a, unsigned i) { units(a, i, [&](W v, unsigned j) { mine += weigh(v, j); }); });
       mine = warp_sum(mine);
       __syncthreads();
       if (lane == 0) s.sum[warp] = mine;
@@ -785,11 +826,11 @@ struct Part {
     }
     u64 mine = 0;
     const unsigned i = lo + threadIdx.x;
-    each(i, min(hi, i + 1), 1, [&](W v, unsigned j) { mine += weigh(v, j); });
+    if (i < hi) units(load(i), i, [&](W v, unsigned j) { mine += weigh(v, j); });
     u64 run = before + block_before(mine, s.sum);
     if (run <= at && at < run + mine) {
       bool found = false;
-      each(i, i + 1, 1, [&](W v, unsigned j) {
+      units(load(i), i, [&](W v, unsigned j) {
         run += weigh(v, j);
         if (!found && run > at) {
           found = true;
@@ -886,7 +927,8 @@ struct Part {
     Block *const first = cluster.num_blocks() == 1 ? &s : cluster.map_shared_rank(&s, 0);
     const unsigned at = atomicAdd(&first->list, 1u);
     if (at >= kList) return;
-    reinterpret_cast<Key *>(first->list_key)[at] = Keys<W>::of(v);
+    // (of 32-bit keys, one number in the order of the units)
+    first->list_key[at] = sizeof(Key) == 4 ? (u64)Keys<W>::of(v) << 32 | ~unit : (u64)Keys<W>::of(v);
     first->list_index[at] = unit;
   }
   // How many of the first `count` numbers of a list are above (below) one's own: four a step.
@@ -918,14 +960,14 @@ struct Part {
     Ranked r{};
     r.rank = kList;
     if (threadIdx.x < count) {
-      const Key *const keys = reinterpret_cast<const Key *>(s.list_key);
-      r.key = keys[threadIdx.x];
+      const u64 own = s.list_key[threadIdx.x];
+      r.key = (Key)(sizeof(Key) == 4 ? own >> 32 : own);
       r.index = s.list_index[threadIdx.x];
       r.mass = weights.of(Keys<W>::value(r.key), best);
       unsigned equal;
-      r.rank = count_of<true>(keys, count, r.key, equal);
-      if (equal > 1)
-        for (unsigned j = 0; j < count; ++j) r.rank += keys[j] == r.key && s.list_index[j] < r.index;
+      r.rank = count_of<true>(s.list_key, count, own, equal);
+      if (equal > 1)   // (of 64-bit keys alone)
+        for (unsigned j = 0; j < count; ++j) r.rank += s.list_key[j] == own && s.list_index[j] < r.index;
       s.sorted_mass[r.rank] = r.mass;
     }
     r.before = sum_in_front(count, r.rank);
@@ -960,6 +1002,134 @@ struct Part {
     }
     const u64 before = sum_in_front(count, at);
     if (mass > 0 && before <= target && target < before + mass) *code = base + r.index;
+  }
+
+  // The cut of a top-p by sums in 32 bits with a bound on what they can be off, or false: exact sums have to decide.  Only the units
+  // above the cut have their weights formed in 64 bits; in the exact form, which adds masses to bins, all have.
+  // A weight e^-x is off by 2^-22 of it and 3 x 2^-24 for every unit of x; over n weights of sum S the mean of x, by weight, is at
+  // most ln n (where all are equal); a sum of eight is off by 7 x 2^-24 more.  So S is off by S (1.8e-7 ln n + 7e-7) at most.
+  template <typename F>
+  __device__ bool cut_quickly(F bin_of, const Settings &set, unsigned n, const Weights &weights, Cut<Key> &cut) {
+    constexpr double kOne = 1099511627776.0;   // 2^40: 32-bit weights are summed in fixed point, up to 2^22 of them
+    const float c = (float)(set.inv_t * 1.4426950408889634);
+    if (best == INFINITY || !(c < 1e30f) || !(set.top_p > 0) || n > 1u << 22) return false;
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBins; b += kThreads) s.bin_count[b] = 0;
+    __syncthreads();
+    double sum = 0;
+    range<STAGED ? 1 : 4>(threadIdx.x, vectors, kThreads, [&](const Vec<T, V> &a, unsigned) {
+      float w[V], eight = 0;
+      widen_all(a, w);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        w[v] = fmaxf(w[v], -3.4e38f);   // (-infinity or a NaN: weighs nothing)
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((w[v] - (float)best) * c));
+        eight += e;
+      }
+      sum += eight;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int b = bin_of(w[v]);
+        if (b < kBins - 1) atomicAdd(&s.bin_count[b], 1u);
+      }
+    });
+    const u64 total = cluster_sum(block_sum(__double2ull_rn(sum * kOne), s.sum));   // (with the barriers that the bins need)
+    const double error = (double)total * (1.9e-7 * log((double)n) + 8e-7) * (1 + set.top_p) + 1024;
+    const double limit = set.top_p * (double)total;
+    if (cluster.block_rank() == 0) {
+      if (threadIdx.x == 0) s.found[0] = kBins, s.found[1] = kBins;
+      unsigned count[kBinsEach];
+      double low = 0, high = 0;   // bounds on the bins' masses: a unit of bin b weighs e^-(b +- 1/2)/128, and e^1/256 is 1.0039
+#pragma unroll
+      for (int j = 0; j < kBinsEach; ++j) {
+        const int b = threadIdx.x * kBinsEach + j;
+        count[j] = s.bin_count[b];
+        for (unsigned o = 1; o < cluster.num_blocks(); ++o) count[j] += cluster.map_shared_rank(&s, o)->bin_count[b];
+        s.bin_count[b] = count[j];
+        const double w = kOne * count[j] * (double)__expf(-b * (1.f / 128));
+        high += w * 1.0041;
+        low += w * 0.9959;
+      }
+      double high_up_to = (double)block_before((u64)high, s.sum), low_up_to = (double)block_before((u64)low, s.sum);
+      __syncthreads();   // s.found is there
+#pragma unroll
+      for (int j = 0; j < kBinsEach; ++j) {
+        const int b = threadIdx.x * kBinsEach + j;
+        const double w = kOne * count[j] * (double)__expf(-b * (1.f / 128));
+        high_up_to += w * 1.0041 + 1;
+        low_up_to += w * 0.9959;
+        if (high_up_to + kThreads >= limit - error) atomicMin(&s.found[0], (u64)b);
+        if (low_up_to >= limit + error) atomicMin(&s.found[1], (u64)b);
+      }
+      __syncthreads();
+      const int first = (int)s.found[0], last = (int)s.found[1];
+      unsigned in = 0, above = 0;
+#pragma unroll
+      for (int j = 0; j < kBinsEach; ++j) {
+        const int b = threadIdx.x * kBinsEach + j;
+        if (b < first) above += count[j];
+        if (b >= first && b <= last) in += count[j];
+      }
+      const u64 both = block_sum((u64)above << 32 | in, s.sum);
+      if (threadIdx.x == 0)
+        for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
+          u64 *const to = cluster.map_shared_rank(&s, o)->found;
+          to[0] = first;
+          to[1] = last >= kBins - 1 ? kList + 1 : (unsigned)both;
+          to[2] = last;
+          to[3] = both >> 32;
+        }
+    }
+    cluster.sync();
+    const int first = (int)s.found[0], last = (int)s.found[2];
+    const unsigned in = (unsigned)s.found[1], above_count = (unsigned)s.found[3];
+    if (in > kList) return false;
+    u64 above = 0;
+    const W low = best - (W)((last + 2) / (128 * set.inv_t));   // no unit of the bins lies below
+    each_from(low, [&](W v, unsigned i) {
+      const int b = bin_of(v);
+      if (b > last) return;
+      if (b < first)
+        above += weights.of(v, best);
+      else
+        put(v, i);
+    });
+    above = cluster_sum(block_sum(above, s.sum));   // (one block: its barriers are between the list's entries and their reader)
+    Ranked r{};
+    if (cluster.block_rank() == 0) {
+      r = rank(in, weights);
+      if (threadIdx.x == 0) s.list = 0;
+    }
+    // Decided by the sum in 32 bits, and again by the exact one where a unit lies within the bound of the limit (a few rows of a
+    // hundred).
+    const double scale = (double)weights.one() / kOne;   // the masses' unit
+    Want want{false, 0, (u64)(limit * scale)};
+    double off = error * scale;
+    for (;;) {
+      if (cluster.block_rank() == 0) {
+        const u64 before = above + r.before;
+        const bool here = threadIdx.x < in, keep = here && want.inside(above_count + r.rank, before);
+        const bool doubt = here && above_count + r.rank > 0 && fabs((double)before - (double)want.limit) <= off;
+        const u64 n_kept = block_sum(keep, s.sum);
+        const bool again = __syncthreads_or(doubt) || n_kept == 0;
+        if (again ? threadIdx.x == 0 : keep && r.rank + 1 == n_kept)
+          for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
+            u64 *const to = cluster.map_shared_rank(&s, o)->found;
+            to[0] = again ? 0 : (u64)r.key;
+            to[1] = r.index;
+          }
+      }
+      cluster.sync();
+      if (s.found[0] != 0) break;   // (no unit's key)
+      if (off < 0) return false;
+      u64 exact = 0;
+      each([&](W v, unsigned) { exact += weights.of(v, best); });
+      want = want_mass(set.top_p, cluster_sum(block_sum(exact, s.sum)));
+      off = -1;
+    }
+    cut = Cut<Key>{(Key)s.found[0], (unsigned)s.found[1], 0};
+    return true;
   }
 
   // The cut that `want` asks for among all units: bins of equal width in the value's distance from the largest first (`found`, by
@@ -1003,7 +1173,7 @@ struct Part {
       const u64 m = weights.of(Keys<W>::value(hi), best);
       const unsigned take = equal_ones(want, in, m, above_count, above_mass);
       const Key key = hi;
-      locate([&](W v, unsigned) { return (u64)(Keys<W>::of(v) == key); }, [&](u64) { return (u64)(take - 1); });
+      locate(Keys<W>::value(key), [&](W v, unsigned) { return (u64)(Keys<W>::of(v) == key); }, [&](u64) { return (u64)(take - 1); });
       cluster.sync();
       return Cut<Key>{key, (unsigned)s.unit, above_mass + take * m};
     }
@@ -1054,10 +1224,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const Vec<T, V> *const memory = reinterpret_cast<const Vec<T, V> *>(from - lead);
   W mine = -INFINITY;   // the largest of the values that pass through this thread, and the first vector that has it
   unsigned where = 0;
-  Part<T, false>{memory, begin, size, lead, vectors, (W)0, s, cluster, 0}.template vectors_of_thread<STAGED ? 4 : 8>([&](const Vec<T, V> &a, unsigned i) {
+  Part<T, false>{memory, begin, size, lead, vectors, (W)0, s, cluster, 0}.template range<STAGED ? 4 : 8>(threadIdx.x, vectors, kThreads, [&](const Vec<T, V> &a, unsigned i) {
     if constexpr (STAGED) reinterpret_cast<Vec<T, V> *>(s_values)[i] = a;
     const W m = max_all(a);
-    if (m > mine || (m == mine && i < where)) mine = m, where = i;
+    if (m > mine) mine = m, where = i;
   });
   P p{STAGED ? reinterpret_cast<const Vec<T, V> *>(s_values) : memory, begin, size, lead, vectors, (W)0, s, cluster, 0};
   const Key own = Keys<W>::of(mine);
@@ -1104,7 +1274,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     u64 last = 0;
     if (mine == best) {
       unsigned unit = ~0u;
-      p.each(where, where + 1, 1, [&](W v, unsigned i) {
+      p.units(p.load(where), where, [&](W v, unsigned i) {
         if (v == best) unit = min(unit, i);
       });
       last = ~unit;
@@ -1119,39 +1289,45 @@ __global__ void __launch_bounds__(kThreads, 2)
   Cut<Key> cut{0, n, 0};
   {
     if (by_count || set.top_p < 1) {
-      // bins of 1/128 in the weights' exponents; all units whose weight is below e^-16 share the last one
+      // bins of 1/128 in the weights' exponents, to the nearest; all units whose weight is below e^-16 share the last one
       const W scale = (W)(128 * set.inv_t);
       auto bin = [&](W v) -> int {
-        const W d = (best - v) * scale;
-        return v == best ? 0 : d < (W)(kBins - 1) ? (int)d : kBins - 1;
+        const W d = v == best ? (W)0 : fmin((best - v) * scale, (W)(kBins - 1));
+        return sizeof(W) == 4 ? (int)(__float_as_uint((float)d + 8388608.f) & (kBins - 1)) : (int)rint(d);   // (2^23: rounds to an integer)
       };
-      u64 total = p.histogram(bin, !by_count, !by_count, weights);
-      if (!by_count) total = p.cluster_sum(block_sum(total, s.sum));
-      Want want = by_count ? want_count(set.top_k) : want_mass(set.top_p, total);
-      const auto found = p.find(want, 0, 0);
-      if (!by_count && found.above_count + found.in_bin <= kList) {
-        // all that may be kept fits the list: the first block goes on by itself
-        p.each([&](W v, unsigned i) {
-          if (bin(v) <= found.bin) p.put(v, i);
-        });
-        cluster.sync();
-        if (rank == 0) p.draw(s.list, set, n, total, least, weights, random[g], base, codes + g);
-        return;
-      }
-      cut = p.cut(want, found, bin, weights);
-      if (by_count && set.top_p < 1) {
-        u64 sum = 0;
-        p.each([&](W v, unsigned i) {
-          if (kept(Keys<W>::of(v), i, cut)) sum += weights.of(v, best);
-        });
-        want = want_mass(set.top_p, p.cluster_sum(block_sum(sum, s.sum)));
-        p.histogram(bin, true, false, weights);
-        cut = p.cut(want, p.find(want, 0, 0), bin, weights);
+      bool quick_p = false;
+      if constexpr (sizeof(W) == 4) quick_p = !by_count && p.cut_quickly(bin, set, n, weights, cut);
+      if (!quick_p) {
+        u64 total = p.histogram(bin, !by_count, !by_count, weights);
+        if (!by_count) total = p.cluster_sum(block_sum(total, s.sum));
+        Want want = by_count ? want_count(set.top_k) : want_mass(set.top_p, total);
+        const auto found = p.find(want, 0, 0);
+        if (!by_count && found.above_count + found.in_bin <= kList) {
+          // all that may be kept fits the list: the first block goes on by itself
+          p.each([&](W v, unsigned i) {
+            if (bin(v) <= found.bin) p.put(v, i);
+          });
+          cluster.sync();
+          if (rank == 0) p.draw(s.list, set, n, total, least, weights, random[g], base, codes + g);
+          return;
+        }
+        cut = p.cut(want, found, bin, weights);
+        if (by_count && set.top_p < 1) {
+          u64 sum = 0;
+          p.each([&](W v, unsigned i) {
+            if (kept(Keys<W>::of(v), i, cut)) sum += weights.of(v, best);
+          });
+          want = want_mass(set.top_p, p.cluster_sum(block_sum(sum, s.sum)));
+          p.histogram(bin, true, false, weights);
+          cut = p.cut(want, p.find(want, 0, 0), bin, weights);
+        }
       }
     }
+    const W value = cut.key ? Keys<W>::value(cut.key) : (W)-INFINITY;
     p.locate(
+        value,
         [&](W v, unsigned i) -> u64 {
-          if (!kept(Keys<W>::of(v), i, cut)) return 0;
+          if (!(v > value || (v == value && i <= cut.index))) return 0;
           const u64 m = weights.of(v, best);
           return m >= least ? m : 0;
         },
@@ -1213,6 +1389,9 @@ cudaError_t launch_sample(const T *support, const float *random, long rows, long
     const size_t bytes = (size_t)n * sizeof(T);
     unsigned cluster = 1;
     const bool alone = groups >= (unsigned)sm_count();
+    // Where every row has its own top-k, some may have none and take several times as long: two blocks share a row if all fit side by
+    // side.  256 x 128000 bf16, us a call: 157 with one, 112 with two; with one top-k of 100 for all 33 and 46.
+    if (alone && s.top_k_rows && groups < 2 * (unsigned)sm_count()) cluster = 2;
     if (!alone) {
       while (cluster < kMostBlocks && bytes > (size_t)cluster * kStage) cluster *= 2;
       while (cluster < kMostBlocks && (size_t)groups * cluster * 2 <= (size_t)sm_count() && n / cluster > 2048) cluster *= 2;

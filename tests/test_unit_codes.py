@@ -603,6 +603,43 @@ def test_operators_copy_what_is_not_contiguous():
     assert all(torch.equal(a, b) for a, b in zip(chain(*strided, h, mc, n), want))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("n,h,mc", [(40, 5, 12), (300, 3, 100), (64, 1, 10)])
+def test_layers_take_codes(n, h, mc, dtype):
+    """A layer's activation from codes and from the dense row they stand for; the units drawn are the sampler's of its support,
+    and feed the next layer.  Both sum n products: 2 (n + 8) roundings of the magnitudes they add, through a softmax, whose
+    derivative is at most a half, and whose own roundings are a dozen."""
+    from streambrain_b200.backend.b200_backend import DenseLayer, StructuralPlasticityLayer
+    np.random.seed(1)
+    hidden = StructuralPlasticityLayer(n, h, mc, 0.01, -100.0, 0.05, 0.02, 0.5, 16, (1, 1 / mc, 1 / mc), dtype=dtype)
+    out = DenseLayer(h * mc, 1, 10, 0.01, (0.1, 0.1, 0.01), dtype=dtype)
+    rng = np.random.default_rng(2)
+    x = (rng.random((33, n)) < 0.3).astype(dtype)
+    length = int(x.sum(1).max())
+    codes = np.full((33, length), -1, dtype=np.int64)
+    for r in range(33):
+        codes[r, :int(x[r].sum())] = np.flatnonzero(x[r])
+    t = F32 if dtype is np.float32 else F64
+    u = half_step(t)
+    c = torch.from_numpy(codes).cuda()
+    want = hidden.compute_activation(torch.from_numpy(x).cuda())
+    size = float((x @ np.abs(hidden.weights)).max()) + float(np.abs(hidden.bias).max())
+    bound = (2 * (n + 8) * size + 24) * u
+    for index in (torch.int64, torch.int32):
+        got = hidden.compute_activation(c.to(index))
+        assert got.dtype == t and float((got - want).abs().max()) <= bound
+    random = torch.from_numpy(rng.random((33, h)).astype(np.float32)).cuda()
+    units = hidden.sample_units(c, random, temperature=0.8, top_p=0.9)
+    support = k().lookup(hidden.state_tensor("weights"), c) + hidden.state_tensor("bias")
+    assert torch.equal(units, k().sample_minicolumns(support, h, mc, random, temperature=0.8, top_p=0.9))
+    assert out.compute_activation(units).shape == (33, 10)
+    with pytest.raises(TypeError):
+        hidden.compute_activation(torch.from_numpy(codes))
+    with pytest.raises(TypeError):
+        hidden.compute_activation(c[0])
+
+
 # ---- refusals (no device needed) -------------------------------------------
 
 def test_wrappers_refuse_host_tensors_and_wrong_types():
