@@ -16,6 +16,7 @@ Nothing here records for autograd: the gradients are calls of their own.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -76,6 +77,11 @@ def lookup(weights, codes, scale=1.0):
     return out
 
 
+@lru_cache(maxsize=256)
+def _gradient_workspace(code, rows, length, n, m):
+    return lib.sbb_lookup_gradient_workspace(code, rows, length, n, m)
+
+
 def lookup_gradient(grad, codes, in_features, scale=1.0, out=None, accumulate=False):
     """The gradient of :func:`lookup` with respect to its weights: ``out[i] = scale *`` the sum of ``grad[r]`` over the
     ``(r, l)`` with ``codes[r, l] == i``; ``grad`` [rows, M], result [in_features, M] of its dtype, rows that no code names
@@ -100,7 +106,7 @@ def lookup_gradient(grad, codes, in_features, scale=1.0, out=None, accumulate=Fa
         if out.shape != (n, m):
             raise ValueError("out must have shape %s, got %s" % ((n, m), tuple(out.shape)))
     code = _DTYPES[grad.dtype]
-    size = lib.sbb_lookup_gradient_workspace(code, rows, length, n, m)
+    size = _gradient_workspace(code, rows, length, n, m)
     work = grad.new_empty(size, dtype=torch.uint8) if size else None
     _call(lib.sbb_lookup_gradient, device, code, grad.data_ptr(), codes.data_ptr(), _INDEX_BYTES[codes.dtype], rows, length, n, m,
           scale, 1 if accumulate else 0, out.data_ptr(), None if work is None else work.data_ptr(), size)
