@@ -526,7 +526,7 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
     const float least = fminf((float)set.min_p, 1.f);
 #pragma unroll
     for (int r = 0; r < EACH; ++r) {
-      g.doubt = g.doubt || (fabsf(g.w[r] - least) <= 6e-6f * least && g.v[r] != best);
+      g.doubt = g.doubt || (fabsf(g.w[r] - least) <= 1e-5f * least && g.v[r] != best);
       if (g.w[r] < least && g.v[r] != best) g.w[r] = 0;
     }
   }
