@@ -48,6 +48,65 @@ __device__ __forceinline__ float expo(float d, float c) {
 }
 __device__ __forceinline__ double expo(double d, double c) { return exp(d * c); }
 
+// The same for all of f: exp((f - best) / t), their sum, and a product with one factor; floats two at a time where there are two (the
+// exponentials' own pipe is busy half of the time, the rest is the issue of what stands around them).
+struct Two {
+  unsigned long long v;
+  __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void add(const Two &o) { asm("add.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(o.v)); }
+  __device__ __forceinline__ void mul(const Two &o) { asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(o.v)); }
+  __device__ __forceinline__ void get(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+template <typename W, int V>
+__device__ __forceinline__ void expo_all(W (&f)[V], W best, W c) {
+  if constexpr (sizeof(W) == 4 && V % 2 == 0) {
+    const Two minus(-best, -best), factor(c, c);
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      Two d(f[v], f[v + 1]);
+      d.add(minus);
+      d.mul(factor);
+      d.get(f[v], f[v + 1]);
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f[v]));
+      asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f[v + 1]));
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] = expo(f[v] - best, c);
+  }
+}
+template <typename W, int V>
+__device__ __forceinline__ W sum_all(const W (&f)[V]) {
+  if constexpr (sizeof(W) == 4 && V % 2 == 0) {
+    Two s(f[0], f[1]);
+#pragma unroll
+    for (int v = 2; v < V; v += 2) s.add(Two(f[v], f[v + 1]));
+    float a, b;
+    s.get(a, b);
+    return a + b;
+  } else {
+    W s = f[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) s += f[v];
+    return s;
+  }
+}
+template <typename W, int V>
+__device__ __forceinline__ void scale_all(W (&f)[V], W by) {
+  if constexpr (sizeof(W) == 4 && V % 2 == 0) {
+    const Two factor(by, by);
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      Two p(f[v], f[v + 1]);
+      p.mul(factor);
+      p.get(f[v], f[v + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) f[v] *= by;
+  }
+}
+
 template <typename W>
 __device__ __forceinline__ W warp_sum(W v) {
   for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
@@ -148,12 +207,10 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
       __syncwarp();
     }
 #pragma unroll
-    for (int r = 0; r < NV; ++r)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        e[r][v] = expo(e[r][v] - best, p.c);
-        total += e[r][v];
-      }
+    for (int r = 0; r < NV; ++r) {
+      expo_all(e[r], best, p.c);
+      total += sum_all(e[r]);
+    }
     const W inv = (W)1 / p.temperature;
     // the teacher's side without its divisor, so that three sums run side by side
     auto entry = [&](bool there, W t, W xu) {
@@ -210,10 +267,10 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
     for (int r = 0; r < NV; ++r)
       if ((r * 32 + lane) * V < p.n) {
         const Vec<W, V> k = s_kept[warp][r * 32 + lane];
-        Vec<T, V> o;
+        scale_all(e[r], scale);
 #pragma unroll
-        for (int v = 0; v < V; ++v) o.v[v] = narrow_to<T>(e[r][v] * scale - wt * k.v[v]);
-        *reinterpret_cast<Vec<T, V> *>(out + (r * 32 + lane) * V) = o;
+        for (int v = 0; v < V; ++v) e[r][v] -= wt * k.v[v];
+        *reinterpret_cast<Vec<T, V> *>(out + (r * 32 + lane) * V) = narrow_all<T, V>(e[r]);
       }
     __syncwarp();
   }
@@ -312,8 +369,8 @@ __global__ void __launch_bounds__(kThreads, 3) distill_block_kernel(const Distil
         const W b = r.best == -INFINITY ? (W)0 : r.best;
         W f[V];
         widen_all(a[u], f);
-#pragma unroll
-        for (int v = 0; v < V; ++v) r.sum += expo(f[v] - b, p.c);
+        expo_all(f, b, p.c);
+        r.sum += sum_all(f);
       }
     }
     if (single < size) r.add(own, p.c);
@@ -405,8 +462,8 @@ __global__ void __launch_bounds__(kThreads, 3) distill_block_kernel(const Distil
   for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
     W f[V];
     widen_all(STAGED ? stage[i] : from[i], f);
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = expo(f[v] - r.best, p.c) * scale;
+    expo_all(f, r.best, p.c);
+    scale_all(f, scale);
     reinterpret_cast<Vec<T, V> *>(out + lead)[i] = narrow_all<T, V>(f);
   }
   if (single < size) out[single] = narrow_to<T>(expo(own - r.best, p.c) * scale);
