@@ -461,8 +461,8 @@ int sbb_read_raw_u8_labels(const char *path, int dtype, void *out, long samples,
  * synchronise nor keep anything between calls: they may be captured into a graph, and run at once on several
  * streams (with a workspace each).  Element types: SBB_F32, SBB_F64 and, for these calls only, SBB_F16 and
  * SBB_BF16; sums are held in 32 bits (64 for SBB_F64) and rounded once.  `code_bytes`: 4 (int32) or 8 (int64).
- * Codes outside [0, N) -- -1 by convention -- name nothing.  Every call gives the same bits for the same
- * inputs.  No counterpart in the reference, whose layers take dense rows only.
+ * Codes outside [0, N) -- -1 by convention -- name nothing.  Results must not overlap inputs.  Every call gives the
+ * same bits for the same inputs.  No counterpart in the reference, whose layers take dense rows only.
  * ---------------------------------------------------------------------- */
 #define SBB_F16 2
 #define SBB_BF16 3
@@ -505,7 +505,7 @@ int sbb_sample_minicolumns(int dtype, const void *support_dev, const float *rand
  * the derivative of the loss with respect to support[rows, H * Mc].  teacher_units[rows, H, K] counts from 0 within
  * the hypercolumn (unit_bytes: 4 or 8); entries outside [0, Mc) are absent, a unit named twice has both parts.
  * teacher[rows, H, K] is of the support's type; loss and weight (null: 1) are float, double for SBB_F64.
- * gradient may be null: the loss alone; it must not overlap an input.  Where the weight is 0, where no unit is kept,
+ * temperature: from 1e-15 to 1e15.  gradient may be null: the loss alone.  Where the weight is 0, where no unit is kept,
  * or where a hypercolumn's support (or the teacher's) is -infinity throughout, both are exactly 0. */
 int sbb_distill(int dtype, const void *support_dev, const void *teacher_units_dev, int unit_bytes,
                 const void *teacher_dev, const void *weight_dev, long rows, long H, long Mc, long K,

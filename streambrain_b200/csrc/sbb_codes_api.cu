@@ -163,7 +163,7 @@ int sbb_distill(int dtype, const void *support_dev, const void *teacher_units_de
   ARG(e != 0, "distill: invalid dtype %d", dtype);
   ARG(unit_bytes == 4 || unit_bytes == 8, "distill: units are of 4 or 8 bytes, not %d", unit_bytes);
   ARG(rows >= 0 && H > 0 && Mc > 0 && K >= 0, "distill: bad shape rows=%ld H=%ld Mc=%ld K=%ld", rows, H, Mc, K);
-  ARG(std::isfinite(temperature) && temperature > 0, "distill: temperature %g is not above 0", temperature);
+  ARG(temperature >= 1e-15 && temperature <= 1e15, "distill: temperature %g is not from 1e-15 to 1e15", temperature);
   FITS(product(rows, H), "distill: %ld x %ld hypercolumns are more than 2^31 - 1", rows, H);
   FITS(Mc, "distill: more than 2^31 - 1 units in a hypercolumn");
   FITS(K, "distill: more than 2^31 - 1 kept units");

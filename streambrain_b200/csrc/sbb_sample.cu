@@ -499,7 +499,7 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
     return (int)__reduce_min_sync(0xffffffffu, index);
   }
   const float c = (float)(set.inv_t * 1.4426950408889634);
-  if (best == INFINITY || !(c < 1e30f)) return -2;
+  if (best == INFINITY || !(c > 1e-30f && c < 1e30f)) return -2;
   float total = 0;
 #pragma unroll
   for (int r = 0; r < EACH; ++r) {
@@ -1012,7 +1012,7 @@ struct Part {
   __device__ bool cut_quickly(F bin_of, const Settings &set, unsigned n, const Weights &weights, Cut<Key> &cut) {
     constexpr double kOne = 1099511627776.0;   // 2^40: 32-bit weights are summed in fixed point, up to 2^22 of them
     const float c = (float)(set.inv_t * 1.4426950408889634);
-    if (best == INFINITY || !(c < 1e30f) || !(set.top_p > 0) || n > 1u << 22) return false;
+    if (best == INFINITY || !(c > 1e-30f && c < 1e30f) || !(set.top_p > 0) || n > 1u << 22) return false;
     __syncthreads();
     for (int b = threadIdx.x; b < kBins; b += kThreads) s.bin_count[b] = 0;
     __syncthreads();
@@ -1257,7 +1257,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   const long long base = (long long)(g % H) * n;
   const Weights weights(s.table, set.inv_t, q);
-  const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
+  const u64 least = set.min_p > 0 ? (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one()) : 0;
   if (quick) {
     const W from_here = low > Keys<W>::of((W)-INFINITY) ? Keys<W>::value(low) : (W)-INFINITY;
     p.each_from(from_here, [&](W v, unsigned i) { p.put(v, i); });

@@ -277,6 +277,7 @@ def test_lookup_leaves_what_lies_around_its_results(t, m):
 SAMPLES = [  # rows, hypercolumns, units, spread of the support
     (1, 1, 1, 1.0), (3, 2, 2, 1.0), (5, 3, 10, 3.0), (9, 4, 33, 2.0), (4, 30, 100, 3.0), (2, 3, 128, 0.0), (2, 3, 300, 1.0),
     (2, 1, 513, 2.0), (2, 2, 1025, 0.5), (2, 1, 5000, 3.0), (1, 1, 40001, 3.0), (2, 1, 20000, 0.0), (1, 1, 70000, 0.05),
+    (80, 2, 611, 2.0), (170, 1, 2051, 0.1), (300, 1, 1024, 3.0),   # as many as SMs: a block each
 ]
 SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=5), dict(top_p=0.6), dict(min_p=0.1), dict(temperature=0.5, top_k=7, top_p=0.8, min_p=0.02),
             dict(temperature=2.0, top_p=0.97), dict(top_k=400, top_p=0.999), dict(top_p=0.0), dict(top_k=1), dict(min_p=1.0)]
@@ -368,9 +369,9 @@ def test_sample_masks(mc, t):
 
 
 @gpu
-@pytest.mark.parametrize("mc", [50, 700, 9000])
-def test_sample_with_settings_of_each_row(mc):
-    rows, h = 16, 2
+@pytest.mark.parametrize("rows,mc", [(16, 50), (16, 700), (16, 9000), (100, 1500)])
+def test_sample_with_settings_of_each_row(rows, mc):
+    h = 2
     x = values((rows, h * mc), BF16, 3, 3.0)
     rng = np.random.default_rng(5)
     u = torch.from_numpy(rng.random((rows, h)).astype(np.float32))
@@ -386,12 +387,65 @@ def test_sample_with_settings_of_each_row(mc):
 
 
 @gpu
+@pytest.mark.parametrize("rows,mc", [(8, 60), (8, 2000), (160, 2000)])
+def test_sample_settings_of_a_row_out_of_range(rows, mc):
+    """They act as the nearest in range: a temperature below 0 as 0, an infinite one as the limit (all that may be drawn is equally
+    likely), a top-p below 0 as 0 and above 1 as 1, a min-p below 0 as 0 and above 1 as 1."""
+    x = values((rows, mc), F32, 13, 2.0)
+    x[:, 3::4] = -math.inf
+    u = torch.from_numpy(np.random.default_rng(6).random((rows, 1)).astype(np.float32))
+    column = lambda *v: torch.tensor(v, dtype=F32).repeat(rows // len(v))
+    draw = lambda t, p, low, kk=0: k().sample_minicolumns(x.cuda(), 1, mc, u.cuda(), column(*t).cuda(), kk, column(*p).cuda(), column(*low).cuda()).cpu()
+    for kk in (0, 9):
+        got = draw((-1.0, 1.0, 1.0, 1.0), (1.0, -0.5, 1.0, 7.0), (0.0, 0.0, -3.0, 5.0), kk)
+        want = draw((0.0, 1.0, 1.0, 1.0), (1.0, 0.0, 1.0, 1.0), (0.0, 0.0, 0.0, 1.0), kk)
+        assert torch.equal(got, want)
+        assert torch.equal(want, plain_sample_fast(x, 1, mc, u, column(0.0, 1.0, 1.0, 1.0), kk, column(1.0, 0.0, 1.0, 1.0), column(0.0, 0.0, 0.0, 1.0)))
+    got = draw((math.inf, math.inf), (1.0, 0.5), (0.0, 0.0))
+    drawn = x.gather(1, got)
+    assert bool((drawn > -math.inf).all())
+    flat = torch.where(x > -math.inf, 0.0, x.double()).to(F32)
+    for r in range(0, rows, 2):
+        assert torch.equal(got[r], plain_sample_fast(flat[r:r + 1], 1, mc, u[r:r + 1], 1.0, 0, 1.0, 0.0)[0])
+
+
+@gpu
 @pytest.mark.parametrize("mc", [37, 2500])
 def test_sample_random_numbers_out_of_range(mc):
     x = values((1, mc), F32, 3).cuda()
     last = mc - 1
     for u, want in ((1.0, last), (5.0, last), (-3.0, 0), (math.nan, 0)):
         assert int(k().sample_minicolumns(x, 1, mc, torch.tensor([[u]], device="cuda"))) == want
+
+
+def offset(a):
+    """The same values one element behind a boundary of 16 bytes and more."""
+    b = torch.empty(a.numel() + 1, dtype=a.dtype, device="cuda")[1:].view(a.shape)
+    b.copy_(a)
+    assert b.is_contiguous() and b.data_ptr() % 16 == a.element_size() % 16
+    return b
+
+
+@gpu
+@pytest.mark.parametrize("t", ALL)
+def test_operators_on_tensors_that_begin_anywhere(t):
+    for rows, mc in ((3, 40), (2, 200), (3, 4096), (160, 1033)):
+        x = values((rows, mc), t, 51, 2.0)
+        u = torch.from_numpy(np.random.default_rng(52).random((rows, 1)).astype(np.float32))
+        for how in (dict(temperature=1.0, top_k=20, top_p=0.9, min_p=0.0), dict(temperature=1.0, top_k=0, top_p=0.9, min_p=0.01),
+                    dict(temperature=0.0, top_k=0, top_p=1.0, min_p=0.0)):
+            assert torch.equal(k().sample_minicolumns(offset(x), 1, mc, offset(u), **how).cpu(), plain_sample_fast(x, 1, mc, u, **how))
+        units, teacher = teacher_of(x, 1, mc, 7, 53)
+        want = k().distill_gradient(x.cuda(), 1, mc, units.cuda(), teacher.cuda(), 2.0)
+        _, grad, loss_off, grad_off = plain_distill(x, 1, mc, units, teacher, 2.0, None)
+        got = k().distill_gradient(offset(x), 1, mc, offset(units), offset(teacher), 2.0)
+        assert_close(got[0], want[0].double().cpu(), 2 * loss_off)
+        assert_close(got[1], grad, grad_off + rounding(t, grad))
+    w, c = values((31, 48), t, 54), codes_of("absent", 20, 5, 31, 55, torch.int64)
+    assert torch.equal(k().lookup(offset(w), offset(c)), k().lookup(w.cuda(), c.cuda()))
+    g = values((20, 48), t, 56)
+    want, size, most = plain_gradient(g, c, 31, 1.0)
+    assert_close(k().lookup_gradient(offset(g), offset(c), 31), want, (most + 2) * wide_half_step(t) * size + rounding(t, want))
 
 
 @gpu
@@ -415,6 +469,7 @@ def test_sample_of_nothing():
 DISTILLS = [  # rows, hypercolumns, units, kept, temperature
     (1, 1, 1, 1, 1.0), (3, 2, 2, 1, 2.0), (4, 1, 10, 3, 2.0), (3, 30, 100, 5, 1.0), (2, 3, 129, 8, 0.5), (2, 2, 300, 300, 4.0),
     (3, 1, 1025, 64, 1.0), (2, 1, 5003, 32, 3.0), (1, 2, 20000, 70, 1.0), (1, 1, 60000, 16, 1.0), (5, 7, 31, 40, 1.0),
+    (1, 1, 600, 700, 2.0), (1, 1, 3001, 1500, 1.0),   # more kept units than a block has threads
 ]
 
 
@@ -574,6 +629,19 @@ def test_operators_captured_into_a_graph():
     graph.replay()
     for a, b, c in zip(got, got2, want):
         assert torch.equal(a, c) and torch.equal(b, c)
+    # ... and the ways that large calls take
+    rows, n, m = 6000, 300, 24
+    g, c, x = values((rows, m), F32, 1).cuda(), codes_of("few", rows, 1, n, 2, torch.int64).cuda(), values((200, 3000), BF16, 3, 3.0).cuda()
+    u = torch.rand((200, 1), device="cuda")
+    large = lambda: (k().lookup_gradient(g, c, n), k().lookup_gradient(g.repeat(30, 1)[:140000], c.repeat(30, 1)[:140000], n),
+                     k().sample_minicolumns(x, 1, 3000, u, top_p=0.9), k().sample_minicolumns(x[:2], 1, 3000, u[:2], top_k=40),
+                     *k().distill_gradient(x, 1, 3000, c[:200, None, :1], x[:, None, :1].contiguous(), 1.0))
+    want = large()
+    third = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(third):
+        got = large()
+    third.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @gpu
