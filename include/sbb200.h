@@ -485,7 +485,8 @@ int sbb_lookup_gradient(int dtype, const void *grad_dev, const void *codes_dev, 
  * reaches top_p times their sum (all where top_p >= 1, at least one), of these the ones with w_i >= min_p (at least
  * the largest).  temperature <= 0: the largest, the first of equal ones.  A NaN support counts as -infinity; where
  * the largest is +infinity the units that have it are equally likely and the others out.
- * `*_rows` (may be null): device arrays with a value per row, used instead of the number beside them. */
+ * Numbers are rounded to float.  `*_rows` (may be null): device arrays with a value per row, used instead of the
+ * number beside them. */
 typedef struct sbb_sampling {
   double temperature, top_p, min_p;
   long top_k;

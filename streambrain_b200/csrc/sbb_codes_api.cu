@@ -147,7 +147,8 @@ int sbb_sample_minicolumns(int dtype, const void *support_dev, const float *rand
       "sample_minicolumns: misaligned pointer");
   if (const int rc = need_device()) return rc;
   if (rows == 0) return SBB_OK;
-  const sbb::Sampling s = {how->temperature,      how->top_p,      how->min_p,      0, how->top_k,
+  // (rounded to float, so that a number gives what a value for every row gives)
+  const sbb::Sampling s = {(float)how->temperature, (float)how->top_p, (float)how->min_p, 0, how->top_k,
                            how->temperature_rows, how->top_p_rows, how->min_p_rows, how->top_k_rows};
   return done(with_element<int>(dtype,
                                 [&](auto t, int) {

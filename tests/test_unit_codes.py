@@ -76,7 +76,7 @@ def plain_sample(x, h, mc, random, temperature, top_k, top_p, min_p):
     """Loops over hypercolumns; 64 bits."""
     rows = x.shape[0]
     x = x.double().numpy().reshape(rows, h, mc)
-    pick = lambda v, r: float(v[r]) if isinstance(v, torch.Tensor) else v
+    pick = lambda v, r: float(v[r]) if isinstance(v, torch.Tensor) else float(np.float32(v))   # (numbers are rounded to float32)
     out = np.full((rows, h), -1, dtype=np.int64)
     for r in range(rows):
         t, k, p, low = pick(temperature, r), int(pick(top_k, r)), pick(top_p, r), min(pick(min_p, r), 1.0)
@@ -302,7 +302,7 @@ def plain_sample_fast(x, h, mc, random, temperature, top_k, top_p, min_p):
     """:func:`plain_sample` without its quadratic sums: running sums in 64 bits."""
     rows = x.shape[0]
     x = x.double().numpy().reshape(rows, h, mc)
-    pick = lambda v, r: float(v[r]) if isinstance(v, torch.Tensor) else v
+    pick = lambda v, r: float(v[r]) if isinstance(v, torch.Tensor) else float(np.float32(v))   # (numbers are rounded to float32)
     out = np.full((rows, h), -1, dtype=np.int64)
     for r in range(rows):
         t, k_, p, low = pick(temperature, r), int(pick(top_k, r)), pick(top_p, r), min(pick(min_p, r), 1.0)
@@ -384,6 +384,9 @@ def test_sample_with_settings_of_each_row(rows, mc):
     assert torch.equal(got.cpu(), plain_sample_fast(x, h, mc, u, temperature, top_k, top_p, min_p))
     got = k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), 0.9, top_k.cuda(), 0.9, min_p.cuda())
     assert torch.equal(got.cpu(), plain_sample_fast(x, h, mc, u, 0.9, top_k, 0.9, min_p))
+    every = lambda v: torch.full((rows,), v, device="cuda")   # a number and the same for every row
+    assert torch.equal(k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), 0.7, 9, 0.95, 0.01),
+                       k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), every(0.7), every(9).int(), every(0.95), every(0.01)))
 
 
 @gpu
