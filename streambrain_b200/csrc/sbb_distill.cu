@@ -278,9 +278,12 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
 
 // ---- a cluster per group ---------------------------------------------------
 
-constexpr int kThreads = 512, kBlockWarps = kThreads / 32, kMostBlocks = 8;
+constexpr int kMostBlocks = 8;
 constexpr int kStage = 100 * 1024;   // bytes of a group that a block keeps in shared memory
-constexpr int kEntries = 512;        // kept units that wait in shared memory; those of longer lists are read again
+// Threads of a block: as many kept units wait in shared memory; those of longer lists are read again.  Groups of up to 8192 units go to
+// small blocks: 16000 groups of 520 float32 units took 151 us in large ones.
+constexpr int kLarge = 512, kSmall = 128;
+constexpr unsigned kSmallMost = 8192;
 
 // A running maximum and the sum of exp((x - maximum) / t).
 template <typename W>
@@ -295,17 +298,18 @@ struct Running {
   }
 };
 
-template <typename W>
+template <typename W, int THREADS>
 struct Block {
-  W best[2][kBlockWarps], sum[2][kBlockWarps], loss[kBlockWarps];
+  W best[2][THREADS / 32], sum[2][THREADS / 32], loss[THREADS / 32];
   Running<W> own;
-  Vec<W, 2> kept[kEntries];   // unit (as bits), p
+  Vec<W, 2> kept[THREADS];   // unit (as bits), p
 };
 
 // Two of them over all threads; all have the same bits.  (Joining maxima and sums one by one took as long as a row of 32000 units
 // itself.)
-template <typename W>
-__device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Block<W> &s) {
+template <typename W, int THREADS>
+__device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Block<W, THREADS> &s) {
+  constexpr unsigned kBlockWarps = THREADS / 32;
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const W r_warp = warp_max(r.best), t_warp = warp_max(t.best);
   if (lane == 0) s.best[0][warp] = r_warp, s.best[1][warp] = t_warp;
@@ -322,13 +326,14 @@ __device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Bl
 // STAGED: the part waits in shared memory between the sum and the gradient; else (no gradient, or groups beyond what a cluster
 // holds) it is read again.  VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last
 // one by single threads; else (support and gradient lie differently to the boundaries) element by element.
-template <typename T, bool VECTOR, bool STAGED>
-__global__ void __launch_bounds__(kThreads, 3) distill_block_kernel(const Distill<T> p, unsigned part) {
+template <typename T, bool VECTOR, bool STAGED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(const Distill<T> p, unsigned part) {
   after_previous();
   using W = Wide<T>;
+  constexpr unsigned kThreads = THREADS, kBlockWarps = THREADS / 32, kEntries = THREADS;
   constexpr int V = VECTOR ? 16 / (int)sizeof(T) : 1;
   extern __shared__ uint4 s_values[];
-  __shared__ Block<W> s;
+  __shared__ Block<W, THREADS> s;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned blocks = cluster.num_blocks(), g = blockIdx.x / blocks, rank = cluster.block_rank(), lane = threadIdx.x & 31;
   const unsigned begin = min(p.n, rank * part), size = min(part, p.n - begin);
@@ -483,14 +488,14 @@ cudaError_t launch_warps(const Distill<T> &p, cudaStream_t st) {
   return launch_next(distill_warp_kernel<T, V, NV>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, p);
 }
 
-template <typename T, bool VECTOR, bool STAGED>
+template <typename T, bool VECTOR, bool STAGED, int THREADS>
 cudaError_t launch_blocks(const Distill<T> &p, unsigned part, unsigned cluster, cudaStream_t st) {
   const size_t smem = STAGED ? (size_t)part * sizeof(T) : 0;
   if (smem > 0) {   // (holds for the current device)
-    const cudaError_t e = cudaFuncSetAttribute(distill_block_kernel<T, VECTOR, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    const cudaError_t e = cudaFuncSetAttribute(distill_block_kernel<T, VECTOR, STAGED, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
     if (e != cudaSuccess) return e;
   }
-  return launch_clusters(distill_block_kernel<T, VECTOR, STAGED>, dim3(p.groups * cluster), dim3(cluster), kThreads, smem, st, p, part);
+  return launch_clusters(distill_block_kernel<T, VECTOR, STAGED, THREADS>, dim3(p.groups * cluster), dim3(cluster), THREADS, smem, st, p, part);
 }
 
 template <typename T>
@@ -505,8 +510,12 @@ cudaError_t launch_wide(const Distill<T> &p, cudaStream_t st) {
   if ((size_t)p.groups * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const bool staged = p.gradient && (size_t)part * sizeof(T) <= kStage;
   const bool vector = !p.gradient || ((reinterpret_cast<uintptr_t>(p.support) ^ reinterpret_cast<uintptr_t>(p.gradient)) & 15) == 0;
-  if (vector) return staged ? launch_blocks<T, true, true>(p, part, cluster, st) : launch_blocks<T, true, false>(p, part, cluster, st);
-  return staged ? launch_blocks<T, false, true>(p, part, cluster, st) : launch_blocks<T, false, false>(p, part, cluster, st);
+  if (p.n <= kSmallMost && cluster == 1) {
+    if (vector) return staged ? launch_blocks<T, true, true, kSmall>(p, part, 1, st) : launch_blocks<T, true, false, kSmall>(p, part, 1, st);
+    return staged ? launch_blocks<T, false, true, kSmall>(p, part, 1, st) : launch_blocks<T, false, false, kSmall>(p, part, 1, st);
+  }
+  if (vector) return staged ? launch_blocks<T, true, true, kLarge>(p, part, cluster, st) : launch_blocks<T, true, false, kLarge>(p, part, cluster, st);
+  return staged ? launch_blocks<T, false, true, kLarge>(p, part, cluster, st) : launch_blocks<T, false, false, kLarge>(p, part, cluster, st);
 }
 
 }  // namespace
