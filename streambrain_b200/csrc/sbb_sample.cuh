@@ -7,8 +7,10 @@
 // A random number may lie next to the border of two units, and of a million draws some do within 32 bits' accuracy.  So weights
 // are formed in 64 bits and summed as integers, multiples of 2^-q: the sums are the same in any order and their errors below
 // n 2^-q of the largest weight.
-// Groups of up to 512 units are a warp's, in its registers; wider ones a cluster's of blocks, each with a part of the group in
-// shared memory, so that the support is read from memory once.
+// Groups of up to 512 units (1024 of the types summed in 32 bits) are a warp's, in its registers; wider ones a cluster's of blocks, each
+// with a part of the group in shared memory, so that the support is read from memory once.
+// (A source for each type, compiled side by side, includes this.)
+#pragma once
 #include "sbb_codes.cuh"
 #include "sbb_launch.cuh"
 
@@ -159,12 +161,13 @@ __device__ __forceinline__ u64 warp_min(u64 v) { return ~warp_max(~v); }
 
 // ---- a warp per group ------------------------------------------------------
 
-// Blocks on an SM, as registers allow; the launch has twice as many, since some draws take longer.
+// Blocks on an SM, as registers allow; the launch has twice as many, since some draws take longer.  Lanes of 32 units leave no registers
+// for the next group's.
 template <int EACH>
 constexpr int kWarpBlocks = EACH <= 4 ? 4 : EACH <= 8 ? 3 : 2;
 
 constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
-constexpr int kWarpBits = 48;   // q: the sum of a lane's 16 masses stays below 2^54
+constexpr int kWarpBits = 48;   // q: the sum of a lane's 32 masses stays below 2^54
 
 template <typename Key>
 struct alignas(16) Few {   // the units a cut lies among
@@ -508,9 +511,9 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
   }
   // A weight is off by 2^-22 of it (ex2.approx) and by 3 x 2^-24 = 1.8e-7 for every unit x of its exponent: x exp(-x) is below 0.37, so
   // by less than 3.1e-7 of the largest weight, 1, and, where it counts at all (x < 40), by 7.4e-6 of itself.  The 21 roundings on
-  // the way through a sum are 1.3e-6 of it.  Two sums are compared, one of them times a rounded factor.
+  // the way through a sum (37 with 32 units a lane) are 1.3e-6 (2.2e-6) of it.  Two sums are compared, one of them times a rounded factor.
   total = warp_sum(total);
-  g.error = 2 * fminf(1.7e-6f * n, 9e-6f * total) + 3e-7f * total;
+  g.error = 2 * fminf((EACH <= 16 ? 1.7e-6f : 2.8e-6f) * n, (EACH <= 16 ? 9e-6f : 1e-5f) * total) + 3e-7f * total;
   g.doubt = false;
   float value = -INFINITY, mass = total;
   unsigned index = n;
@@ -559,7 +562,7 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
   after_previous();
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
-  constexpr bool QUICK = sizeof(W) == 4;
+  constexpr bool QUICK = sizeof(W) == 4, AHEAD = QUICK && EACH <= 16;
   __shared__ double s_table[kTable];
   __shared__ Few<Key> s_few[kWarps];
   static_assert(sizeof(Few<Key>) >= sizeof(FewFloats), "one place for both");
@@ -572,7 +575,7 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
   unsigned g = blockIdx.x * kWarps + warp, row = g / H, h = g % H;
   if (g >= groups) return;
   T next[EACH];   // the next group's units, under way
-  if constexpr (QUICK) load_units<T, EACH>(support + (long)g * n, n, whole, next);
+  if constexpr (AHEAD) load_units<T, EACH>(support + (long)g * n, n, whole, next);
   for (; g < groups; g += step, row += rows, h += rest) {
     if (h >= H) h -= H, row += 1;
     const T *const x = support + (long)g * n;
@@ -581,9 +584,10 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
     int unit = -2;
     if constexpr (QUICK) {
       QuickGroup<EACH> group;
+      if constexpr (!AHEAD) load_units<T, EACH>(x, n, whole, next);
 #pragma unroll
       for (int r = 0; r < EACH; ++r) group.v[r] = no_nan(widen(next[r])) + 0.f;   // (no -0)
-      if (g + step < groups) load_units<T, EACH>(x + (long)step * n, n, whole, next);
+      if (AHEAD && g + step < groups) load_units<T, EACH>(x + (long)step * n, n, whole, next);
       unit = draw_quickly(group, n, set, u, reinterpret_cast<FewFloats &>(s_few[warp]));
     }
     if (unit == -2) unit = draw_exactly<T, EACH>(x, n, whole, set, u, s_table, s_few[warp]);
@@ -594,12 +598,27 @@ __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
 
 // ---- a cluster per group ---------------------------------------------------
 
-constexpr int kThreads = 512, kBlockWarps = kThreads / 32, kBins = 2048, kBinsEach = kBins / kThreads, kList = 512;
 constexpr int kMostBlocks = 8;       // of a cluster
 constexpr int kStage = 64 * 1024;    // bytes of a group that a block keeps in shared memory
-constexpr unsigned kQuickCount = 256;   // a top-k of up to this many goes by the threads' maxima
+// Threads of a block.  Where there are four groups for every SM, or they are short, small blocks with fewer and wider bins and a shorter
+// list take groups of up to 8192 units.  A top-p over float32, large and small blocks, us a call: 16000 groups of 520, 947 and 239; of
+// 8192, 4000 groups 345 and 306, 600 groups 66 and 64, but 160 groups 31 and 49.
+constexpr int kLarge = 512, kSmall = 128;
+constexpr unsigned kSmallMost = 8192;
+template <int THREADS>
+struct Shape {
+  static constexpr int kThreads = THREADS, kBlockWarps = THREADS / 32;
+  static constexpr int kPer = THREADS == kLarge ? 128 : 32;              // bins to one of the weights' exponent, 16 of these
+  static constexpr int kBins = 16 * kPer, kBinsEach = kBins / THREADS;
+  static constexpr int kList = THREADS;                                  // units that are ranked, a thread each
+  static constexpr unsigned kQuickCount = THREADS / 2;                   // a top-k of up to this many goes by the threads' maxima
+};
 
-struct Block {
+template <int THREADS>
+struct Block : Shape<THREADS> {
+  using Shape<THREADS>::kBins;
+  using Shape<THREADS>::kList;
+  using Shape<THREADS>::kBlockWarps;
   unsigned bin_count[kBins], bin_low[kBins], bin_high[kBins];   // masses in halves
   u64 list_key[kList];
   unsigned list_index[kList];
@@ -615,7 +634,9 @@ struct Block {
   __device__ __forceinline__ u64 mass(int b) const { return ((u64)bin_high[b] << 32) + bin_low[b]; }
 };
 
+template <int THREADS>
 __device__ __forceinline__ u64 block_sum(u64 v, u64 *s) {
+  constexpr int kBlockWarps = THREADS / 32;
   v = warp_sum(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
@@ -625,8 +646,9 @@ __device__ __forceinline__ u64 block_sum(u64 v, u64 *s) {
   for (int i = 0; i < kBlockWarps; ++i) v += s[i];
   return v;
 }
-template <typename Key>
+template <int THREADS, typename Key>
 __device__ __forceinline__ Key block_max(Key v, u64 *s) {
+  constexpr int kBlockWarps = THREADS / 32;
   v = warp_max(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
@@ -637,7 +659,9 @@ __device__ __forceinline__ Key block_max(Key v, u64 *s) {
   return (Key)m;
 }
 // The sum over the threads in front, in order.
+template <int THREADS>
 __device__ __forceinline__ u64 block_before(u64 v, u64 *s) {
+  constexpr int kBlockWarps = THREADS / 32;
   const u64 in = warp_up_to(v);
   __syncthreads();
   if ((threadIdx.x & 31) == 31) s[threadIdx.x >> 5] = in;
@@ -651,17 +675,29 @@ __device__ __forceinline__ u64 block_before(u64 v, u64 *s) {
 // The part of a group that a block works on: units [begin, begin + size), as elements [lead, lead + size) of `vectors` vectors.
 // Elements around them are -infinity: in shared memory, STAGED, they are there; else the first and the last vector are put
 // together from the elements that exist.
-template <typename T, bool STAGED>
-struct Part {
+template <typename T, bool STAGED, int THREADS>
+struct Part : Shape<THREADS> {
+  using Shape<THREADS>::kThreads;
+  using Shape<THREADS>::kBlockWarps;
+  using Shape<THREADS>::kPer;
+  using Shape<THREADS>::kBins;
+  using Shape<THREADS>::kBinsEach;
+  using Shape<THREADS>::kList;
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
   static constexpr int V = 16 / (int)sizeof(T);
   const Vec<T, V> *x;
   unsigned begin, size, lead, vectors;
   W best;
-  Block &s;
+  Block<THREADS> &s;
   cg::cluster_group cluster;
   int turn;
+
+  __device__ __forceinline__ Part(const Vec<T, V> *x_, unsigned begin_, unsigned size_, unsigned lead_, unsigned vectors_, Block<THREADS> &s_,
+                                  cg::cluster_group cluster_)
+      : x(x_), begin(begin_), size(size_), lead(lead_), vectors(vectors_), best(0), s(s_), cluster(cluster_), turn(0) {}
+  __device__ __forceinline__ u64 block_sum(u64 v, u64 *sum) const { return sbb::block_sum<THREADS>(v, sum); }
+  __device__ __forceinline__ u64 block_before(u64 v, u64 *sum) const { return sbb::block_before<THREADS>(v, sum); }
 
   // whole vectors: [first_whole(), end_whole())
   __device__ __forceinline__ unsigned first_whole() const { return STAGED || lead == 0 ? 0 : 1; }
@@ -772,7 +808,7 @@ struct Part {
     if (threadIdx.x == 0) s.swap[turn][0] = a, s.swap[turn][1] = b;
     cluster.sync();
     for (unsigned o = 0; o < cluster.num_blocks(); ++o) {
-      const Block *const other = cluster.map_shared_rank(&s, o);
+      const Block<THREADS> *const other = cluster.map_shared_rank(&s, o);
       f(other->swap[turn][0], other->swap[turn][1]);
     }
     turn ^= 1;
@@ -867,7 +903,7 @@ struct Part {
         unsigned c = s.bin_count[b];
         u64 m = s.mass(b);
         for (unsigned o = 1; o < cluster.num_blocks(); ++o) {
-          const Block *const other = cluster.map_shared_rank(&s, o);
+          const Block<THREADS> *const other = cluster.map_shared_rank(&s, o);
           c += other->bin_count[b];
           if (masses) m += other->mass(b);
         }
@@ -924,7 +960,7 @@ struct Part {
   // Puts a unit into the first block's list while there is room; s.list there counts all.  (It is 0 at first; the first block sets it
   // back to 0 ahead of a barrier of the cluster.)
   __device__ __forceinline__ void put(W v, unsigned unit) {
-    Block *const first = cluster.num_blocks() == 1 ? &s : cluster.map_shared_rank(&s, 0);
+    Block<THREADS> *const first = cluster.num_blocks() == 1 ? &s : cluster.map_shared_rank(&s, 0);
     const unsigned at = atomicAdd(&first->list, 1u);
     if (at >= kList) return;
     // (of 32-bit keys, one number in the order of the units)
@@ -1040,25 +1076,26 @@ struct Part {
     if (cluster.block_rank() == 0) {
       if (threadIdx.x == 0) s.found[0] = kBins, s.found[1] = kBins;
       unsigned count[kBinsEach];
-      double low = 0, high = 0;   // bounds on the bins' masses: a unit of bin b weighs e^-(b +- 1/2)/128, and e^1/256 is 1.0039
+      double low = 0, high = 0;   // bounds on the bins' masses: a unit of bin b weighs e^-(b +- 1/2)/kPer
+      constexpr double kUp = kPer == 128 ? 1.0041 : 1.0161, kDown = kPer == 128 ? 0.9959 : 0.9842;   // (e^1/256 is 1.0039, e^1/64 1.0158)
 #pragma unroll
       for (int j = 0; j < kBinsEach; ++j) {
         const int b = threadIdx.x * kBinsEach + j;
         count[j] = s.bin_count[b];
         for (unsigned o = 1; o < cluster.num_blocks(); ++o) count[j] += cluster.map_shared_rank(&s, o)->bin_count[b];
         s.bin_count[b] = count[j];
-        const double w = kOne * count[j] * (double)__expf(-b * (1.f / 128));
-        high += w * 1.0041;
-        low += w * 0.9959;
+        const double w = kOne * count[j] * (double)__expf(-b * (1.f / kPer));
+        high += w * kUp;
+        low += w * kDown;
       }
       double high_up_to = (double)block_before((u64)high, s.sum), low_up_to = (double)block_before((u64)low, s.sum);
       __syncthreads();   // s.found is there
 #pragma unroll
       for (int j = 0; j < kBinsEach; ++j) {
         const int b = threadIdx.x * kBinsEach + j;
-        const double w = kOne * count[j] * (double)__expf(-b * (1.f / 128));
-        high_up_to += w * 1.0041 + 1;
-        low_up_to += w * 0.9959;
+        const double w = kOne * count[j] * (double)__expf(-b * (1.f / kPer));
+        high_up_to += w * kUp + 1;
+        low_up_to += w * kDown;
         if (high_up_to + kThreads >= limit - error) atomicMin(&s.found[0], (u64)b);
         if (low_up_to >= limit + error) atomicMin(&s.found[1], (u64)b);
       }
@@ -1086,7 +1123,7 @@ struct Part {
     const unsigned in = (unsigned)s.found[1], above_count = (unsigned)s.found[3];
     if (in > kList) return false;
     u64 above = 0;
-    const W low = best - (W)((last + 2) / (128 * set.inv_t));   // no unit of the bins lies below
+    const W low = best - (W)((last + 2) / (kPer * set.inv_t));   // no unit of the bins lies below
     each_from(low, [&](W v, unsigned i) {
       const int b = bin_of(v);
       if (b > last) return;
@@ -1153,7 +1190,7 @@ struct Part {
           high = max(high, k);
         }
       });
-      const Key high_here = block_max(high, s.sum), low_here = block_max((Key)~low, s.sum);
+      const Key high_here = block_max<THREADS>(high, s.sum), low_here = block_max<THREADS>((Key)~low, s.sum);
       high = 0, low = 0;
       exchange(high_here, low_here, [&](u64 a, u64 b) { high = max(high, (Key)a), low = max(low, (Key)b); });
       lo = (Key)~low, hi = high;
@@ -1201,17 +1238,17 @@ struct Part {
   }
 };
 
-template <typename T, bool STAGED>
-__global__ void __launch_bounds__(kThreads, 2)
+template <typename T, bool STAGED, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     sample_block_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned H, unsigned n, unsigned part, const Sampling how,
                         int q, long long *__restrict__ codes) {
   after_previous();
   using W = Wide<T>;
   using Key = typename Keys<W>::type;
-  using P = Part<T, STAGED>;
-  constexpr int V = P::V;
+  using P = Part<T, STAGED, THREADS>;
+  constexpr int V = P::V, kThreads = THREADS, kBins = P::kBins, kList = P::kList;
   extern __shared__ uint4 s_values[];
-  __shared__ Block s;
+  __shared__ Block<THREADS> s;
   cg::cluster_group cluster = cg::this_cluster();
   const unsigned blocks = cluster.num_blocks(), g = blockIdx.x / blocks, rank = cluster.block_rank();
   const unsigned begin = min(n, rank * part), size = min(part, n - begin);
@@ -1224,15 +1261,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   const Vec<T, V> *const memory = reinterpret_cast<const Vec<T, V> *>(from - lead);
   W mine = -INFINITY;   // the largest of the values that pass through this thread, and the first vector that has it
   unsigned where = 0;
-  Part<T, false>{memory, begin, size, lead, vectors, (W)0, s, cluster, 0}.template range<STAGED ? 4 : 8>(threadIdx.x, vectors, kThreads, [&](const Vec<T, V> &a, unsigned i) {
+  Part<T, false, THREADS>(memory, begin, size, lead, vectors, s, cluster).template range<STAGED ? 4 : 8>(threadIdx.x, vectors, kThreads, [&](const Vec<T, V> &a, unsigned i) {
     if constexpr (STAGED) reinterpret_cast<Vec<T, V> *>(s_values)[i] = a;
     const W m = max_all(a);
     if (m > mine) mine = m, where = i;
   });
-  P p{STAGED ? reinterpret_cast<const Vec<T, V> *>(s_values) : memory, begin, size, lead, vectors, (W)0, s, cluster, 0};
+  P p(STAGED ? reinterpret_cast<const Vec<T, V> *>(s_values) : memory, begin, size, lead, vectors, s, cluster);
   const Key own = Keys<W>::of(mine);
-  Key top = block_max(own, s.sum), low = 0;
-  const bool by_count = set.top_k < n, quick = by_count && set.top_k > 1 && set.top_k <= kQuickCount;
+  Key top = block_max<THREADS>(own, s.sum), low = 0;
+  const bool by_count = set.top_k < n, quick = by_count && set.top_k > 1 && set.top_k <= P::kQuickCount;
   if (quick) {
     // A value that at least this block's share of the k units reach: the share's largest of the threads' maxima, in its first bits.
     const unsigned share = (set.top_k + blocks - 1) / blocks;
@@ -1279,7 +1316,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       });
       last = ~unit;
     }
-    last = block_max(last, s.sum);
+    last = block_max<THREADS>(last, s.sum);
     u64 of_all = 0;
     p.exchange(last, 0, [&](u64 a, u64) { of_all = max(of_all, a); });
     if (rank == 0 && threadIdx.x == 0) codes[g] = base + (long long)(unsigned)~of_all;
@@ -1289,8 +1326,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   Cut<Key> cut{0, n, 0};
   {
     if (by_count || set.top_p < 1) {
-      // bins of 1/128 in the weights' exponents, to the nearest; all units whose weight is below e^-16 share the last one
-      const W scale = (W)(128 * set.inv_t);
+      // bins of 1/128 (1/32) in the weights' exponents, to the nearest; all units whose weight is below e^-16 share the last one
+      const W scale = (W)(P::kPer * set.inv_t);
       auto bin = [&](W v) -> int {
         const W d = v == best ? (W)0 : fmin((best - v) * scale, (W)(kBins - 1));
         return sizeof(W) == 4 ? (int)(__float_as_uint((float)d + 8388608.f) & (kBins - 1)) : (int)rint(d);   // (2^23: rounds to an integer)
@@ -1299,7 +1336,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       if constexpr (sizeof(W) == 4) quick_p = !by_count && p.cut_quickly(bin, set, n, weights, cut);
       if (!quick_p) {
         u64 total = p.histogram(bin, !by_count, !by_count, weights);
-        if (!by_count) total = p.cluster_sum(block_sum(total, s.sum));
+        if (!by_count) total = p.cluster_sum(p.block_sum(total, s.sum));
         Want want = by_count ? want_count(set.top_k) : want_mass(set.top_p, total);
         const auto found = p.find(want, 0, 0);
         if (!by_count && found.above_count + found.in_bin <= kList) {
@@ -1317,7 +1354,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           p.each([&](W v, unsigned i) {
             if (kept(Keys<W>::of(v), i, cut)) sum += weights.of(v, best);
           });
-          want = want_mass(set.top_p, p.cluster_sum(block_sum(sum, s.sum)));
+          want = want_mass(set.top_p, p.cluster_sum(p.block_sum(sum, s.sum)));
           p.histogram(bin, true, false, weights);
           cut = p.cut(want, p.find(want, 0, 0), bin, weights);
         }
@@ -1354,15 +1391,15 @@ cudaError_t launch_warps(const T *support, const float *random, unsigned groups,
                      codes);
 }
 
-template <typename T, bool STAGED>
+template <typename T, bool STAGED, int THREADS>
 cudaError_t launch_blocks(const T *support, const float *random, unsigned groups, unsigned H, unsigned n, unsigned part, unsigned cluster,
                           const Sampling &s, long long *codes, cudaStream_t st) {
   const size_t smem = STAGED ? (size_t)part * sizeof(T) + 16 : 0;   // (a vector more where the part begins inside one)
   if (smem > 0) {   // (holds for the current device)
-    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage + 16);
+    const cudaError_t e = cudaFuncSetAttribute(sample_block_kernel<T, STAGED, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage + 16);
     if (e != cudaSuccess) return e;
   }
-  return launch_clusters(sample_block_kernel<T, STAGED>, dim3(groups * cluster), dim3(cluster), kThreads, smem, st, support, random, H, n, part, s,
+  return launch_clusters(sample_block_kernel<T, STAGED, THREADS>, dim3(groups * cluster), dim3(cluster), THREADS, smem, st, support, random, H, n, part, s,
                          mass_bits(n), codes);
 }
 
@@ -1383,6 +1420,10 @@ cudaError_t launch_sample(const T *support, const float *random, long rows, long
     e = launch_warps<T, 8>(support, random, groups, h, n, s, codes, st);
   } else if (n <= 512) {
     e = launch_warps<T, 16>(support, random, groups, h, n, s, codes, st);
+  } else if (n <= 1024 && sizeof(Wide<T>) == 4) {
+    // (16000 groups of 520 float32 units: a top-p 98 us here and 239 in small blocks, a top-k of 20 90 and 107; of float64, 193 and 193,
+    // 202 and 115)
+    if constexpr (sizeof(Wide<T>) == 4) e = launch_warps<T, 32>(support, random, groups, h, n, s, codes, st);
   } else {
     // With a group for every SM, a block each, which reads its group again where it has to (it is in L2 by then).  Fewer: the smallest
     // cluster whose blocks hold their parts in shared memory, and a larger one while there are SMs and parts are long.
@@ -1391,7 +1432,7 @@ cudaError_t launch_sample(const T *support, const float *random, long rows, long
     const bool alone = groups >= (unsigned)sm_count();
     // Where every row has its own top-k, some may have none and take several times as long: two blocks share a row if all fit side by
     // side.  256 x 128000 bf16, us a call: 157 with one, 112 with two; with one top-k of 100 for all 33 and 46.
-    if (alone && s.top_k_rows && groups < 2 * (unsigned)sm_count()) cluster = 2;
+    if (alone && n > kSmallMost && s.top_k_rows && groups < 2 * (unsigned)sm_count()) cluster = 2;
     if (!alone) {
       while (cluster < kMostBlocks && bytes > (size_t)cluster * kStage) cluster *= 2;
       while (cluster < kMostBlocks && (size_t)groups * cluster * 2 <= (size_t)sm_count() && n / cluster > 2048) cluster *= 2;
@@ -1399,15 +1440,16 @@ cudaError_t launch_sample(const T *support, const float *random, long rows, long
     constexpr unsigned V = 16 / (unsigned)sizeof(T);
     const unsigned part = ((n + cluster - 1) / cluster + V - 1) / V * V;
     if ((size_t)groups * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    e = !alone && (size_t)part * sizeof(T) <= kStage ? launch_blocks<T, true>(support, random, groups, h, n, part, cluster, s, codes, st)
-                                                     : launch_blocks<T, false>(support, random, groups, h, n, part, cluster, s, codes, st);
+    const bool staged = !alone && (size_t)part * sizeof(T) <= kStage;
+    if (alone && n <= kSmallMost && (n <= 2048 || groups >= 4 * (unsigned)sm_count())) {
+      e = launch_blocks<T, false, kSmall>(support, random, groups, h, n, part, cluster, s, codes, st);
+    } else {
+      e = staged ? launch_blocks<T, true, kLarge>(support, random, groups, h, n, part, cluster, s, codes, st)
+                 : launch_blocks<T, false, kLarge>(support, random, groups, h, n, part, cluster, s, codes, st);
+    }
   }
   if (e == cudaSuccess) count_launches(1);
   return e;
 }
-template cudaError_t launch_sample<float>(const float *, const float *, long, long, long, Sampling, long long *, cudaStream_t);
-template cudaError_t launch_sample<double>(const double *, const float *, long, long, long, Sampling, long long *, cudaStream_t);
-template cudaError_t launch_sample<__half>(const __half *, const float *, long, long, long, Sampling, long long *, cudaStream_t);
-template cudaError_t launch_sample<__nv_bfloat16>(const __nv_bfloat16 *, const float *, long, long, long, Sampling, long long *, cudaStream_t);
 
 }  // namespace sbb

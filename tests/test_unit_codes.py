@@ -278,6 +278,7 @@ SAMPLES = [  # rows, hypercolumns, units, spread of the support
     (1, 1, 1, 1.0), (3, 2, 2, 1.0), (5, 3, 10, 3.0), (9, 4, 33, 2.0), (4, 30, 100, 3.0), (2, 3, 128, 0.0), (2, 3, 300, 1.0),
     (2, 1, 513, 2.0), (2, 2, 1025, 0.5), (2, 1, 5000, 3.0), (1, 1, 40001, 3.0), (2, 1, 20000, 0.0), (1, 1, 70000, 0.05),
     (80, 2, 611, 2.0), (170, 1, 2051, 0.1), (300, 1, 1024, 3.0),   # as many as SMs: a block each
+    (150, 2, 513, 0.1), (3, 1, 1024, 0.0), (600, 1, 8001, 2.0), (300, 2, 5000, 0.0), (150, 1, 8001, 0.5),
 ]
 SETTINGS = [dict(), dict(temperature=0.0), dict(top_k=5), dict(top_p=0.6), dict(min_p=0.1), dict(temperature=0.5, top_k=7, top_p=0.8, min_p=0.02),
             dict(temperature=2.0, top_p=0.97), dict(top_k=400, top_p=0.999), dict(top_p=0.0), dict(top_k=1), dict(min_p=1.0)]
@@ -473,6 +474,7 @@ DISTILLS = [  # rows, hypercolumns, units, kept, temperature
     (1, 1, 1, 1, 1.0), (3, 2, 2, 1, 2.0), (4, 1, 10, 3, 2.0), (3, 30, 100, 5, 1.0), (2, 3, 129, 8, 0.5), (2, 2, 300, 300, 4.0),
     (3, 1, 1025, 64, 1.0), (2, 1, 5003, 32, 3.0), (1, 2, 20000, 70, 1.0), (1, 1, 60000, 16, 1.0), (5, 7, 31, 40, 1.0),
     (1, 1, 600, 700, 2.0), (1, 1, 3001, 1500, 1.0),   # more kept units than a block has threads
+    (400, 1, 5003, 200, 1.0), (150, 1, 8192, 5, 2.0), (150, 1, 8193, 5, 2.0),
 ]
 
 
