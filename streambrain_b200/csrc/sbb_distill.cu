@@ -126,7 +126,8 @@ __device__ __forceinline__ double warp_max(double v) {
 
 constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
 
-// Lane l holds vectors l, l + 32, ... of V units each, NV of them.
+// Lane l holds vectors l, l + 32, ... of V units each, NV of them.  Instructions and the latency of a warp's reductions bound it: 102400 groups
+// of 300 float32 units, 8 kept, 61 us, 70 % of the issue slots busy, 0.63 of a plain copy's bandwidth.
 template <typename T, int V, int NV>
 __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2) distill_warp_kernel(const Distill<T> p) {
   after_previous();
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
 constexpr int kMostBlocks = 8;
 constexpr int kStage = 100 * 1024;   // bytes of a group that a block keeps in shared memory
 // Threads of a block: as many kept units wait in shared memory; those of longer lists are read again.  Groups of up to 8192 units go to
-// small blocks: 16000 groups of 520 float32 units took 151 us in large ones.
+// small blocks: 16000 groups of 520 float32 units take 55 us, and took 151 in large ones; 4000 of 6000 units 47 and 57.
 constexpr int kLarge = 512, kSmall = 128;
 constexpr unsigned kSmallMost = 8192;
 
@@ -326,6 +327,8 @@ __device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Bl
 // STAGED: the part waits in shared memory between the sum and the gradient; else (no gradient, or groups beyond what a cluster
 // holds) it is read again.  VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last
 // one by single threads; else (support and gradient lie differently to the boundaries) element by element.
+// Instructions, and phases that do not overlap within a block, bound it: 4096 x 32000 bf16 units, 64 kept, 114 us, 71 % of the issue slots
+// busy, 0.70 of a plain copy's bandwidth.
 template <typename T, bool VECTOR, bool STAGED, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(const Distill<T> p, unsigned part) {
   after_previous();

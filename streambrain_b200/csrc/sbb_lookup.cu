@@ -13,7 +13,8 @@ constexpr int kThreads = 256;
 
 // `lanes` threads take V columns each of a row's tile; `parts` such groups of a block split the row's codes and the parts are added in
 // order; the block's other groups take other rows or tiles.  Codes are read eight at a time, so that as many weight rows are in
-// flight, and the next eight while these are.
+// flight, and the next eight while these are.  Bytes of the weight rows bound it: 4096 x 30 codes of 3000 x 1000 float32 51 us, 9.6 TB/s
+// (mostly out of L2); 784 codes of one row of 3000 float32 4.6 us, two trips to memory behind one another and the join of the parts.
 template <typename T, typename I, int V>
 __global__ void __launch_bounds__(kThreads)
     lookup_kernel(const T *__restrict__ weights, const I *__restrict__ codes, long rows, long L, long N, long M, Wide<T> scale, T *__restrict__ out,
@@ -80,6 +81,7 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // One code a row: copies of weight rows, U under way per thread.  A block takes whole pieces of kThreads * U vectors of the result.
+// Memory bounds it: 16384 codes of 50000 x 1024 bf16 8.2 us, 0.86 of a plain copy's bandwidth.
 template <typename T, typename I, int V, int U>
 __global__ void __launch_bounds__(kThreads)
     lookup_one_kernel(const T *__restrict__ weights, const I *__restrict__ codes, long rows, long N, long M, Wide<T> scale, T *__restrict__ out,
@@ -180,7 +182,7 @@ __device__ __forceinline__ void set_zero(const Zero &z, unsigned block) {
 __device__ __forceinline__ unsigned below(unsigned a, unsigned b) { return (a - b) >> 31; }
 
 // Sorted position of an entry = the entries with a smaller key + those with the same key in front.  A warp takes four entries;
-// one launch where a radix sort is four.
+// one launch where a radix sort is four.  Comparisons bound it, the entries squared: 3840 codes with their sums 9.6 us.
 template <typename I>
 __global__ void __launch_bounds__(kThreads)
     rank_kernel(const I *__restrict__ codes, unsigned entries, unsigned L, long N, uint2 *__restrict__ to, unsigned blocks, const Zero zero) {
@@ -304,7 +306,8 @@ __global__ void __launch_bounds__(kSortThreads)
 
 // The same sort by one cluster in one launch, for as many entries as its threads hold: an entry's place is found in registers and
 // shared memory, and the entries move between the blocks' shared memories.  They are put in order within the block first, so that
-// neighbours go to neighbouring places (one by one, each store was 32 requests, and 65536 entries took 24 us).
+// neighbours go to neighbouring places (one by one, each store was 32 requests, and 65536 entries took 24 us).  The steps of a pass and the
+// cluster's barriers between them bound it: 7505 entries of two passes 8 us, 65536 with 100 MB of zeros beside them 29 us.
 constexpr int kClusterThreads = 1024, kClusterWarps = kClusterThreads / 32, kClusterBlocks = 16;
 
 struct SortSpace {
@@ -444,6 +447,7 @@ struct Sums {
 
 // `lanes` threads take a chunk and a tile of columns, a block the chunks of a span.  A run inside a chunk is written; the others'
 // parts wait in shared memory and the group in which a run begins (the first one, for a run from the span before) adds them up.
+// Memory bounds it: 65536 rows of 1024 bf16 elements in the order of their codes 33 us, 0.55 of the DRAM peak.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p) {
   after_previous();
@@ -548,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p) {
 
 // Adds the parts of the runs that cross the end of a span and begin in it: a group of `lanes` threads for each span and tile
 // of columns, all groups of the block together for runs of many parts (of which a block, with spans that follow one another,
-// has few).
+// has few).  Latency bounds it: 3 to 6 us.
 constexpr unsigned kLongRun = 32;
 template <typename T, int V, int THREADS>
 struct JoinSpace {

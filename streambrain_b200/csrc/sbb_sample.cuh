@@ -555,6 +555,8 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
   return (int)__shfl_sync(0xffffffffu, unit, who & 31);
 }
 
+// Instructions bound it: 122880 groups of 100 float32 units with a top-p of 0.9 87 us, 600 instructions a group, 78 % of the issue slots busy
+// (no top-p 41 us, greedy 24).  All in registers, a warp needs no barrier; a block for a group of 520 took twice as long.
 template <typename T, int EACH>
 __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
     sample_warp_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned groups, unsigned H, unsigned n, bool whole,
@@ -1238,6 +1240,9 @@ struct Part : Shape<THREADS> {
   }
 };
 
+// Few groups are bound by latency, the barriers of a block and its cluster: one of 32000 float16 units, top-k 50 and top-p 0.9, 12 us.
+// Many by instructions on every unit: 256 x 128000 bf16 with a top-k of 100 33 us (greedy 14, the support at the copy bandwidth 10), with
+// settings of each row, some without a top-k, 113.
 template <typename T, bool STAGED, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     sample_block_kernel(const T *__restrict__ support, const float *__restrict__ random, unsigned H, unsigned n, unsigned part, const Sampling how,
