@@ -3,7 +3,7 @@
 // With p the softmax of the teacher's kept units, q the softmax of all of the student's group, both at temperature t, and w the
 // row's weight: loss = w t^2 sum_k p_k (log p_k - log q_{u_k}), and d loss / d x_i = w t (q_i - sum over k with u_k = i of p_k).
 // What bounds it is memory: the student's support is read once and its gradient written once.  Groups of up to 512 units are a
-// warp's, in its registers; wider ones a cluster's of blocks, which keep their parts in shared memory for the gradient while they
+// warp's (of up to 64, eight lanes'), in its registers; wider ones a cluster's of blocks, which keep their parts in shared memory for the gradient while they
 // form the running maximum and sum.
 #include "sbb_codes.cuh"
 #include "sbb_launch.cuh"
@@ -124,18 +124,26 @@ __device__ __forceinline__ double warp_max(double v) {
 
 // ---- a warp per group ------------------------------------------------------
 
-constexpr int kWarpThreads = 256, kWarps = kWarpThreads / 32;
+constexpr int kWarpThreads = 256;
 
-// Lane l holds vectors l, l + 32, ... of V units each, NV of them.  Instructions and the latency of a warp's reductions bound it: 102400 groups
+// LANES lanes take a group: a warp, or eight lanes where it has few units.  Lane l holds vectors l, l + LANES, ... of V units each, NV of
+// them.   Instructions and the latency of a warp's reductions bound it: 102400 groups
 // of 300 float32 units, 8 kept, 61 us, 70 % of the issue slots busy, 0.63 of a plain copy's bandwidth.
-template <typename T, int V, int NV>
+template <typename T, int V, int NV, int LANES>
 __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2) distill_warp_kernel(const Distill<T> p) {
   after_previous();
   using W = Wide<T>;
-  __shared__ Vec<W, V> s_kept[kWarps][NV * 32];   // what the teacher gives each unit
-  const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, step = gridDim.x * kWarps, rows = step / p.H, rest = step % p.H;
-  W *const kept = s_kept[warp][0].v;
-  unsigned g = blockIdx.x * kWarps + warp, row = g / p.H, h = g % p.H;
+  constexpr unsigned kGroups = kWarpThreads / LANES;   // of a block at a time
+  __shared__ Vec<W, V> s_kept[kGroups][NV * LANES];   // what the teacher gives each unit
+  const unsigned lane = threadIdx.x % LANES, group = threadIdx.x / LANES, step = gridDim.x * kGroups, rows = step / p.H, rest = step % p.H;
+  const unsigned first_lane = (threadIdx.x & 31) - lane, mask = (0xffffffffu >> (32 - LANES)) << first_lane;   // the group's lanes
+  auto group_max = [&](W v) {
+    if constexpr (LANES == 32) return warp_max(v);
+    for (int off = LANES / 2; off > 0; off >>= 1) v = fmax(v, __shfl_xor_sync(mask, v, off));
+    return v;
+  };
+  W *const kept = s_kept[group][0].v;
+  unsigned g = blockIdx.x * kGroups + group, row = g / p.H, h = g % p.H;
   // the next group's units and teacher, under way while one is worked on
   struct Ahead {
     Vec<T, V> raw[NV];
@@ -146,7 +154,7 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
     const T *const x = p.support + (long)i * p.n;
 #pragma unroll
     for (int r = 0; r < NV; ++r)
-      if ((r * 32 + lane) * V < p.n) next.raw[r] = *reinterpret_cast<const Vec<T, V> *>(x + (r * 32 + lane) * V);
+      if ((r * LANES + lane) * V < p.n) next.raw[r] = *reinterpret_cast<const Vec<T, V> *>(x + (r * LANES + lane) * V);
     if (lane < p.K) {
       next.u = p.unit(i, lane);
       next.t = p.teacher[(long)i * p.K + lane];
@@ -162,7 +170,7 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
 #pragma unroll
     for (int r = 0; r < NV; ++r)
 #pragma unroll
-      for (int v = 0; v < V; ++v) e[r][v] = (r * 32 + lane) * V < p.n ? widen(next.raw[r].v[v]) : (W)-INFINITY;
+      for (int v = 0; v < V; ++v) e[r][v] = (r * LANES + lane) * V < p.n ? widen(next.raw[r].v[v]) : (W)-INFINITY;
     const unsigned u0 = lane < p.K ? next.u : p.n;
     const W t0 = u0 < p.n ? widen(next.t) : (W)-INFINITY, x0 = u0 < p.n ? widen(x[u0]) : (W)0;
     if (g + step < p.groups) fetch(g + step);
@@ -171,11 +179,11 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
       for (int r = 0; r < NV; ++r)
 #pragma unroll
         for (int v = 0; v < V; ++v) best = fmax(best, e[r][v]);
-      best = warp_max(best);
+      best = group_max(best);
       tbest = t0;
-      for (unsigned k = lane + 32; k < p.K; k += 32)
+      for (unsigned k = lane + LANES; k < p.K; k += LANES)
         if (p.unit(g, k) < p.n) tbest = fmax(tbest, widen(p.teacher[(long)g * p.K + k]));
-      tbest = warp_max(tbest);
+      tbest = group_max(tbest);
     }
     bool nothing = w == (W)0 || best == -INFINITY || tbest == -INFINITY;
     if (nothing && w != (W)0) {   // (the maxima pass over NaN, which is not nothing)
@@ -184,8 +192,8 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
       for (int r = 0; r < NV; ++r)
 #pragma unroll
         for (int v = 0; v < V; ++v) nan = nan || e[r][v] != e[r][v];
-      for (unsigned k = lane + 32; k < p.K; k += 32) nan = nan || (p.unit(g, k) < p.n && isnan(widen(p.teacher[(long)g * p.K + k])));
-      nothing = !__any_sync(0xffffffffu, nan);
+      for (unsigned k = lane + LANES; k < p.K; k += LANES) nan = nan || (p.unit(g, k) < p.n && isnan(widen(p.teacher[(long)g * p.K + k])));
+      nothing = !__any_sync(mask, nan);
     }
     if (nothing) {
       if (lane == 0) p.loss[g] = 0;
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
         for (int v = 0; v < V; ++v) zero.v[v] = narrow_to<T>((W)0);
 #pragma unroll
         for (int r = 0; r < NV; ++r)
-          if ((r * 32 + lane) * V < p.n) *reinterpret_cast<Vec<T, V> *>(out + (r * 32 + lane) * V) = zero;
+          if ((r * LANES + lane) * V < p.n) *reinterpret_cast<Vec<T, V> *>(out + (r * LANES + lane) * V) = zero;
       }
       continue;
     }
@@ -204,8 +212,8 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
 #pragma unroll
       for (int v = 0; v < V; ++v) zero.v[v] = 0;
 #pragma unroll
-      for (int r = 0; r < NV; ++r) s_kept[warp][r * 32 + lane] = zero;
-      __syncwarp();
+      for (int r = 0; r < NV; ++r) s_kept[group][r * LANES + lane] = zero;
+      __syncwarp(mask);
     }
 #pragma unroll
     for (int r = 0; r < NV; ++r) {
@@ -221,19 +229,19 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
       return pk;
     };
     const W p0 = entry(u0 < p.n, t0, x0);
-    for (unsigned k = lane + 32; k < p.K; k += 32) {
+    for (unsigned k = lane + LANES; k < p.K; k += LANES) {
       const unsigned u = p.unit(g, k);
       if (u < p.n) entry(true, widen(p.teacher[(long)g * p.K + k]), widen(x[u]));
     }
-    for (int off = 16; off > 0; off >>= 1) {
-      total += __shfl_xor_sync(0xffffffffu, total, off);
-      ttotal += __shfl_xor_sync(0xffffffffu, ttotal, off);
-      sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    for (int off = LANES / 2; off > 0; off >>= 1) {
+      total += __shfl_xor_sync(mask, total, off);
+      ttotal += __shfl_xor_sync(mask, ttotal, off);
+      sum += __shfl_xor_sync(mask, sum, off);
     }
     const W share = (W)1 / ttotal;
     sum = sum * share + (sbb_log(total) - sbb_log(ttotal));
     if (p.gradient)
-      for (unsigned k0 = 0; k0 < p.K; k0 += 32) {
+      for (unsigned k0 = 0; k0 < p.K; k0 += LANES) {
         unsigned u = u0;
         W pk = p0;
         if (k0 > 0) {
@@ -245,35 +253,35 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2
         const bool there = u < p.n;
         W before = 0;
         if (there && k0 > 0) before = kept[u];
-        __syncwarp();
+        __syncwarp(mask);
         if (there) kept[u] = (W)lane;
-        __syncwarp();
-        if (__any_sync(0xffffffffu, there && kept[u] != (W)lane)) {
-          const unsigned same = __match_any_sync(0xffffffffu, there ? u : ~lane);
+        __syncwarp(mask);
+        if (__any_sync(mask, there && kept[u] != (W)lane)) {
+          const unsigned same = __match_any_sync(mask, there ? u : ~lane) >> first_lane;
           W part = 0;
-          for (int j = 0; j < 32; ++j) {
-            const W o = __shfl_sync(0xffffffffu, pk, j);
+          for (int j = 0; j < LANES; ++j) {
+            const W o = __shfl_sync(mask, pk, j, LANES);
             if (same >> j & 1) part += o;
           }
           pk = part;
         }
-        __syncwarp();
+        __syncwarp(mask);
         if (there) kept[u] = before + pk;   // (those that name the same unit write the same)
-        __syncwarp();
+        __syncwarp(mask);
       }
     if (lane == 0) p.loss[g] = w * p.temperature * p.temperature * sum;
     if (!p.gradient) continue;
     const W wt = w * p.temperature, scale = wt / total;
 #pragma unroll
     for (int r = 0; r < NV; ++r)
-      if ((r * 32 + lane) * V < p.n) {
-        const Vec<W, V> k = s_kept[warp][r * 32 + lane];
+      if ((r * LANES + lane) * V < p.n) {
+        const Vec<W, V> k = s_kept[group][r * LANES + lane];
         scale_all(e[r], scale);
 #pragma unroll
         for (int v = 0; v < V; ++v) e[r][v] -= wt * k.v[v];
-        *reinterpret_cast<Vec<T, V> *>(out + (r * 32 + lane) * V) = narrow_all<T, V>(e[r]);
+        *reinterpret_cast<Vec<T, V> *>(out + (r * LANES + lane) * V) = narrow_all<T, V>(e[r]);
       }
-    __syncwarp();
+    __syncwarp(mask);
   }
 }
 
@@ -485,10 +493,11 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(
   }
 }
 
-template <typename T, int V, int NV>
+template <typename T, int V, int NV, int LANES = 32>
 cudaError_t launch_warps(const Distill<T> &p, cudaStream_t st) {
-  const unsigned most = 16 * (unsigned)sm_count(), blocks = (p.groups + kWarps - 1) / kWarps;
-  return launch_next(distill_warp_kernel<T, V, NV>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, p);
+  constexpr unsigned groups = kWarpThreads / LANES;
+  const unsigned most = 16 * (unsigned)sm_count(), blocks = (p.groups + groups - 1) / groups;
+  return launch_next(distill_warp_kernel<T, V, NV, LANES>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, p);
 }
 
 template <typename T, bool VECTOR, bool STAGED, int THREADS>
@@ -534,18 +543,28 @@ cudaError_t launch_distill(const T *support, const I *units, const T *teacher, c
   cudaError_t e;
   if (Mc > 512) {
     e = launch_wide(p, st);
-  } else if (vec == V) {
+  } else if (Mc <= 64) {   // eight lanes a group.  227000 float64 groups of 16, 16 kept, without a gradient: 63 us, with a warp each 173
+    if (vec != V) {
+      e = Mc <= 8 ? launch_warps<T, 1, 1, 8>(p, st) : Mc <= 16 ? launch_warps<T, 1, 2, 8>(p, st) : Mc <= 32 ? launch_warps<T, 1, 4, 8>(p, st)
+          : launch_warps<T, 1, 8, 8>(p, st);
+    } else if constexpr (V == 8) {
+      e = launch_warps<T, V, 1, 8>(p, st);
+    } else if constexpr (V == 4) {
+      e = Mc <= 32 ? launch_warps<T, V, 1, 8>(p, st) : launch_warps<T, V, 2, 8>(p, st);
+    } else {
+      e = Mc <= 16 ? launch_warps<T, V, 1, 8>(p, st) : Mc <= 32 ? launch_warps<T, V, 2, 8>(p, st) : launch_warps<T, V, 4, 8>(p, st);
+    }
+  } else if (vec == V) {   // a warp a group
     const long vectors = (Mc + 32 * V - 1) / (32 * V);
     if constexpr (V == 8) {
       e = vectors <= 1 ? launch_warps<T, V, 1>(p, st) : launch_warps<T, V, 2>(p, st);
     } else if constexpr (V == 4) {
       e = vectors <= 1 ? launch_warps<T, V, 1>(p, st) : vectors <= 2 ? launch_warps<T, V, 2>(p, st) : vectors <= 3 ? launch_warps<T, V, 3>(p, st) : launch_warps<T, V, 4>(p, st);
     } else {
-      e = vectors <= 1 ? launch_warps<T, V, 1>(p, st) : vectors <= 2 ? launch_warps<T, V, 2>(p, st) : vectors <= 4 ? launch_warps<T, V, 4>(p, st) : launch_warps<T, V, 8>(p, st);
+      e = vectors <= 2 ? launch_warps<T, V, 2>(p, st) : vectors <= 4 ? launch_warps<T, V, 4>(p, st) : launch_warps<T, V, 8>(p, st);
     }
   } else {
-    e = Mc <= 32 ? launch_warps<T, 1, 1>(p, st) : Mc <= 64 ? launch_warps<T, 1, 2>(p, st) : Mc <= 128 ? launch_warps<T, 1, 4>(p, st)
-        : Mc <= 256 ? launch_warps<T, 1, 8>(p, st) : launch_warps<T, 1, 16>(p, st);
+    e = Mc <= 128 ? launch_warps<T, 1, 4>(p, st) : Mc <= 256 ? launch_warps<T, 1, 8>(p, st) : launch_warps<T, 1, 16>(p, st);
   }
   if (e == cudaSuccess) count_launches(1);
   return e;

@@ -475,6 +475,7 @@ DISTILLS = [  # rows, hypercolumns, units, kept, temperature
     (3, 1, 1025, 64, 1.0), (2, 1, 5003, 32, 3.0), (1, 2, 20000, 70, 1.0), (1, 1, 60000, 16, 1.0), (5, 7, 31, 40, 1.0),
     (1, 1, 600, 700, 2.0), (1, 1, 3001, 1500, 1.0),   # more kept units than a block has threads
     (400, 1, 5003, 200, 1.0), (150, 1, 8192, 5, 2.0), (150, 1, 8193, 5, 2.0),
+    (37, 5, 8, 3, 1.0), (11, 3, 9, 20, 2.0), (50, 3, 16, 16, 1.0), (7, 3, 33, 9, 1.0), (301, 7, 47, 10, 2.0), (5, 5, 64, 64, 1.0), (5, 5, 65, 40, 1.0),
 ]
 
 
