@@ -2,8 +2,8 @@
 //
 // With p the softmax of the teacher's kept units, q the softmax of all of the student's group, both at temperature t, and w the
 // row's weight: loss = w t^2 sum_k p_k (log p_k - log q_{u_k}), and d loss / d x_i = w t (q_i - sum over k with u_k = i of p_k).
-// What bounds it is memory: the student's support is read once and its gradient written once.  Groups of up to 512 units are a
-// warp's (of up to 64, eight lanes'), in its registers; wider ones a cluster's of blocks, which keep their parts in shared memory for the gradient while they
+// What bounds it is memory: the student's support is read once and its gradient written once.  Groups of up to 512 units are 8
+// to 32 lanes', in their registers; wider ones a cluster's of blocks, which keep their parts in shared memory for the gradient while they
 // form the running maximum and sum.
 #include "sbb_codes.cuh"
 #include "sbb_launch.cuh"
@@ -122,15 +122,15 @@ __device__ __forceinline__ double warp_max(double v) {
   return v;
 }
 
-// ---- a warp per group ------------------------------------------------------
+// ---- lanes of a warp per group ----------------------------------------------
 
 constexpr int kWarpThreads = 256;
 
-// LANES lanes take a group: a warp, or eight lanes where it has few units.  Lane l holds vectors l, l + LANES, ... of V units each, NV of
-// them.   Instructions and the latency of a warp's reductions bound it: 102400 groups
-// of 300 float32 units, 8 kept, 61 us, 70 % of the issue slots busy, 0.63 of a plain copy's bandwidth.
+// LANES lanes take a group, 8, 16 or 32: as few as hold it in their registers, so that a warp's reductions serve several groups.  Lane l
+// holds vectors l, l + LANES, ... of V units each, NV of them.  Instructions and the latency of the reductions bound it: 102400 groups of
+// 300 float32 units, 8 kept, 49 us (a warp each 61), 0.79 of a plain copy's bandwidth; 224000 of 100, 5 kept, 53 us (137).
 template <typename T, int V, int NV, int LANES>
-__global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 64 ? 3 : 2) distill_warp_kernel(const Distill<T> p) {
+__global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 80 ? 3 : 2) distill_warp_kernel(const Distill<T> p) {
   after_previous();
   using W = Wide<T>;
   constexpr unsigned kGroups = kWarpThreads / LANES;   // of a block at a time
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(
   }
 }
 
-template <typename T, int V, int NV, int LANES = 32>
+template <typename T, int V, int NV, int LANES>
 cudaError_t launch_warps(const Distill<T> &p, cudaStream_t st) {
   constexpr unsigned groups = kWarpThreads / LANES;
   const unsigned most = 16 * (unsigned)sm_count(), blocks = (p.groups + groups - 1) / groups;
@@ -554,17 +554,19 @@ cudaError_t launch_distill(const T *support, const I *units, const T *teacher, c
     } else {
       e = Mc <= 16 ? launch_warps<T, V, 1, 8>(p, st) : Mc <= 32 ? launch_warps<T, V, 2, 8>(p, st) : launch_warps<T, V, 4, 8>(p, st);
     }
-  } else if (vec == V) {   // a warp a group
-    const long vectors = (Mc + 32 * V - 1) / (32 * V);
+  } else if (Mc <= 128) {
+    e = vec == V ? launch_warps<T, V, 16 / V, 8>(p, st) : launch_warps<T, 1, 16, 8>(p, st);
+  } else if (vec == V) {   // (20 float32 units a lane leave registers for three blocks on an SM: with two, groups of 300 take 62 us, not 49)
     if constexpr (V == 8) {
-      e = vectors <= 1 ? launch_warps<T, V, 1>(p, st) : launch_warps<T, V, 2>(p, st);
+      e = Mc <= 256 ? launch_warps<T, V, 4, 8>(p, st) : launch_warps<T, V, 4, 16>(p, st);
     } else if constexpr (V == 4) {
-      e = vectors <= 1 ? launch_warps<T, V, 1>(p, st) : vectors <= 2 ? launch_warps<T, V, 2>(p, st) : vectors <= 3 ? launch_warps<T, V, 3>(p, st) : launch_warps<T, V, 4>(p, st);
+      e = Mc <= 256 ? launch_warps<T, V, 4, 16>(p, st) : Mc <= 320 ? launch_warps<T, V, 5, 16>(p, st) : Mc <= 384 ? launch_warps<T, V, 3, 32>(p, st)
+          : launch_warps<T, V, 4, 32>(p, st);
     } else {
-      e = vectors <= 2 ? launch_warps<T, V, 2>(p, st) : vectors <= 4 ? launch_warps<T, V, 4>(p, st) : launch_warps<T, V, 8>(p, st);
+      e = Mc <= 256 ? launch_warps<T, V, 8, 16>(p, st) : launch_warps<T, V, 8, 32>(p, st);
     }
   } else {
-    e = Mc <= 128 ? launch_warps<T, 1, 4>(p, st) : Mc <= 256 ? launch_warps<T, 1, 8>(p, st) : launch_warps<T, 1, 16>(p, st);
+    e = Mc <= 256 ? launch_warps<T, 1, 16, 16>(p, st) : launch_warps<T, 1, 16, 32>(p, st);
   }
   if (e == cudaSuccess) count_launches(1);
   return e;
