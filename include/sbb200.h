@@ -495,7 +495,11 @@ typedef struct sbb_sampling {
 } sbb_sampling;
 /* codes[rows, H] (int64) = h * Mc + the unit drawn from hypercolumn h of support[rows, H * Mc]: the first unit in
  * index order at which the running sum of the kept w passes random[row, h] times their sum; random[rows, H] in
- * [0, 1).  -1 where every unit of the hypercolumn is at -infinity.  Weights are formed in 64 bits. */
+ * [0, 1) (1 and more: the last unit that weighs anything; below 0 and NaN: as 0).  -1 where every unit of the
+ * hypercolumn is at -infinity.  Weights are formed in 64 bits and summed in fixed point: sums are off by at most
+ * Mc 2^-(q+1) of the largest weight, with q = 48 for hypercolumns of up to 512 units (1024 of all types but SBB_F64) and
+ * the largest up to 50 with Mc 2^q < 2^62 for wider ones; for random numbers below 2^-20, of random times the sum too, so
+ * that a random number of 0 draws the first kept unit whose weight is above 0 in 64 bits. */
 int sbb_sample_minicolumns(int dtype, const void *support_dev, const float *random_dev, long rows, long H, long Mc,
                            const sbb_sampling *how, long long *codes_dev, void *stream);
 

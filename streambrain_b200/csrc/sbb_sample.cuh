@@ -6,7 +6,7 @@
 // are compared with one another.
 // A random number may lie next to the border of two units, and of a million draws some do within 32 bits' accuracy.  So weights
 // are formed in 64 bits and summed as integers, multiples of 2^-q: the sums are the same in any order and their errors below
-// n 2^-q of the largest weight.
+// n 2^-q of the largest weight; where the random number is small, of what is looked for (Lift).
 // Groups of up to 512 units (1024 of the types summed in 32 bits) are a warp's, in its registers; wider ones a cluster's of blocks, each
 // with a part of the group in shared memory, so that the support is read from memory once.
 // (A source for each type, compiled side by side, includes this.)
@@ -80,22 +80,53 @@ struct Weights {
   }
   __device__ __forceinline__ Weights(const double *tab, double inv_t, int q_) : table(tab), c(inv_t * 92.332482616893656877), q(q_) {}
   __device__ __forceinline__ u64 one() const { return 1ull << q; }
-  __device__ __forceinline__ u64 mass(double d) const {
+  // 2^lift times the mass of a weight of 2^(x/64)
+  __device__ __forceinline__ u64 power(double x, int lift) const {
     constexpr double kRound = 6755399441055744.0;            // 1.5 * 2^52: what is added to it is rounded to an integer
     constexpr double a = 0.010830424696249145252;            // ln 2 / 64
     constexpr double a2 = a * a / 2, a3 = a2 * a / 3, a4 = a3 * a / 4, a5 = a4 * a / 5;
-    const double t = d * c;
-    if (!(t > -(double)kTable * (q + 2))) return 0;
-    const double big = t + kRound, r = t - (big - kRound);
+    if (!(x > -(double)kTable * (q + lift + 2))) return 0;
+    const double big = x + kRound, r = x - (big - kRound);
     const int n = __double2loint(big);
     const double p = fma(fma(fma(fma(fma(a5, r, a4), r, a3), r, a2), r, a), r, 1.0);
     const double v = table[n & (kTable - 1)] * p;
-    const double scaled = __hiloint2double(__double2hiint(v) + (((n >> 6) + q) << 20), __double2loint(v));
+    const double scaled = __hiloint2double(__double2hiint(v) + (((n >> 6) + q + lift) << 20), __double2loint(v));
     return (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
   }
   template <typename W>
   __device__ __forceinline__ u64 of(W v, W best) const {   // v is no NaN
-    return v == best ? one() : mass((double)v - (double)best);
+    return v == best ? one() : power(((double)v - (double)best) * c, 0);
+  }
+  // 2^lift times the weight where that is less than the largest, else as much as the largest
+  template <typename W>
+  __device__ __forceinline__ u64 lifted(W v, W best, int lift) const {
+    const double x = ((double)v - (double)best) * c;
+    return v == best || x >= -(double)kTable * lift ? one() : power(x, lift);
+  }
+  // Whether a weight reaches min_p, however small: compared where min_p lies from 1/2 to 1
+  template <typename W>
+  __device__ __forceinline__ bool reaches(W v, W best, double min_p) const {
+    if (!(min_p > 0)) return true;
+    const int lift = max(0, 1022 - (__double2hiint(min_p) >> 20));
+    return lifted(v, best, lift) >= (u64)__double2ll_rn(fmin(ldexp(min_p, lift), 1.0) * (double)one());
+  }
+};
+
+// A small random number may fall to units whose weights are nothing, or a few multiples of 2^-q, beside the largest.  The draw is then
+// made by weights multiplied by 2^lift and cut off at 2^q, where what is looked for, the random number times the sum of the kept
+// weights, lies from 2^(q-1) to 2^q: sums up to it are exact to n 2^-q of it, and a weight that is cut off passes it by itself.
+// For 0 (and what is below, and NaN) it is the first unit whose weight is above 0 in 64 bits.
+// Small is below 2^-20: other numbers pass what weights below 2^-q may add up to, and so few draws are small that the microseconds
+// they take longer are hardly met (with 2^-12, 40960 groups of 256 float32 units took 55 us and not 53).  They have functions of their
+// own, which take few registers from the others.
+__device__ __forceinline__ bool is_small(float random) { return !(random >= 1.f / (1 << 20)); }
+struct Lift {
+  int lift;
+  u64 target;   // what is looked for
+  __device__ __forceinline__ Lift(float random, u64 total, int q) {
+    const double at = (double)random * (double)total;
+    lift = at > 0 ? max(0, q - 1 - ((__double2hiint(at) >> 20) - 1023)) : 1074 - q;   // (0: of very many weights; less than their sum)
+    target = at > 0 ? (u64)ldexp(at, lift) : 0;
   }
 };
 
@@ -307,6 +338,45 @@ __device__ __forceinline__ void load_units(const T *x, unsigned n, bool whole, T
   }
 }
 
+// The unit drawn of those that are kept, for a small random number.
+template <typename T, int EACH>
+__device__ __noinline__ int draw_small(const T *x, unsigned n, bool whole, double inv_t, double min_p, float random, const double *table,
+                                       typename Keys<Wide<T>>::type top, typename Keys<Wide<T>>::type cut_key, unsigned cut_index) {
+  using W = Wide<T>;
+  using Key = typename Keys<W>::type;
+  const unsigned lane = threadIdx.x & 31;
+  const Weights weights(table, inv_t, kWarpBits);
+  const W best = Keys<W>::value(top);
+  const Cut<Key> cut{cut_key, cut_index, 0};
+  T raw[EACH];
+  load_units<T, EACH>(x, n, whole, raw);
+  u64 total = 0, mass[EACH];
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    const W v = no_nan(widen(raw[r]));
+    const bool in = kept(Keys<W>::of(v), lane * EACH + r, cut) && weights.reaches(v, best, min_p);
+    if (!in) raw[r] = narrow_to<T>((W)-INFINITY);
+    total += in ? weights.lifted(v, best, 0) : 0;
+  }
+  const Lift small(random, warp_sum_54(total), kWarpBits);
+  total = 0;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    mass[r] = weights.lifted(no_nan(widen(raw[r])), best, small.lift);   // (0 at -infinity)
+    total += mass[r];
+  }
+  const u64 up_to = warp_up_to(total);
+  const unsigned who = __ffs(__ballot_sync(0xffffffffu, up_to > small.target)) - 1;
+  u64 run = up_to - total;
+  unsigned index = lane * EACH;
+#pragma unroll
+  for (int r = 0; r < EACH; ++r) {
+    run += mass[r];
+    index += run <= small.target;
+  }
+  return (int)__shfl_sync(0xffffffffu, index, who);
+}
+
 // The unit drawn from one group, or -1; the same for all lanes.
 template <typename T, int EACH>
 __device__ __noinline__ int draw_exactly(const T *x, unsigned n, bool whole, const Settings &set, float random, const double *table,
@@ -350,6 +420,7 @@ __device__ __noinline__ int draw_exactly(const T *x, unsigned n, bool whole, con
     const Want want = want_mass(set.top_p, cut.mass);
     cut = group.cut(want, want.limit > 0 && want.limit < cut.mass ? (cut.mass - want.limit) / n : 0, top, few);
   }
+  if (is_small(random)) return draw_small<T, EACH>(x, n, whole, set.inv_t, set.min_p, random, table, top, cut.key, cut.index);
   if (set.min_p > 0) {
     const u64 least = (u64)__double2ll_rn(fmin(set.min_p, 1.0) * (double)weights.one());
 #pragma unroll
@@ -1032,7 +1103,16 @@ struct Part : Shape<THREADS> {
     }
     if (set.top_p < 1) keep = keep && want_mass(set.top_p, total).inside(r.rank, r.before);
     keep = keep && r.mass >= least;   // (the largest have 2^q, which is no less)
-    const u64 mass = keep ? r.mass : 0, target = target_of(random, block_sum(mass, s.sum));
+    u64 mass = keep ? r.mass : 0, target = block_sum(mass, s.sum);
+    if (is_small(random)) {
+      const W v = Keys<W>::value(r.key);
+      keep = keep && weights.reaches(v, best, set.min_p);
+      const Lift small(random, block_sum(keep ? r.mass : 0, s.sum), weights.q);
+      mass = keep ? weights.lifted(v, best, small.lift) : 0;
+      target = small.target;
+    } else {
+      target = target_of(random, target);
+    }
     unsigned equal, at = 0;
     if (threadIdx.x < count) {
       at = count_of<false>(s.list_index, count, r.index, equal);
@@ -1240,6 +1320,27 @@ struct Part : Shape<THREADS> {
   }
 };
 
+// Part::locate of the units that are kept, for a small random number.
+template <typename T, bool STAGED, int THREADS>
+__device__ __noinline__ void locate_small(const Vec<T, 16 / (int)sizeof(T)> *x, unsigned begin, unsigned size, unsigned lead, unsigned vectors,
+                                          Block<THREADS> &s, int turn, Wide<T> best, double inv_t, int q, double min_p, float random,
+                                          typename Keys<Wide<T>>::type cut_key, unsigned cut_index) {
+  using W = Wide<T>;
+  Part<T, STAGED, THREADS> p(x, begin, size, lead, vectors, s, cg::this_cluster());
+  p.best = best;
+  p.turn = turn;
+  const Weights weights(s.table, inv_t, q);
+  const W value = cut_key ? Keys<W>::value(cut_key) : (W)-INFINITY;
+  auto weigh = [&](W v, unsigned i, int lift) -> u64 {
+    const bool in = (v > value || (v == value && i <= cut_index)) && weights.reaches(v, best, min_p);
+    return in ? weights.lifted(v, best, lift) : 0;
+  };
+  u64 total = 0;
+  p.each([&](W v, unsigned i) { total += weigh(v, i, 0); });
+  const Lift small(random, p.cluster_sum(p.block_sum(total, s.sum)), q);
+  p.locate(value, [&](W v, unsigned i) { return weigh(v, i, small.lift); }, [&](u64) { return small.target; });
+}
+
 // Few groups are bound by latency, the barriers of a block and its cluster: one of 32000 float16 units, top-k 50 and top-p 0.9, 12 us.
 // Many by instructions on every unit: 256 x 128000 bf16 with a top-k of 100 33 us (greedy 14, the support at the copy bandwidth 10), with
 // settings of each row, some without a top-k, 113.
@@ -1366,14 +1467,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       }
     }
     const W value = cut.key ? Keys<W>::value(cut.key) : (W)-INFINITY;
-    p.locate(
-        value,
-        [&](W v, unsigned i) -> u64 {
-          if (!(v > value || (v == value && i <= cut.index))) return 0;
-          const u64 m = weights.of(v, best);
-          return m >= least ? m : 0;
-        },
-        [&](u64 total) { return target_of(random[g], total); });
+    if (is_small(random[g]))
+      locate_small<T, STAGED, THREADS>(p.x, begin, size, lead, vectors, s, p.turn, best, set.inv_t, q, set.min_p, random[g], cut.key, cut.index);
+    else
+      p.locate(
+          value,
+          [&](W v, unsigned i) -> u64 {
+            if (!(v > value || (v == value && i <= cut.index))) return 0;
+            const u64 m = weights.of(v, best);
+            return m >= least ? m : 0;
+          },
+          [&](u64 total) { return target_of(random[g], total); });
   }
   cluster.sync();
   if (rank == 0 && threadIdx.x == 0) codes[g] = base + (long long)s.unit;

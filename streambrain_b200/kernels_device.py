@@ -131,7 +131,8 @@ def sample_minicolumns(support, hypercolumns, minicolumns, random, temperature=1
     ``w_i = exp((x_i - max) / temperature)`` and units in order of falling ``w`` (equal ones by index), the first ``top_k``
     are kept (all with 0), of these the shortest beginning whose sum reaches ``top_p`` times their sum (at least one), of
     these the ones with ``w_i >= min_p`` (at least the largest); the unit drawn is the first in index order at which the
-    running sum of the kept ``w`` passes ``random`` times their sum.  ``temperature`` 0 takes the largest, the first of
+    running sum of the kept ``w`` passes ``random`` times their sum (with ``random`` 0 the first kept unit whose ``w`` is above 0
+    in 64 bits, however small).  ``temperature`` 0 takes the largest, the first of
     equal ones.  NaN counts as -infinity.  Each setting is a number (rounded to float32) or a CUDA tensor with a value per row
     (``top_k`` int32, the others float32; values out of range act as the nearest in range)."""
     support = _dense(support, "support", 2, _DTYPES)

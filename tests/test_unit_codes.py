@@ -422,6 +422,34 @@ def test_sample_random_numbers_out_of_range(mc):
         assert int(k().sample_minicolumns(x, 1, mc, torch.tensor([[u]], device="cuda"))) == want
 
 
+def small_numbers(shape, seed):
+    """Random numbers spread over the logarithm of what float32 holds above 0, and zeros."""
+    rng = np.random.default_rng(seed)
+    u = np.float32(2.0) ** rng.uniform(-149, 0, shape).astype(np.float32)
+    u[rng.random(shape) < 0.25] = 0
+    return torch.from_numpy(u.astype(np.float32).clip(0, np.nextafter(np.float32(1), np.float32(0))))
+
+
+@gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("rows,h,mc", [(40, 3, 2), (40, 3, 40), (40, 2, 300), (30, 1, 700), (30, 1, 3001), (20, 1, 20011), (160, 1, 2049), (600, 1, 1500)])
+def test_sample_small_random_numbers(rows, h, mc, t):
+    """A small random number falls to the units in front, however little they weigh: weights down to e^-700 of the largest, and some
+    that are 0 in 64 bits.  (The plain form's running sums from the front are exact to n 2^-53 of themselves.)"""
+    x = values((rows, h, mc), t, 61, 2.0)
+    rng = np.random.default_rng(62)
+    below = torch.from_numpy(rng.choice([0.0, 15, 30, 60, 100, 250, 700, 1500], (rows, h, 1)))
+    first = torch.from_numpy(rng.integers(1, mc, (rows, h, 1)))
+    x = torch.where(torch.arange(mc) < first, (x.double() - below).to(t), x).reshape(rows, h * mc)
+    u = small_numbers((rows, h), 63)
+    for how in (dict(), dict(top_k=mc // 2 + 1), dict(top_k=mc), dict(min_p=1e-20), dict(temperature=0.5, min_p=1e-12), dict(top_k=3, top_p=0.9),
+                dict(top_p=0.99), dict(temperature=7.0, top_k=300)):
+        how = {**dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **how}
+        got = k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), **how).cpu()
+        assert torch.equal(got, plain_sample_fast(x, h, mc, u, **how)), how
+    assert int(k().sample_minicolumns(torch.tensor([[-60.0, 0.0]], dtype=t).cuda(), 1, 2, torch.zeros((1, 1)).cuda())) == 0
+
+
 def offset(a):
     """The same values one element behind a boundary of 16 bytes and more."""
     b = torch.empty(a.numel() + 1, dtype=a.dtype, device="cuda")[1:].view(a.shape)
