@@ -420,6 +420,11 @@ __global__ void __launch_bounds__(kClusterThreads, 1)
   cluster_sort<I, EACH>(cg::this_cluster(), s, s_space, codes, entries, L, N, passes, digit_bits, result);
 }
 
+// Entries of a span, whose keys and rows (and a key at either end) lie in shared memory beside two parts for every thread: 48 KB in
+// all, which a block has without asking.
+constexpr size_t kPartMost = 32;   // bytes of a part
+constexpr unsigned kSpanMost = ((48 * 1024 - 2 * kThreads * kPartMost) / sizeof(unsigned) - 2) / 2;
+
 template <typename T, int V>
 struct Sums {
   const T *grad;
@@ -452,6 +457,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kThreads, 4) sums_kernel(const Sums<T, V> p) {
   after_previous();
   using W = Wide<T>;
+  static_assert(sizeof(Vec<W, V>) <= kPartMost, "kSpanMost");
   __shared__ Vec<W, V> s_head[kThreads], s_tail[kThreads];
   // the block's sorted entries, with one more at either end
   extern __shared__ unsigned s_entry[];
@@ -689,10 +695,10 @@ GradientPlan gradient_plan(long rows, long L, long N, long M, int vec) {
   p.lanes = 4;
   while (p.lanes < 32 && p.lanes < across) p.lanes *= 2;
   p.tiles = (unsigned)((across + p.lanes - 1) / p.lanes);
-  // as many chunks as keep all threads busy, of 8 to 64 entries
-  const long want = 2048l * sm_count() / p.lanes;
+  // as many chunks as keep all threads busy, of 8 to 64 entries (56 where a block has 64 groups: kSpanMost)
+  const long want = 2048l * sm_count() / p.lanes, fits = kSpanMost / (kThreads / p.lanes) / 8 * 8, most = fits < 64 ? fits : 64;
   long chunk = (long)p.entries * p.tiles / want / 8 * 8;
-  chunk = chunk < 8 ? 8 : chunk > 64 ? 64 : chunk;
+  chunk = chunk < 8 ? 8 : chunk > most ? most : chunk;
   p.chunk = (unsigned)chunk;
   p.span = p.chunk * (kThreads / p.lanes);
   p.spans = (p.entries + p.span - 1) / p.span;

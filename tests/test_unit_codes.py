@@ -221,6 +221,32 @@ def test_lookup_gradient(rows, length, n, m, kind, scale, t):
     assert torch.equal(out.cpu()[~named], old[~named])
 
 
+def gradient_by_torch(grad, codes, n):
+    """(result, sum of magnitudes, number of terms of the fullest row) in 64 bits, on the tensors' device."""
+    c = codes.long().reshape(-1)
+    row = torch.arange(c.numel(), device=c.device) // codes.shape[1]
+    keep = (c >= 0) & (c < n)
+    c, row = c[keep], row[keep]
+    out = torch.zeros((n, grad.shape[1]), dtype=F64, device=grad.device)
+    size = torch.zeros_like(out)
+    for lo in range(0, c.numel(), 1 << 20):
+        g = grad.double()[row[lo:lo + (1 << 20)]]
+        out.index_add_(0, c[lo:lo + (1 << 20)], g)
+        size.index_add_(0, c[lo:lo + (1 << 20)], g.abs())
+    return out, size, int(torch.bincount(c, minlength=n).max())
+
+
+@gpu
+@pytest.mark.parametrize("t,m", [(F16, 8), (BF16, 16), (BF16, 32), (F32, 16), (F64, 8), (BF16, 3)])
+def test_lookup_gradient_of_millions_of_codes(t, m):
+    """The longest chunks, in the narrowest rows: four lanes to a chunk, 64 chunks to a block."""
+    rows, length, n = 8192, 600, 90001
+    g, c = values((rows, m), t, 71).cuda(), codes_of("few", rows, length, n, 72, torch.int32).cuda()
+    want, size, most = gradient_by_torch(g, c, n)
+    got = k().lookup_gradient(g, c, n)
+    assert_close(got, want.cpu(), ((most + 2) * wide_half_step(t) * size + rounding(t, want)).cpu())
+
+
 @gpu
 def test_lookup_gradient_against_differences():
     """The derivative of a weighted sum of lookups, by central differences in float64: the operator is linear, so they are
