@@ -511,7 +511,9 @@ int sbb_sample_minicolumns(int dtype, const void *support_dev, const float *rand
  * the hypercolumn (unit_bytes: 4 or 8); entries outside [0, Mc) are absent, a unit named twice has both parts.
  * teacher[rows, H, K] is of the support's type; loss and weight (null: 1) are float, double for SBB_F64.
  * temperature: from 1e-15 to 1e15.  gradient may be null: the loss alone.  Where the weight is 0, where no unit is kept,
- * or where a hypercolumn's support (or the teacher's) is -infinity throughout, both are exactly 0. */
+ * or where a hypercolumn's support (or the teacher's) is -infinity throughout, both are exactly 0.  Elsewhere NaN or
+ * +infinity in a hypercolumn's support makes its loss and all of its gradient NaN; among the teacher's, the loss and
+ * the gradient of the units that it keeps. */
 int sbb_distill(int dtype, const void *support_dev, const void *teacher_units_dev, int unit_bytes,
                 const void *teacher_dev, const void *weight_dev, long rows, long H, long Mc, long K,
                 double temperature, void *loss_dev, void *gradient_dev, void *stream);

@@ -303,7 +303,7 @@ struct Running {
   }
   __device__ __forceinline__ void add(W v, W c) {
     if (v > best) move_to(v, c);
-    sum += v == best && v != -INFINITY ? (W)1 : v == -INFINITY ? (W)0 : expo(v - (best == -INFINITY ? (W)0 : best), c);
+    sum += v == -INFINITY ? (W)0 : v == best && v < (W)INFINITY ? (W)1 : expo(v - (best == -INFINITY ? (W)0 : best), c);   // (+infinity: NaN)
   }
 };
 

@@ -605,6 +605,28 @@ def test_distill_masks(mc, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("mc,kept", [(6, 2), (100, 3), (333, 40), (700, 4), (1025, 4), (9001, 600), (30001, 4)])
+def test_distill_with_infinity(mc, kept, t):
+    """exp(infinity - infinity) is not a number, and so is what is divided by it, wherever in the hypercolumn the infinity stands and
+    wherever the tensor begins.  A teacher's reaches the loss and the units that it keeps."""
+    x = values((5, mc), t, 81, 2.0)
+    units, teacher = teacher_of(x, 1, mc, kept, 82)
+    for j, at in enumerate((0, mc // 2, mc - 1)):
+        x[j, at] = math.inf
+    teacher[3, 0, kept // 2] = math.inf
+    for place in (lambda a: a.cuda(), offset):
+        loss, gradient = k().distill_gradient(place(x), 1, mc, units.cuda(), teacher.cuda(), 2.0)
+        assert torch.equal(torch.isnan(loss.cpu()[:, 0]), torch.tensor([True, True, True, True, False]))
+        named = torch.zeros(mc, dtype=torch.bool)
+        named[units[3, 0]] = True
+        gradient = gradient.cpu()
+        assert bool(torch.isnan(gradient[:3]).all()) and torch.equal(torch.isnan(gradient[3]), named) and not torch.isnan(gradient[4]).any()
+        again = k().distill_loss(place(x), 1, mc, units.cuda(), teacher.cuda(), 2.0)
+        assert torch.equal(torch.isnan(again), torch.isnan(loss))
+
+
+@gpu
 def test_distill_gradient_against_differences():
     """Central differences in float64 with steps of 1e-4: the loss's third derivative is below its temperature-scaled size of
     one, so they are off by at most 1e-8 and by 1e-16 / 1e-4 for the roundings."""
