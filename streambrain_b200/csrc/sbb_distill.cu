@@ -187,13 +187,15 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 80 ? 3 : 2
     }
     bool nothing = w == (W)0 || best == -INFINITY || tbest == -INFINITY;
     if (nothing && w != (W)0) {   // (the maxima pass over NaN, which is not nothing)
-      bool nan = u0 < p.n && t0 != t0;
+      bool nan = false, teacher_nan = u0 < p.n && t0 != t0;
 #pragma unroll
       for (int r = 0; r < NV; ++r)
 #pragma unroll
         for (int v = 0; v < V; ++v) nan = nan || e[r][v] != e[r][v];
-      for (unsigned k = lane + LANES; k < p.K; k += LANES) nan = nan || (p.unit(g, k) < p.n && isnan(widen(p.teacher[(long)g * p.K + k])));
-      nothing = !__any_sync(mask, nan);
+      for (unsigned k = lane + LANES; k < p.K; k += LANES)
+        teacher_nan = teacher_nan || (p.unit(g, k) < p.n && isnan(widen(p.teacher[(long)g * p.K + k])));
+      const bool student = best != -INFINITY || __any_sync(mask, nan), teacher = tbest != -INFINITY || __any_sync(mask, teacher_nan);
+      nothing = !student || !teacher;
     }
     if (nothing) {
       if (lane == 0) p.loss[g] = 0;

@@ -627,6 +627,26 @@ def test_distill_with_infinity(mc, kept, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("mc", [6, 100, 512, 700, 9000])
+def test_distill_where_nothing_is_kept_beside_a_nan(mc, t):
+    """Exactly 0 where the teacher keeps nothing or the student rules all out, whatever the other holds."""
+    x = values((5, mc), t, 91, 2.0)
+    units, teacher = teacher_of(x, 1, mc, 3, 92)
+    x[0, mc // 2] = math.nan
+    units[0] = -1
+    x[1, 0] = math.nan
+    teacher[1] = -math.inf
+    x[2] = -math.inf
+    teacher[2, 0, 1] = math.nan
+    x[3, mc - 1] = math.inf
+    teacher[3] = -math.inf
+    loss, gradient = k().distill_gradient(x.cuda(), 1, mc, units.cuda(), teacher.cuda(), 2.0)
+    assert bool((loss[:4] == 0).all()) and bool((gradient[:4] == 0).all()) and float(loss[4]) > 0
+    assert torch.equal(loss, k().distill_loss(x.cuda(), 1, mc, units.cuda(), teacher.cuda(), 2.0))
+
+
+@gpu
 def test_distill_gradient_against_differences():
     """Central differences in float64 with steps of 1e-4: the loss's third derivative is below its temperature-scaled size of
     one, so they are off by at most 1e-8 and by 1e-16 / 1e-4 for the roundings."""
