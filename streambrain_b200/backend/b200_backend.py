@@ -143,6 +143,10 @@ class _DeviceLayer:
             raise TypeError("torch inputs must be CUDA tensors (pass numpy arrays for host data)")
         if codes.dim() != 2:
             raise TypeError("expected a [B, L] tensor of codes")
+        # (the C entry refuses a layer that is not on the current device)
+        here = _current_device() if _current_device is not None else torch.cuda.current_device()
+        if codes.get_device() != here:
+            raise ValueError("codes are on cuda:%d, not on the layer's cuda:%d" % (codes.get_device(), here))
         c = codes if codes.is_contiguous() else codes.contiguous()
         y = torch.empty((c.shape[0], self.out_features), dtype=self._tdtype, device=c.device)
         check(lib.sbb_layer_forward_codes(self._handle, c.data_ptr(), c.element_size(), c.shape[0], c.shape[1], softmax,

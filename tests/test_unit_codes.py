@@ -812,6 +812,46 @@ def test_layers_take_codes(n, h, mc, dtype):
 
 # ---- refusals (no device needed) -------------------------------------------
 
+class _Codes:
+    """What a layer asks of a tensor of codes on CUDA device ``device``, without the device."""
+    is_cuda, dtype, shape = True, torch.int64, (2, 3)
+
+    def __init__(self, device):
+        self.device, self._number = torch.device("cpu"), device
+
+    def dim(self):
+        return 2
+
+    def get_device(self):
+        return self._number
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return 4096
+
+    def element_size(self):
+        return 8
+
+
+def test_layers_refuse_codes_of_another_device(monkeypatch):
+    from types import SimpleNamespace
+
+    from streambrain_b200.backend import b200_backend as b
+    layer = b.DenseLayer.__new__(b.DenseLayer)
+    layer.out_features, layer._tdtype, layer._handle, layer.hypercolumns, layer.minicolumns = 4, F32, None, 2, 2
+    calls = []
+    monkeypatch.setattr(b, "_current_device", lambda: 1)
+    monkeypatch.setattr(b, "_stream_ptr", lambda: 0)
+    monkeypatch.setattr(b, "lib", SimpleNamespace(sbb_layer_forward_codes=lambda *a: calls.append(a) or 0))
+    for call in (lambda c: layer._forward_codes(c, 1), lambda c: layer.sample_units(c, None)):
+        with pytest.raises(ValueError):
+            call(_Codes(0))
+    assert not calls
+    assert layer._forward_codes(_Codes(1), 1).shape == (2, 4) and len(calls) == 1
+
+
 def test_wrappers_refuse_host_tensors_and_wrong_types():
     pytest.importorskip("streambrain_b200.kernels_device")
     w, c = torch.zeros((4, 3)), torch.zeros((2, 1), dtype=torch.int64)
