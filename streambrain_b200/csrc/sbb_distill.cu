@@ -114,7 +114,7 @@ __device__ __forceinline__ W warp_sum(W v) {
 }
 __device__ __forceinline__ float warp_max(float v) {
   float m;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
 }
 __device__ __forceinline__ double warp_max(double v) {

@@ -450,7 +450,7 @@ __device__ __noinline__ int draw_exactly(const T *x, unsigned n, bool whole, con
 // made again in 64 bits.  With 100 units that is one draw in some thousands; the others cost a third of the instructions.
 __device__ __forceinline__ float warp_max(float v) {
   float m;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
 }
 __device__ __forceinline__ float warp_min(float v) { return -warp_max(-v); }

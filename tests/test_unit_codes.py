@@ -900,6 +900,17 @@ def test_wrappers_refuse():
             pytest.fail("call %d went through" % j)
 
 
+def test_warp_collectives_stay_where_they_are():
+    """An asm statement that is not volatile may be moved into a branch that not all lanes take; one that waits for all of them may not."""
+    import pathlib
+    import re
+    sources = [f for f in (pathlib.Path(_lib.__file__).parent / "csrc").iterdir() if f.suffix in (".cu", ".cuh", ".h")]
+    assert sources
+    for f in sources:
+        for m in re.finditer(r"\basm\s*(volatile)?\s*\(\s*\"([^\"]*)", f.read_text()):
+            assert m.group(1) or not re.search(r"\b(redux|shfl|vote|match|bar|barrier|activemask)\.", m.group(2)), (f.name, m.group(2))
+
+
 def test_entries_refuse_before_any_device_work():
     at, big = ctypes.c_void_p(4096), 1 << 40
     how = _lib.Sampling(1.0, 1.0, 0.0, 0)
