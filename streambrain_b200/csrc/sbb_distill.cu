@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kWarpThreads, sizeof(T) * V * NV <= 80 ? 3 : 2
 
 constexpr int kMostBlocks = 8;
 constexpr int kStage = 100 * 1024;   // bytes of a group that a block keeps in shared memory
-// Threads of a block: as many kept units wait in shared memory; those of longer lists are read again.  Groups of up to 8192 units go to
+// Threads of a block: as many kept units wait in shared memory; longer lists are read again, as many at a time.  Groups of up to 8192 units go to
 // small blocks: 16000 groups of 520 float32 units take 55 us, and took 151 in large ones; 4000 of 6000 units 47 and 57.
 constexpr int kLarge = 512, kSmall = 128;
 constexpr unsigned kSmallMost = 8192;
@@ -335,15 +335,16 @@ __device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Bl
 }
 
 // STAGED: the part waits in shared memory between the sum and the gradient; else (no gradient, or groups beyond what a cluster
-// holds) it is read again.  VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last
+// holds) it is read again.  LONG: there is a gradient and a list of more entries than threads; `room` units' parts of it fit the shared
+// memory.  (Within the kernel for short lists, 512 x 50001 float16 took 34.5 us and not 33, without a gradient 20 and not 18.5.)  VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last
 // one by single threads; else (support and gradient lie differently to the boundaries) element by element.
 // Instructions, and phases that do not overlap within a block, bound it: 4096 x 32000 bf16 units, 64 kept, 114 us, 71 % of the issue slots
 // busy, 0.70 of a plain copy's bandwidth.
-template <typename T, bool VECTOR, bool STAGED, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(const Distill<T> p, unsigned part) {
+template <typename T, bool VECTOR, bool STAGED, int THREADS, bool LONG>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(const Distill<T> p, unsigned part, unsigned room) {
   after_previous();
   using W = Wide<T>;
-  constexpr unsigned kThreads = THREADS, kBlockWarps = THREADS / 32, kEntries = THREADS;
+  constexpr unsigned kThreads = THREADS, kBlockWarps = THREADS / 32;
   constexpr int V = VECTOR ? 16 / (int)sizeof(T) : 1;
   extern __shared__ uint4 s_values[];
   __shared__ Block<W, THREADS> s;
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(
   }
   const W inv = (W)1 / p.temperature, shift = sbb_log(r.sum) - sbb_log(t.sum), wt = w * p.temperature, scale = wt / r.sum, share = (W)1 / t.sum;
   auto p_of = [&](W v) { return expo(v - t.best, p.c) * share; };
-  const bool listed = p.K <= kEntries;
+  const bool listed = !LONG && p.K <= kThreads;
   {
     W sum = 0;
     for (unsigned k = threadIdx.x; k < p.K; k += kThreads) {
@@ -458,25 +459,17 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(
     bool first = true;
     sum = 0;
     for (unsigned j = 0; j < p.K; ++j) {
-      unsigned o;
-      W pj;
-      if (listed) {
-        const Vec<W, 2> e = s.kept[j];
-        o = *reinterpret_cast<const unsigned *>(&e.v[0]);
-        pj = e.v[1];
-      } else {
-        o = p.unit(g, j);
-        pj = o == u ? p_of(widen(p.teacher[(long)g * p.K + j])) : (W)0;
-      }
+      const Vec<W, 2> e = s.kept[j];
+      const unsigned o = *reinterpret_cast<const unsigned *>(&e.v[0]);
       if (o == u) {
         first = first && j >= k;
-        sum += pj;
+        sum += e.v[1];
       }
     }
     return first;
   };
   W sum0 = 0;
-  const bool mine = u0 >= begin && u0 < begin + size && given(threadIdx.x, u0, sum0);
+  const bool mine = !LONG && u0 >= begin && u0 < begin + size && given(threadIdx.x, u0, sum0);
   for (unsigned i = threadIdx.x; i < vectors; i += kThreads) {
     W f[V];
     widen_all(STAGED ? stage[i] : from[i], f);
@@ -487,11 +480,41 @@ __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(
   if (single < size) out[single] = narrow_to<T>(expo(own - r.best, p.c) * scale);
   __syncthreads();   // the kept units' elements are written again
   if (mine) out[u0 - begin] = narrow_to<T>(expo(x0 - r.best, p.c) * scale - wt * sum0);
-  for (unsigned k = threadIdx.x + kThreads; k < p.K; k += kThreads) {
-    const unsigned u = p.unit(g, k);
-    W sum;
-    if (u >= begin && u < begin + size && given(k, u, sum))
-      out[u - begin] = narrow_to<T>(expo(widen(p.support[(long)g * p.n + u]) - r.best, p.c) * scale - wt * sum);
+  if constexpr (!LONG) return;
+  // A long list: what the teacher gives `room` units at a time is added up in shared memory, kThreads entries at a time.  (Comparing every
+  // entry with all others took the square of their number.)
+  W *const parts = reinterpret_cast<W *>(s_values);
+  for (unsigned lo = 0; lo < size; lo += room) {
+    const unsigned here = min(room, size - lo);
+    for (unsigned i = threadIdx.x; i < here; i += kThreads) parts[i] = 0;
+    __syncthreads();
+    for (unsigned k0 = 0; k0 < p.K; k0 += kThreads) {
+      const unsigned k = k0 + threadIdx.x, u = k < p.K ? p.unit(g, k) : p.n, at = u - begin - lo;   // (wraps for units in front)
+      const bool there = u < p.n && at < here;
+      W sum = there ? p_of(widen(p.teacher[(long)g * p.K + k])) : (W)0;
+      s.kept[threadIdx.x].v[1] = sum;
+      *reinterpret_cast<unsigned *>(&s.kept[threadIdx.x].v[0]) = there ? at : ~0u;
+      const W before = there ? parts[at] : (W)0;
+      __syncthreads();
+      // Whoever reads another's mark than its own shares its unit: the parts in the order of the entries then.
+      if (there) parts[at] = (W)threadIdx.x;
+      __syncthreads();
+      const bool shared = there && parts[at] != (W)threadIdx.x;
+      if (__syncthreads_or(shared) && there) {
+        sum = 0;
+        for (unsigned j = 0; j < kThreads; ++j) {
+          const Vec<W, 2> e = s.kept[j];
+          if (*reinterpret_cast<const unsigned *>(&e.v[0]) == at) sum += e.v[1];
+        }
+      }
+      if (there) parts[at] = before + sum;   // (those that name the same unit write the same)
+      __syncthreads();
+    }
+    for (unsigned i = threadIdx.x; i < here; i += kThreads) {
+      const W given = parts[i];
+      if (given != (W)0) out[lo + i] = narrow_to<T>(expo(widen(x[lo + i]) - r.best, p.c) * scale - wt * given);
+    }
+    __syncthreads();
   }
 }
 
@@ -502,14 +525,21 @@ cudaError_t launch_warps(const Distill<T> &p, cudaStream_t st) {
   return launch_next(distill_warp_kernel<T, V, NV, LANES>, dim3(blocks < most ? blocks : most), kWarpThreads, 0, st, p);
 }
 
-template <typename T, bool VECTOR, bool STAGED, int THREADS>
+template <typename T, bool VECTOR, bool STAGED, int THREADS, bool LONG = false>
 cudaError_t launch_blocks(const Distill<T> &p, unsigned part, unsigned cluster, cudaStream_t st) {
-  const size_t smem = STAGED ? (size_t)part * sizeof(T) : 0;
+  size_t smem = STAGED ? (size_t)part * sizeof(T) : 0;
+  unsigned room = 0;
+  if constexpr (LONG) {
+    constexpr unsigned most = kStage / sizeof(Wide<T>);
+    room = part < most ? part : most;
+    if (smem < room * sizeof(Wide<T>)) smem = room * sizeof(Wide<T>);
+  }
+  auto kernel = distill_block_kernel<T, VECTOR, STAGED, THREADS, LONG>;
   if (smem > 0) {   // (holds for the current device)
-    const cudaError_t e = cudaFuncSetAttribute(distill_block_kernel<T, VECTOR, STAGED, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kStage);
     if (e != cudaSuccess) return e;
   }
-  return launch_clusters(distill_block_kernel<T, VECTOR, STAGED, THREADS>, dim3(p.groups * cluster), dim3(cluster), THREADS, smem, st, p, part);
+  return launch_clusters(kernel, dim3(p.groups * cluster), dim3(cluster), THREADS, smem, st, p, part, room);
 }
 
 template <typename T>
@@ -524,6 +554,11 @@ cudaError_t launch_wide(const Distill<T> &p, cudaStream_t st) {
   if ((size_t)p.groups * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const bool staged = p.gradient && (size_t)part * sizeof(T) <= kStage;
   const bool vector = !p.gradient || ((reinterpret_cast<uintptr_t>(p.support) ^ reinterpret_cast<uintptr_t>(p.gradient)) & 15) == 0;
+  if (p.gradient && p.K > (p.n <= kSmallMost && cluster == 1 ? kSmall : kLarge)) {   // (groups for small blocks are staged)
+    if (!vector) return launch_blocks<T, false, false, kLarge, true>(p, part, cluster, st);
+    if (p.n <= kSmallMost && cluster == 1) return launch_blocks<T, true, true, kSmall, true>(p, part, 1, st);
+    return staged ? launch_blocks<T, true, true, kLarge, true>(p, part, cluster, st) : launch_blocks<T, true, false, kLarge, true>(p, part, cluster, st);
+  }
   if (p.n <= kSmallMost && cluster == 1) {
     if (vector) return staged ? launch_blocks<T, true, true, kSmall>(p, part, 1, st) : launch_blocks<T, true, false, kSmall>(p, part, 1, st);
     return staged ? launch_blocks<T, false, true, kSmall>(p, part, 1, st) : launch_blocks<T, false, false, kSmall>(p, part, 1, st);

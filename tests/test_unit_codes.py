@@ -561,6 +561,54 @@ def test_distill(rows, h, mc, kept, temperature, t):
         assert_close(k().distill_loss(*args), want, loss_off)
 
 
+def distill_by_torch(x, units, teacher, temperature):
+    """(loss, gradient, bound of the loss, bound of the gradient) of whole rows in 64 bits, as in :func:`plain_distill`; on the tensors' device.
+    Entries out of range are absent; no row is without one."""
+    u = wide_half_step(x.dtype)
+    mc, kept = x.shape[1], units.shape[1]
+    there = (units >= 0) & (units < mc)
+    named = torch.where(there, units, 0)
+    v, tv = x.double() / temperature, torch.where(there, teacher.double(), -math.inf) / temperature
+    log_q, log_p = torch.log_softmax(v, 1), torch.log_softmax(tv, 1)
+    p, of = log_p.exp(), log_q.gather(1, named)
+    pp = torch.zeros_like(v).scatter_add_(1, named, p)
+    span = max(float(v.max() - v.min()), float(tv[there].max() - tv[there].min()))
+    c = (6 * span + mc + kept + 40) * u
+    zero = torch.zeros_like(p)
+    loss = temperature ** 2 * torch.where(p > 0, p * (log_p - of), zero).sum(1)
+    loss_off = temperature ** 2 * torch.where(p > 0, p * (log_p.abs() + of.abs() + 1), zero).sum(1) * c
+    q = log_q.exp()
+    return loss, temperature * (q - pp), loss_off, temperature * (q + pp) * c + (1e-37 if x.dtype != F64 else 1e-300)
+
+
+@gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("rows,mc,kept,among", [(3, 600, 300000, 600), (2, 9001, 300000, 9001), (1, 60001, 300000, 60001), (2, 700, 300000, 3), (1, 700001, 5000, 700001),
+                                                 (2, 8192, 129, 8192), (2, 8193, 513, 100), (3, 513, 128, 513)])
+def test_distill_with_long_lists(rows, mc, kept, among, t):
+    """Lists of more entries than a block has threads, most units named many times, some entries absent; within a time that their square
+    would exceed by far (300000 entries in pieces of 128: 2344 x 300000 steps a thread)."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(kept + mc)
+    x = (torch.randn((rows, mc), generator=gen, device="cuda") * 2).to(t)
+    units = torch.randint(-among // 8 - 1, among + among // 8 + 1, (rows, kept), generator=gen, device="cuda")
+    units = torch.where(units < among, units, mc + units)   # (no unit from among on)
+    teacher = (torch.randn((rows, kept), generator=gen, device="cuda") * 2).to(t)
+    call = lambda: k().distill_gradient(x, 1, mc, units[:, None], teacher[:, None], 2.0)
+    call()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    loss, gradient = call()
+    end.record()
+    end.synchronize()
+    assert start.elapsed_time(end) < 300
+    want, grad, loss_off, grad_off = distill_by_torch(x, units, teacher, 2.0)
+    assert_close(loss[:, 0], want.cpu(), loss_off.cpu())
+    assert_close(gradient, grad.cpu(), (grad_off + rounding(t, grad)).cpu())
+    again, same = call()
+    assert torch.equal(loss, again) and torch.equal(gradient, same)
+
+
 @gpu
 @pytest.mark.parametrize("t", ALL)
 @pytest.mark.parametrize("mc", [6, 100, 700, 9000])
