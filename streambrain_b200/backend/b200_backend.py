@@ -117,12 +117,18 @@ class _DeviceLayer:
             self._handle = None
 
     # -- reference API ---------------------------------------------------
-    def compute_activation(self, inputs):
+    def compute_activation(self, inputs, codes=False):
         """softmax_minicolumns(inputs . weights + bias): _cpu_base_backend.py:44-51, 126-133.  An int32 or int64 CUDA
-        tensor [B, L] holds codes: the positions of each sample's active inputs (:mod:`streambrain_b200.kernels_device`)."""
+        tensor [B, L] holds codes: the positions of each sample's active inputs (:mod:`streambrain_b200.kernels_device`).
+        One of ``in_features`` columns may as well be dense rows of another dtype, and is refused unless ``codes`` is true."""
         if _is_tensor(inputs):
             if inputs.dtype in (torch.int32, torch.int64):
+                if not codes and inputs.dim() == 2 and inputs.shape[1] == self.in_features:
+                    raise TypeError("expected a [B, %d] %s tensor; integers are codes, a tensor of as many columns only with codes=True"
+                                    % (self.in_features, np.dtype(self.dtype)))
                 return self._forward_codes(inputs, 1)
+            if codes:
+                raise TypeError("codes must be an int32 or int64 tensor")
             x = self._dev_input(inputs, self.in_features)
             B = x.shape[0]
             y = x.new_empty((B, self.out_features))
@@ -130,6 +136,8 @@ class _DeviceLayer:
             if rc:
                 check(rc)
             return y
+        if codes:
+            raise TypeError("codes must be a CUDA tensor")
         B = inputs.shape[0]
         x = np.ascontiguousarray(inputs, dtype=self.dtype)
         if x.shape[1] != self.in_features:

@@ -948,6 +948,25 @@ def test_wrappers_refuse():
             pytest.fail("call %d went through" % j)
 
 
+def test_layers_refuse_dense_rows_of_integers(monkeypatch):
+    """An integer tensor of a dense row's shape is refused, as it was before layers took codes, unless it is said to hold codes."""
+    from streambrain_b200.backend import b200_backend as b
+    layer = b.DenseLayer.__new__(b.DenseLayer)
+    layer.in_features, layer._handle, layer.dtype, layer._tdtype, calls = 6, None, np.float32, F32, []
+    monkeypatch.setattr(layer, "_forward_codes", lambda c, softmax: calls.append(c.shape), raising=False)
+    for t in (torch.int32, torch.int64):
+        with pytest.raises(TypeError):
+            layer.compute_activation(torch.zeros((2, 6), dtype=t))
+    assert not calls
+    layer.compute_activation(torch.zeros((2, 6), dtype=torch.int64), codes=True)
+    layer.compute_activation(torch.zeros((2, 5), dtype=torch.int64))
+    layer.compute_activation(torch.zeros((2, 5), dtype=torch.int32), codes=True)
+    assert calls == [(2, 6), (2, 5), (2, 5)]
+    for other in (torch.zeros((2, 6)), np.zeros((2, 6), dtype=np.int64)):
+        with pytest.raises(TypeError):
+            layer.compute_activation(other, codes=True)
+
+
 def test_warp_collectives_stay_where_they_are():
     """An asm statement that is not volatile may be moved into a branch that not all lanes take; one that waits for all of them may not."""
     import pathlib
