@@ -581,10 +581,16 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
     total += g.w[r];
   }
   // A weight is off by 2^-22 of it (ex2.approx) and by 3 x 2^-24 = 1.8e-7 for every unit x of its exponent: x exp(-x) is below 0.37, so
-  // by less than 3.1e-7 of the largest weight, 1, and, where it counts at all (x < 40), by 7.4e-6 of itself.  The 21 roundings on
-  // the way through a sum (37 with 32 units a lane) are 1.3e-6 (2.2e-6) of it.  Two sums are compared, one of them times a rounded factor.
+  // by less than 3.1e-7 of the largest weight, 1, and, where it counts at all (x < 40), by 7.5e-6 of itself.  Two sums of them are
+  // compared.  Of their roundings, each 2^-24 of the sum of all at most:
+  //   a border of the last step, the sum in front of the lane and its units one by one: EACH - 1 in every lane, 5 over the lanes, 1 for
+  //   taking the lane's own out, EACH; against the random number's part of a sum: EACH - 1, 5, and 1 for the product;
+  //   a mass at a cut: EACH - 1 and 5 up to a round's bound, 5 in the list, 1 for adding the two, 1 for taking out its own; against the
+  //   limit: EACH - 1, 5, and 1 for the product.
+  constexpr int kBorder = (EACH - 1) + 5 + 1 + EACH + (EACH - 1) + 5 + 1, kCut = (EACH - 1) + 5 + 5 + 1 + 1 + (EACH - 1) + 5 + 1;
+  constexpr int kRoundings = kBorder > kCut ? kBorder : kCut;
   total = warp_sum(total);
-  g.error = 2 * fminf((EACH <= 16 ? 1.7e-6f : 2.8e-6f) * n, (EACH <= 16 ? 9e-6f : 1e-5f) * total) + 3e-7f * total;
+  g.error = 2 * fminf(3.1e-7f * n, 7.5e-6f * total) + (kRoundings + 1) * 6e-8f * total;   // (one more for the bound's own; 2^-24 is 5.97e-8)
   g.doubt = false;
   float value = -INFINITY, mass = total;
   unsigned index = n;

@@ -476,6 +476,28 @@ def test_sample_small_random_numbers(rows, h, mc, t):
     assert int(k().sample_minicolumns(torch.tensor([[-60.0, 0.0]], dtype=t).cuda(), 1, 2, torch.zeros((1, 1)).cuda())) == 0
 
 
+@gpu
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+@pytest.mark.parametrize("mc", [32, 61, 127, 256, 512, 1000, 1024])
+def test_sample_random_numbers_at_the_borders(mc, t):
+    """The floats around every border of two units (which sums in 32 bits do not tell apart), of nearly equal weights, so that
+    roundings add up, and of spread ones."""
+    for spread, top_p in ((0.0, 1.0), (1e-3, 1.0), (1.0, 1.0), (0.01, 0.7)):
+        x = values((1, mc), t, 65, spread)
+        w = torch.exp(x.double() - x.double().max())[0]
+        if top_p < 1:
+            order = torch.sort(w, descending=True, stable=True).indices
+            c = w[order].cumsum(0)
+            out = order[(c - w[order]) >= float(np.float32(top_p)) * c[-1]]
+            w[out] = 0
+        border = (w.cumsum(0) / w.sum()).numpy().astype(np.float32)
+        u = np.concatenate([border, np.nextafter(border, np.float32(0)), np.nextafter(border, np.float32(1))]).clip(0, np.nextafter(np.float32(1), np.float32(0)))
+        u = torch.from_numpy(u)[:, None]
+        rows = x.expand(u.shape[0], mc)
+        got = k().sample_minicolumns(rows.cuda(), 1, mc, u.cuda(), top_p=top_p).cpu()
+        assert torch.equal(got, plain_sample_fast(rows, 1, mc, u, 1.0, 0, top_p, 0.0)), spread
+
+
 def offset(a):
     """The same values one element behind a boundary of 16 bytes and more."""
     b = torch.empty(a.numel() + 1, dtype=a.dtype, device="cuda")[1:].view(a.shape)
