@@ -2,6 +2,7 @@
 #include "../../include/sbb200.h"
 #include "sbb_codes.cuh"
 
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -33,7 +34,7 @@ int fail(int code, const char *fmt, ...) {
   } while (0)
 
 int need_device() {
-  static bool found = false;   // (a device that is there stays)
+  static std::atomic<bool> found{false};   // (a device that is there stays)
   if (found) return SBB_OK;
   int n = 0;
   if (cudaGetDeviceCount(&n) != cudaSuccess) {

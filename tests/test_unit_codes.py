@@ -1000,6 +1000,20 @@ def test_warp_collectives_stay_where_they_are():
             assert m.group(1) or not re.search(r"\b(redux|shfl|vote|match|bar|barrier|activemask)\.", m.group(2)), (f.name, m.group(2))
 
 
+def test_entries_from_many_threads():
+    """(Without rows nothing is launched.)"""
+    from concurrent.futures import ThreadPoolExecutor
+    at, how = ctypes.c_void_p(4096), _lib.Sampling(1.0, 1.0, 0.0, 0)
+    want = 0 if lib.sbb_device_count() > 0 else _lib.ERR_NO_DEVICE
+
+    def calls(_):
+        return (lib.sbb_lookup(0, at, at, 8, 0, 1, 4, 3, 1.0, at, None), lib.sbb_sample_minicolumns(0, at, at, 0, 1, 3, ctypes.byref(how), at, None),
+                lib.sbb_distill(0, at, at, 8, at, None, 0, 1, 3, 1, 1.0, at, at, None), lib.sbb_lookup(7, at, at, 8, 0, 1, 4, 3, 1.0, at, None))
+
+    with ThreadPoolExecutor(16) as pool:
+        assert set(pool.map(calls, range(400))) == {(want, want, want, _lib.ERR_INVALID)}
+
+
 def test_entries_refuse_before_any_device_work():
     at, big = ctypes.c_void_p(4096), 1 << 40
     how = _lib.Sampling(1.0, 1.0, 0.0, 0)
