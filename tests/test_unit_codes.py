@@ -248,6 +248,39 @@ def test_lookup_gradient_of_millions_of_codes(t, m):
 
 
 @gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("kind", ["any", "few", "same", "absent"])
+def test_lookup_gradient_of_long_chunks(kind, t):
+    """Chunks of 16 to 64 entries (elsewhere they are of 8): some ten thousand codes of wide rows."""
+    rows, n, m = 20011, 3001, 2048
+    g, c = values((rows, m), t, 73).cuda(), codes_of(kind, rows, 1, n, 74, torch.int64).cuda()
+    want, size, most = gradient_by_torch(g, c, n)
+    got = k().lookup_gradient(g, c, n)
+    assert_close(got, want.cpu(), ((most + 2) * wide_half_step(t) * size + rounding(t, want)).cpu())
+    assert k().lookup_gradient(g, c.int(), n, out=got, accumulate=True) is got
+    assert_close(got, 2 * want.cpu(), (2 * ((most + 2) * wide_half_step(t) * size + rounding(t, want)) + 2 * wide_half_step(t) * size + rounding(t, 2 * want)).cpu())
+
+
+@gpu
+@pytest.mark.parametrize("n", [262143, 262144, 300007, 150000001])
+@pytest.mark.parametrize("rows", [3000, 6000, 140001])
+def test_lookup_gradient_of_large_tables(rows, n):
+    """Sorts of two, three and four digits, by comparison, by a cluster and by launches; what no code names is zero."""
+    m = 4 if n < 1000000 else 1
+    g = values((rows, m), F32, 75).cuda()
+    c = torch.from_numpy(np.random.default_rng(76).integers(-5, n + 5, (rows, 1))).cuda()
+    c[:: 7] = n - 1
+    c[3:: 7] = 0
+    got = k().lookup_gradient(g, c, n)
+    named, place = torch.unique(c.flatten(), return_inverse=True)
+    inside = (named >= 0) & (named < n)
+    want, size, most = gradient_by_torch(g, place[:, None], len(named))
+    assert_close(got[named[inside]], want[inside].cpu(), ((most + 2) * 2.0 ** -24 * size + rounding(F32, want))[inside].cpu())
+    got[named[inside]] = 0
+    assert not got.any()
+
+
+@gpu
 def test_lookup_gradient_against_differences():
     """The derivative of a weighted sum of lookups, by central differences in float64: the operator is linear, so they are
     off by rounding alone (a dozen terms, steps of one)."""
@@ -414,6 +447,46 @@ def test_sample_with_settings_of_each_row(rows, mc):
     every = lambda v: torch.full((rows,), v, device="cuda")   # a number and the same for every row
     assert torch.equal(k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), 0.7, 9, 0.95, 0.01),
                        k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), every(0.7), every(9).int(), every(0.95), every(0.01)))
+
+
+def own_settings(rows, rng):
+    """Settings of every row: temperatures, some of them 0, top-k, some of them none, top-p, min-p."""
+    temperature = torch.from_numpy(rng.uniform(0.2, 2, rows).astype(np.float32))
+    temperature[::5] = 0
+    top_k = torch.from_numpy(rng.integers(-1, 60, rows).astype(np.int32))
+    top_k[1::3] = 0
+    return temperature, top_k, torch.from_numpy(rng.uniform(0.5, 1.1, rows).astype(np.float32)), torch.from_numpy(rng.uniform(0, 0.1, rows).astype(np.float32))
+
+
+@gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("rows,h,mc", [(700, 30, 10), (400, 30, 50), (700, 30, 100), (509, 31, 200), (400, 30, 401), (200, 30, 900)])
+def test_sample_of_more_groups_than_warps(rows, h, mc, t):
+    """A warp takes one hypercolumn after another, and each the settings of its own row."""
+    x = values((rows, h * mc), t, 66, 2.0)
+    rng = np.random.default_rng(67)
+    u = torch.from_numpy(rng.random((rows, h)).astype(np.float32))
+    u[::9] = small_numbers((len(u[::9]), h), 68)
+    how = own_settings(rows, rng)
+    got = k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), *[a.cuda() for a in how])
+    assert torch.equal(got.cpu(), plain_sample_fast(x, h, mc, u, *how))
+    assert torch.equal(k().sample_minicolumns(x.cuda(), h, mc, u.cuda(), top_p=0.9).cpu(), plain_sample_fast(x, h, mc, u, 1.0, 0, 0.9, 0.0))
+
+
+@gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("rows,mc", [(148, 8193), (295, 9001), (160, 20000), (150, 50001), (296, 9001)])
+def test_sample_wide_batches_with_settings_of_each_row(rows, mc, t):
+    """Two blocks to a row, which read their parts from memory (from 296 rows on, one)."""
+    x = values((rows, mc), t, 69, 2.0)
+    x[2::4, ::3] = -math.inf
+    x[3] = -math.inf
+    rng = np.random.default_rng(70)
+    u = torch.from_numpy(rng.random((rows, 1)).astype(np.float32))
+    u[::9] = small_numbers((len(u[::9]), 1), 71)
+    how = own_settings(rows, rng)
+    assert torch.equal(k().sample_minicolumns(x.cuda(), 1, mc, u.cuda(), *[a.cuda() for a in how]).cpu(), plain_sample_fast(x, 1, mc, u, *how))
+    assert torch.equal(k().sample_minicolumns(offset(x), 1, mc, u.cuda(), 1.0, how[1].cuda(), 0.95).cpu(), plain_sample_fast(x, 1, mc, u, 1.0, how[1], 0.95, 0.0))
 
 
 @gpu
@@ -629,6 +702,27 @@ def test_distill_with_long_lists(rows, mc, kept, among, t):
     assert_close(gradient, grad.cpu(), (grad_off + rounding(t, grad)).cpu())
     again, same = call()
     assert torch.equal(loss, again) and torch.equal(gradient, same)
+
+
+@gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("rows,h,mc,kept", [(1009, 80, 10, 3), (1001, 80, 7, 9), (1000, 80, 100, 5), (503, 80, 200, 8), (500, 80, 300, 8), (251, 80, 400, 8), (250, 80, 511, 40)])
+def test_distill_of_more_groups_than_lanes(rows, h, mc, kept, t):
+    """Lanes take one hypercolumn after another, and each the weight of its own row."""
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(mc)
+    x = (torch.randn((rows, h * mc), generator=gen, device="cuda") * 2).to(t)
+    units = torch.randint(0, mc, (rows, h, kept), generator=gen, device="cuda")
+    units[..., 1:][torch.rand(units[..., 1:].shape, generator=gen, device="cuda") < 0.2] = -1
+    teacher = (torch.randn((rows, h, kept), generator=gen, device="cuda") * 2).to(t)
+    weight = torch.rand(rows, generator=gen, device="cuda", dtype=F64).to(F64 if t == F64 else F32) + 0.5
+    weight[::10] = 0
+    loss, gradient = k().distill_gradient(x, h, mc, units, teacher, 2.0, weight)
+    want, grad, loss_off, grad_off = distill_by_torch(x.view(-1, mc), units.view(-1, kept), teacher.view(-1, kept), 2.0)
+    w = weight.double().repeat_interleave(h)
+    assert_close(loss.flatten(), (want * w).cpu(), (loss_off * w).cpu())
+    grad = grad * w[:, None]
+    assert_close(gradient.view(-1, mc), grad.cpu(), (grad_off * w[:, None] + rounding(t, grad)).cpu())
 
 
 @gpu
