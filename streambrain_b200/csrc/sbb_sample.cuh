@@ -54,6 +54,7 @@ struct Settings {
   unsigned top_k;   // n: all
 };
 __host__ __device__ __forceinline__ double inverse(double t) { return t > 1e-300 ? 1 / t : t > 0 ? 1e300 : 1; }
+__device__ __forceinline__ double min_p_of(const Sampling &s, long row) { return s.min_p_rows ? (double)s.min_p_rows[row] : s.min_p; }
 __device__ __forceinline__ Settings settings_of(const Sampling &s, long row, unsigned n) {
   const bool own = s.temperature_rows != nullptr;
   const float t = own ? s.temperature_rows[row] : s.temperature > 0 ? 1 : 0;
@@ -61,7 +62,7 @@ __device__ __forceinline__ Settings settings_of(const Sampling &s, long row, uns
   Settings r;
   r.top_k = k <= 0 || k > (long)n ? n : (unsigned)k;
   r.top_p = s.top_p_rows ? (double)s.top_p_rows[row] : s.top_p;
-  r.min_p = s.min_p_rows ? (double)s.min_p_rows[row] : s.min_p;
+  r.min_p = min_p_of(s, row);
   if (!(t > 0)) r.top_k = 1;
   r.inv_t = own ? inverse((double)t) : s.inv_t;
   return r;
@@ -117,8 +118,9 @@ struct Weights {
 // weights, lies from 2^(q-1) to 2^q: sums up to it are exact to n 2^-q of it, and a weight that is cut off passes it by itself.
 // For 0 (and what is below, and NaN) it is the first unit whose weight is above 0 in 64 bits.
 // Small is below 2^-20: other numbers pass what weights below 2^-q may add up to, and so few draws are small that the microseconds
-// they take longer are hardly met (with 2^-12, 40960 groups of 256 float32 units took 55 us and not 53).  They have functions of their
-// own, which take few registers from the others.
+// they take longer are hardly met (with 2^-12, 40960 groups of 256 float32 units took 55 us and not 53).  What draws them is kept short,
+// so that it takes few registers from the others: a call to a function of its own at the end of a block's draw cost 4000 groups of 8192
+// float32 units with a top-p 316 us and not 309, and 256 x 128000 bf16 with settings of each row 2 %.
 __device__ __forceinline__ bool is_small(float random) { return !(random >= 1.f / (1 << 20)); }
 struct Lift {
   int lift;
@@ -1326,27 +1328,6 @@ struct Part : Shape<THREADS> {
   }
 };
 
-// Part::locate of the units that are kept, for a small random number.
-template <typename T, bool STAGED, int THREADS>
-__device__ __noinline__ void locate_small(const Vec<T, 16 / (int)sizeof(T)> *x, unsigned begin, unsigned size, unsigned lead, unsigned vectors,
-                                          Block<THREADS> &s, int turn, Wide<T> best, double inv_t, int q, double min_p, float random,
-                                          typename Keys<Wide<T>>::type cut_key, unsigned cut_index) {
-  using W = Wide<T>;
-  Part<T, STAGED, THREADS> p(x, begin, size, lead, vectors, s, cg::this_cluster());
-  p.best = best;
-  p.turn = turn;
-  const Weights weights(s.table, inv_t, q);
-  const W value = cut_key ? Keys<W>::value(cut_key) : (W)-INFINITY;
-  auto weigh = [&](W v, unsigned i, int lift) -> u64 {
-    const bool in = (v > value || (v == value && i <= cut_index)) && weights.reaches(v, best, min_p);
-    return in ? weights.lifted(v, best, lift) : 0;
-  };
-  u64 total = 0;
-  p.each([&](W v, unsigned i) { total += weigh(v, i, 0); });
-  const Lift small(random, p.cluster_sum(p.block_sum(total, s.sum)), q);
-  p.locate(value, [&](W v, unsigned i) { return weigh(v, i, small.lift); }, [&](u64) { return small.target; });
-}
-
 // Few groups are bound by latency, the barriers of a block and its cluster: one of 32000 float16 units, top-k 50 and top-p 0.9, 12 us.
 // Many by instructions on every unit: 256 x 128000 bf16 with a top-k of 100 33 us (greedy 14, the support at the copy bandwidth 10), with
 // settings of each row, some without a top-k, 113.
@@ -1473,17 +1454,35 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       }
     }
     const W value = cut.key ? Keys<W>::value(cut.key) : (W)-INFINITY;
-    if (is_small(random[g]))
-      locate_small<T, STAGED, THREADS>(p.x, begin, size, lead, vectors, s, p.turn, best, set.inv_t, q, set.min_p, random[g], cut.key, cut.index);
-    else
-      p.locate(
-          value,
-          [&](W v, unsigned i) -> u64 {
-            if (!(v > value || (v == value && i <= cut.index))) return 0;
-            const u64 m = weights.of(v, best);
-            return m >= least ? m : 0;
-          },
-          [&](u64 total) { return target_of(random[g], total); });
+    p.locate(
+        value,
+        [&](W v, unsigned i) -> u64 {
+          if (!(v > value || (v == value && i <= cut.index))) return 0;
+          const u64 m = weights.of(v, best);
+          return m >= least ? m : 0;
+        },
+        [&](u64 total) {
+          if (!is_small(random[g])) return target_of(random[g], total);
+          s.sorted_mass[0] = total;   // (the same from every thread)
+          return ~0ull;
+        });
+    // A small random number's: from the front, by the first block alone.  (Most are found in the first units.)
+    if (rank == 0 && is_small(random[g])) {
+      __syncthreads();
+      const Lift small(random[g], s.sorted_mass[0], q);
+      const T *const group = support + (long)g * n;
+      u64 before = 0;
+#pragma unroll 1
+      for (unsigned i0 = 0; i0 < n; i0 += kThreads) {   // (the largest passes what is looked for)
+        const unsigned i = i0 + threadIdx.x;
+        const W v = i < n ? no_nan(widen(group[i])) : (W)-INFINITY;
+        const bool in = (v > value || (v == value && i <= cut.index)) && weights.reaches(v, best, min_p_of(how, g / H));
+        const u64 m = in ? weights.lifted(v, best, small.lift) : 0, run = before + p.block_before(m, s.sum);
+        if (run <= small.target && small.target < run + m) s.unit = i;
+        before += p.block_sum(m, s.sum);
+        if (before > small.target) break;
+      }
+    }
   }
   cluster.sync();
   if (rank == 0 && threadIdx.x == 0) codes[g] = base + (long long)s.unit;

@@ -189,7 +189,8 @@ def distill_loss(support, hypercolumns, minicolumns, teacher_units, teacher_supp
     teacher keeps, counted within the hypercolumn (entries out of range are absent, a unit named twice has both parts), and
     ``teacher_support`` their support, of the student's dtype.  With ``p`` the softmax of the kept units and ``q`` that of all
     of the student's, both at ``temperature``: ``loss = weight * temperature**2 * sum_k p_k (log p_k - log q_{unit_k})``.
-    ``weight`` [rows] (float32, float64 for float64; default 1).  ``temperature`` is from 1e-15 to 1e15.  The loss is exactly 0 where the weight is, where nothing is
+    ``weight`` [rows] (float32, float64 for float64; default 1).  ``temperature`` is from 1e-15 to 1e15.  In 32 bits an exponential
+    ``e**-x`` is off by ``2**-22 + 3 * x * 2**-24`` of itself.  The loss is exactly 0 where the weight is, where nothing is
     kept, and where a hypercolumn of the student or of the teacher is at -infinity throughout; elsewhere NaN where the hypercolumn of
     either holds a NaN or +infinity."""
     return _distill(support, hypercolumns, minicolumns, teacher_units, teacher_support, temperature, weight, False)[0]
