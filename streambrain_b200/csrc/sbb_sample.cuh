@@ -1479,7 +1479,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
         const bool in = (v > value || (v == value && i <= cut.index)) && weights.reaches(v, best, min_p_of(how, g / H));
         const u64 m = in ? weights.lifted(v, best, small.lift) : 0, run = before + p.block_before(m, s.sum);
         if (run <= small.target && small.target < run + m) s.unit = i;
-        before += p.block_sum(m, s.sum);
+        for (int w = 0; w < P::kBlockWarps; ++w) before += s.sum[w];   // (the warps' sums, from block_before)
         if (before > small.target) break;
       }
     }

@@ -550,6 +550,24 @@ def test_sample_small_random_numbers(rows, h, mc, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("rows,mc", [(2, 200001), (150, 20001), (9, 700)])
+def test_sample_small_random_numbers_behind_a_mask(rows, mc, t):
+    """The first unit that may be drawn stands far behind: those in front are masked, or too light for 64 bits."""
+    x = values((rows, mc), t, 64, 2.0)
+    x[:, :mc // 3] = -math.inf
+    x[:, mc // 3:mc // 2] -= 2000
+    x[0, :mc - 1] = -math.inf
+    u = torch.zeros((rows, 1))
+    u[1::2] = 1e-30
+    for how in (dict(), dict(top_k=mc - 5), dict(min_p=1e-3)):
+        how = {**dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **how}
+        got = k().sample_minicolumns(x.cuda(), 1, mc, u.cuda(), **how).cpu()
+        assert torch.equal(got, plain_sample_fast(x, 1, mc, u, **how)), how
+        assert int(got[0]) == mc - 1
+
+
+@gpu
 @pytest.mark.parametrize("t", [F32, F16, BF16])
 @pytest.mark.parametrize("mc", [32, 61, 127, 256, 512, 1000, 1024])
 def test_sample_random_numbers_at_the_borders(mc, t):
