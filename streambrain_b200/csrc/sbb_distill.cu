@@ -336,9 +336,10 @@ __device__ __forceinline__ void block_join(Running<W> &r, Running<W> &t, W c, Bl
 
 // STAGED: the part waits in shared memory between the sum and the gradient; else (no gradient, or groups beyond what a cluster
 // holds) it is read again.  LONG: there is a gradient and a list of more entries than threads; `room` units' parts of it fit the shared
-// memory.  (Within the kernel for short lists, 512 x 50001 float16 took 34.5 us and not 33, without a gradient 20 and not 18.5.)  VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last
-// one by single threads; else (support and gradient lie differently to the boundaries) element by element.
-// Instructions, and phases that do not overlap within a block, bound it: 4096 x 32000 bf16 units, 64 kept, 114 us, 71 % of the issue slots
+// memory.  (Within the kernel for short lists, 512 x 50001 float16 took 34.5 us and not 33, without a gradient 20 and not 18.5.)
+// VECTOR: 16-byte accesses from the first boundary on, the elements in front of it and behind the last one by single threads; else
+// (support and gradient lie differently to the boundaries) element by element.
+// Instructions, and phases that do not overlap within a block, bound it: 4096 x 32000 bf16 units, 64 kept, 114 us, 62 % of the issue slots
 // busy, 0.70 of a plain copy's bandwidth.
 template <typename T, bool VECTOR, bool STAGED, int THREADS, bool LONG>
 __global__ void __launch_bounds__(THREADS, 1536 / THREADS) distill_block_kernel(const Distill<T> p, unsigned part, unsigned room) {

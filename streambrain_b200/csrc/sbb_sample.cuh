@@ -634,7 +634,7 @@ __device__ __forceinline__ int draw_quickly(QuickGroup<EACH> &g, unsigned n, con
   return (int)__shfl_sync(0xffffffffu, unit, who & 31);
 }
 
-// Instructions bound it: 122880 groups of 100 float32 units with a top-p of 0.9 87 us, 600 instructions a group, 78 % of the issue slots busy
+// Instructions bound it: 122880 groups of 100 float32 units with a top-p of 0.9 87 us, 600 instructions a group, 80 % of the issue slots busy
 // (no top-p 41 us, greedy 24).  All in registers, a warp needs no barrier; a block for a group of 520 took twice as long.
 template <typename T, int EACH>
 __global__ void __launch_bounds__(kWarpThreads, kWarpBlocks<EACH>)
